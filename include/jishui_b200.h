@@ -55,8 +55,9 @@ int64_t jx_launch_count(void);
 /* Device-side status word: non-zero when a kernel abandoned work after a
  * bounded wait expired (code identifies the wait: 101-103 GEMM producer / MMA /
  * epilogue, 301-303 attention producer / MMA / softmax, 501 the staged RMSNorm
- * backward's row copies) or met a bad input (201 token id, 202 target, 401 / 402
- * packed-row column / source). Reads and optionally clears it; synchronises the
+ * backward's row copies, 601-603 shared-prefix attention producer / MMA / softmax)
+ * or met a bad input (201 token id, 202 target, 203 teacher token id, 204 sequence
+ * length of the shared-prefix attention, 401 / 402 packed-row column / source). Reads and optionally clears it; synchronises the
  * current device. */
 int jx_device_status(int* status_out, int clear);
 /* Number of SMs that the persistent kernels (GEMM, attention) launched from the
@@ -207,6 +208,39 @@ int jx_attn_decode(const void* qkv, int64_t ld_qkv, void* kcache, void* vcache, 
                    int64_t cache_batch_stride, int B, int len, const int* len_dev, int H, int D, float scale,
                    void* workspace, void* out, int64_t ld_out, jx_stream_t stream);
 
+/* The same for a batch whose sequences share a prefix, which is read once for all of them: the new token of
+ * sequence b attends to prefix keys 0 .. prefix_len-1 and to its own keys 0 .. lens[b]-1, of which the last is
+ * its own k / v, appended to the cache at lens[b]-1. qkv rows are q (H heads) | k (Hkv) | v (Hkv); H must be a
+ * multiple of Hkv (at most 64 times), query head h reads key / value head h / (H / Hkv). kprefix / vprefix:
+ * [prefix_len, Hkv*64], row stride ld_prefix (prefix_len may be 0); kcache / vcache: row stride ld_cache, sequence
+ * stride cache_batch_stride, room for max_len rows per sequence. lens: device int32 [B]; 0 or less marks an idle
+ * sequence (its output row is zero, its cache untouched), more than max_len does too and sets the device status
+ * word to 204. Cache rows at and past lens[b] are never used and, but for the appended one, never written.
+ * workspace: caller scratch of jx_attn_decode_prefix_workspace_bytes (-1 for a bad shape), with the same sizes;
+ * calls that may overlap need their own. head_dim must be 64. Results repeat bit for bit. */
+int64_t jx_attn_decode_prefix_workspace_bytes(int B, int H, int Hkv, int64_t prefix_len, int64_t max_len);
+int jx_attn_decode_prefix(const void* qkv, int64_t ld_qkv, const void* kprefix, const void* vprefix, int64_t ld_prefix,
+                          int64_t prefix_len, void* kcache, void* vcache, int64_t ld_cache, int64_t cache_batch_stride,
+                          const int32_t* lens, int64_t max_len, int B, int H, int Hkv, int D, float scale,
+                          void* workspace, void* out, int64_t ld_out, jx_stream_t stream);
+
+/* ---- Next tokens from f16 logits (generate_torch.py:278-345 draws on the host) ----
+ * Row r: with T = temperature, e_i = exp((x_i - max x) / T), values ranked larger first and, among equal ones,
+ * lower index first: top_k keeps the first top_k ranks (<= 0 or >= vocab: all), top_p the fewest of those whose e
+ * reach top_p of their sum (>= 1: all), min_p those with e_i >= min_p (<= 0: all); the first rank always stays. The
+ * token is the first index at which the running sum, in index order, of the kept e exceeds uniforms[r] times their
+ * whole sum; uniforms f32 in [0, 1). T <= 0 takes the lowest index of the maximum. Each setting is one value for
+ * all rows or, where its pointer is not NULL, a device array of one per row. tokens int64 [rows]; logprobs f32
+ * [rows] (may be NULL): log of the token's share of the kept sum. A row with a NaN, or whose logits are all -inf,
+ * gives token -1 and a NaN. Probabilities are held in 64 bits and results repeat bit for bit. vocab <= 2^20. */
+int jx_sample(const void* logits16, int64_t rows, int vocab, int64_t ld, const float* uniforms,
+              const float* temperatures, float temperature, const int32_t* top_ks, int top_k, const float* top_ps,
+              float top_p, const float* min_ps, float min_p, int64_t* tokens, float* logprobs, jx_stream_t stream);
+/* The k largest logits of each row in the same ranking (NaN last): values16 f16 [rows, k], ids int64 [rows, k].
+ * k <= min(vocab, 1024). */
+int jx_top_logits(const void* logits16, int64_t rows, int vocab, int64_t ld, int k, void* values16, int64_t* ids,
+                  jx_stream_t stream);
+
 /* ---- Packed corpus rows (data.py:233-379 row filling, pretrain_torch.py:38-40 widening) ----
  * out: int64 [rows, width]. Row r is covered by runs[row_start[r] .. row_start[r+1]) (int64 triples
  * dst column, src token index into `tokens` (uint16 [ntokens]) or -(eod + 1), count), sorted by dst.
@@ -240,6 +274,30 @@ int jx_ce_loss(const float* row_loss, const int64_t* targets, int64_t ignore_ind
  * incoming gradient of the loss. */
 int jx_ce_bwd(void* logits16, int64_t rows, int vocab, int64_t ld, const int64_t* targets, int64_t ignore_index,
               const float* lse, const float* grad_loss, const float* count, jx_stream_t stream);
+
+/* ---- Distillation from a teacher's top logits ----
+ * Row r has student logits z, K teacher slots (token id, teacher logit t) and a target y. With p the softmax of
+ * t / temperature over the used slots (id >= 0), q = softmax(z / temperature), q1 = softmax(z):
+ *   row_loss = alpha temperature^2 sum_k p_k (log p_k - log q[id_k]) + (1 - alpha) (-log q1[y]).
+ * Slots naming the same id count as separate entries of that sum. A slot with t = -inf has no weight; a row
+ * without a weighted slot has no first term. Rows with y == ignore_index give loss 0. A target outside
+ * [0, vocab) that is not ignore_index gives a NaN loss and status 202, an id >= vocab a NaN loss and status 203.
+ * teacher_logits: [rows, K], f16 or f32 (teacher_is_f16). stats: f32 [3, rows], the log-sum-exp of z / temperature,
+ * of z (where alpha < 1) and of the used t / temperature, for the backward. parts (may be NULL): the block
+ * statistics that jx_gemm_f16_ce_parts left for these logits; with them the log-sum-exp of z is merged from
+ * there, and at temperature 1 the logits are read only at the slots and the target. The mean over the counted
+ * rows is jx_ce_loss of row_loss. K in [1, 1024], temperature in [0.001, 1000], alpha in [0, 1]. */
+int jx_distill_fwd(const void* logits16, int64_t rows, int vocab, int64_t ld, const int64_t* teacher_ids,
+                   const void* teacher_logits, int teacher_is_f16, int K, const int64_t* targets, int64_t ignore_index,
+                   float temperature, float alpha, const void* parts, float* stats, float* row_loss,
+                   jx_stream_t stream);
+/* out16 = f16(g (alpha temperature (q_j - sum_{k: id_k = j} p_k) + (1 - alpha) (q1_j - [j = y]))) with
+ * g = (*grad_loss) / (*count); zero rows where the target is ignored or invalid. out16 may be logits16 (with the
+ * same row stride), but not overlap it otherwise. */
+int jx_distill_bwd(const void* logits16, int64_t rows, int vocab, int64_t ld, const int64_t* teacher_ids,
+                   const void* teacher_logits, int teacher_is_f16, int K, const int64_t* targets, int64_t ignore_index,
+                   float temperature, float alpha, const float* stats, const float* grad_loss, const float* count,
+                   void* out16, int64_t ld_out, jx_stream_t stream);
 
 /* ---- GradScaler unscale + inf check + global norm, then AdamW ----
  * Stats over a flat gradient buffer (grad_is_f16 selects f16 or f32 input):

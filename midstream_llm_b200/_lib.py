@@ -28,6 +28,11 @@ _SIGNATURES: dict[str, tuple] = {
     "jx_attn_decode_workspace_bytes": (c_int64, [c_int, c_int, c_int]),
     "jx_attn_decode": (c_int, [_P, c_int64, _P, _P, c_int64, c_int64, c_int, c_int, _P, c_int, c_int, c_float, _P,
                                _P, c_int64, _P]),
+    "jx_attn_decode_prefix_workspace_bytes": (c_int64, [c_int, c_int, c_int, c_int64, c_int64]),
+    "jx_attn_decode_prefix": (c_int, [_P, c_int64, _P, _P, c_int64, c_int64, _P, _P, c_int64, c_int64, _P, c_int64, c_int,
+                                      c_int, c_int, c_int, c_float, _P, _P, c_int64, _P]),
+    "jx_sample": (c_int, [_P, c_int64, c_int, c_int64, _P, _P, c_float, _P, c_int, _P, c_float, _P, c_float, _P, _P, _P]),
+    "jx_top_logits": (c_int, [_P, c_int64, c_int, c_int64, c_int, _P, _P, _P]),
     "jx_pack_rows": (c_int, [_P, c_int64, _P, _P, c_int, c_int, _P, _P]),
     "jx_rmsnorm_bwd_noalloc": (c_int, [_P, _P, _P, _P, _P, _P, _P, c_int, c_int64, c_int, _P]),
     "jx_embed_fwd": (c_int, [_P, c_int64, _P, c_int64, c_int, _P, _P]),
@@ -49,6 +54,10 @@ _SIGNATURES: dict[str, tuple] = {
     "jx_ce_fwd_parts": (c_int, [_P, c_int, _P, c_int64, c_int, c_int64, _P, c_int64, _P, _P, _P]),
     "jx_ce_loss": (c_int, [_P, _P, c_int64, c_int64, _P, c_int, _P]),
     "jx_ce_bwd": (c_int, [_P, c_int64, c_int, c_int64, _P, c_int64, _P, _P, _P, _P]),
+    "jx_distill_fwd": (c_int, [_P, c_int64, c_int, c_int64, _P, _P, c_int, c_int, _P, c_int64, c_float, c_float, _P, _P,
+                               _P, _P]),
+    "jx_distill_bwd": (c_int, [_P, c_int64, c_int, c_int64, _P, _P, c_int, c_int, _P, c_int64, c_float, c_float, _P, _P,
+                               _P, _P, c_int64, _P]),
     "jx_grad_stats_parts": (c_int, [c_int64]),
     "jx_grad_stats": (c_int, [_P, c_int, c_int64, _P, _P, _P, _P, _P]),
     "jx_grad_finalize": (c_int, [_P, c_int, c_float, _P, _P]),

@@ -56,6 +56,8 @@ enum DeviceStatus : int {
   kStatusGemmEpilogueWait = 103,
   kStatusEmbedBadId = 201,
   kStatusCeBadTarget = 202,
+  kStatusDistillBadId = 203,    // a teacher token id past the vocabulary
+  kStatusDecodeBadLength = 204, // a sequence longer than its cache (shared-prefix decoding)
   kStatusNormWait = 501,  // the staged RMSNorm backward's row-copy wait
 };
 
@@ -69,5 +71,10 @@ bool make_tmap_f16(CUtensorMap* map, const void* base, uint64_t inner, uint64_t 
 // The same for fp32 tensors (box_inner * 4 bytes <= swizzle_bytes; 128- or 64-byte swizzle).
 bool make_tmap_f32(CUtensorMap* map, const void* base, uint64_t inner, uint64_t outer, uint64_t ld,
                    uint32_t box_inner, uint32_t box_outer, int swizzle_bytes = 128);
+
+// A 3-D fp16 descriptor with 128-byte swizzle: dims innermost first (box[0] * 2 = 128 bytes), byte strides of
+// the second and third dimension.
+bool make_tmap_f16_3d(CUtensorMap* map, const void* base, const uint64_t dims[3], const uint64_t strides[2],
+                      const uint32_t box[3]);
 
 }  // namespace jx

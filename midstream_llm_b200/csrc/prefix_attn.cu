@@ -1,0 +1,632 @@
+// Single-token attention of a batch whose sequences share a long prefix (head_dim 64).
+//
+// Every sequence's new query attends to the P keys of one shared prefix and to its own keys (of which the last
+// is the new token's, appended here). The reference has no counterpart: it re-runs each whole context
+// (Midstream-LLM src/jishui/generate_torch.py:279-285); decode_attn.cu is the form for caches that share nothing.
+//
+// With G query heads per key / value head, the queries of all sequences at one key / value head are rows of one
+// matrix, so the prefix is read once for up to 128 rows and its scores are matrix products: for every 128 keys
+//   S = Q K^T  (tcgen05, M 128 rows, N 128 keys, K 64, Q and K in shared memory)   -> TMEM
+//   P = exp2(S scale - m) as fp16, with a lazily updated row maximum m             -> TMEM
+//   O += P V   (tcgen05, M 128, N 64, K 128, P from TMEM, V from shared memory)    -> TMEM
+// A sequence's own keys go through the same pipeline with only its G heads as rows: the matrix unit has far
+// more than the time that the 32 KB of a tile take from memory, whatever part of its rows is used.
+//
+// Work: the prefix tiles of all (row tile, key / value head) units stand in one line that is cut into equal runs, one
+// a block, so that each unit is split over a few blocks; the (sequence, head, chunk) items of the own keys
+// follow, dealt round robin. Each part leaves (m, l, o[64]) of its rows in the workspace, the second kernel joins
+// them. The schedule is fixed by the sizes, so results repeat bit for bit.
+//
+// 192 threads, two blocks an SM (256 TMEM columns each):
+//   warp 0    TMA producer: Q of the item, K and V tiles (2 and 3 slots of 16 KB),
+//   warp 1    MMA issuer; before the tile that holds a sequence's end it puts the new key and value into the
+//             tile (and the cache) and clears the values behind them, since 0 * garbage may be NaN,
+//   warps 2-5 softmax, one row per thread, and the parts' output.
+#include <algorithm>
+#include <atomic>
+
+#include "jx_common.cuh"
+#include "jx_host.h"
+
+namespace jx {
+namespace pfx {
+
+constexpr int D = 64;
+constexpr int BKV = 128;
+constexpr int kThreads = 192;
+constexpr uint32_t kTile = BKV * D * 2;  // 16 KiB
+constexpr int kKSlots = 2, kVSlots = 3;
+constexpr int kMaxGroup = 64;
+constexpr int kLens = 1024;  // lengths kept in shared memory
+constexpr uint32_t kTmemCols = 256;  // S [0,128), P (fp16 pairs) [128,192), O [192,256)
+
+enum Status : int { kProducer = 601, kMma = 602, kSoftmax = 603 };
+
+struct Sched {
+  int B, G, Hkv, H;
+  int nb;              // sequences per row tile
+  int P, NT;           // prefix keys and tiles of one unit
+  int T, gp;           // prefix tiles in all, and blocks that share them
+  int max_len, OC;     // own keys: upper bound, tiles per item
+  int pairs, n_own;    // B * Hkv, items
+  int nparts;          // parts a row has room for
+  int nsp;             // of those, for the prefix
+
+  // Block that has prefix tile x: block c has [c T / gp, (c + 1) T / gp).
+  __host__ __device__ int block_of(int x) const { return (int)((((int64_t)x + 1) * gp - 1) / T); }
+};
+
+__device__ __forceinline__ int own_length(const Sched& s, int raw) { return raw > 0 && raw <= s.max_len ? raw : 0; }
+
+// The tiles of one block in order. Every role walks its own copy.
+struct Cursor {
+  int t, t1;    // prefix tiles left
+  int own;      // next item of own keys
+  int b, h;     // first sequence of the row tile, or the sequence; key / value head
+  int key0, n, j, limit;  // first key, tiles, current tile, end of the keys
+  int part, ipre, iown;   // part index; prefix / own items begun before
+  bool is_own;
+
+  __device__ __forceinline__ void init(const Sched& s) {
+    const int c = blockIdx.x;
+    t = t1 = 0;
+    if (c < s.gp) {
+      t = (int)((int64_t)c * s.T / s.gp);
+      t1 = (int)((int64_t)(c + 1) * s.T / s.gp);
+    }
+    own = gridDim.x - 1 - c;  // dealt from the last block on: those may have no prefix tiles
+    ipre = iown = -1;
+  }
+  __device__ __forceinline__ bool next_item(const Sched& s, const int* lens) {
+    j = 0;
+    if (t < t1) {
+      const int unit = t / s.NT, first = t - unit * s.NT;
+      h = unit % s.Hkv;
+      b = unit / s.Hkv * s.nb;
+      n = min(s.NT - first, t1 - t);
+      key0 = first * BKV;
+      limit = s.P;
+      part = (int)blockIdx.x - s.block_of(unit * s.NT);
+      is_own = false;
+      ++ipre;
+      t += n;
+      return true;
+    }
+    while (own < s.n_own) {
+      const int chunk = own / s.pairs, pair = own - chunk * s.pairs;
+      own += gridDim.x;
+      b = pair / s.Hkv;
+      h = pair - b * s.Hkv;
+      limit = own_length(s, lens[b]);
+      key0 = chunk * s.OC * BKV;
+      if (key0 >= limit) continue;
+      n = min(s.OC, (limit - key0 + BKV - 1) / BKV);
+      part = s.nsp + chunk;
+      is_own = true;
+      ++iown;
+      return true;
+    }
+    return false;
+  }
+  __device__ __forceinline__ bool next_tile(const Sched& s, const int* lens) {
+    return ++j < n || next_item(s, lens);
+  }
+  __device__ __forceinline__ int key() const { return key0 + j * BKV; }
+  __device__ __forceinline__ bool ends() const { return is_own && key() + BKV >= limit; }
+};
+
+struct Bars {
+  uint64_t k_full[kKSlots], k_empty[kKSlots], v_full[kVSlots], v_empty[kVSlots];
+  uint64_t q_full[3], q_empty[3];  // own items alternate between 0 and 1, prefix items use 2
+  uint64_t s_full, s_free, p_full, p_empty;
+  uint32_t tmem_base;
+  int abort;
+  int lens[kLens];
+};
+
+__device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* status, int code) {
+  const long long start = clock64();
+  for (uint32_t i = 0;; ++i) {
+    if (mbar_try_wait(bar, parity)) return true;
+    if ((i & 255u) == 255u) {
+      if (*abort_flag) return false;
+      if (clock64() - start > (1ll << 32)) {
+        *abort_flag = 1;
+        if (status) atomicExch(status, code);
+        return false;
+      }
+    }
+  }
+}
+
+// Lane 0 polls, the warp follows.
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* status,
+                                          int code) {
+  int ok = 1;
+  if ((threadIdx.x & 31) == 0) ok = wait(bar, parity, abort_flag, status, code) ? 1 : 0;
+  ok = __shfl_sync(0xffffffffu, ok, 0);
+  __syncwarp();
+  return ok != 0;
+}
+
+__device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, uint64_t* bar, int x, int y, int z) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], "
+      "[%2];" ::"r"(smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z)
+      : "memory");
+}
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+struct Params {
+  Sched s;
+  const __half* qkv;
+  int64_t ld_qkv;
+  __half* kcache;
+  __half* vcache;
+  int64_t ld_cache, batch_stride;
+  const int* lens;
+  float scale_log2;
+  float2* ml;  // [B * H][nparts]
+  float* o;    // [B * H][nparts][64]
+  __half* out;
+  int64_t ld_out;
+  uint32_t q_own_bytes, q_own_stride, q_pre_bytes;
+};
+
+__global__ void __launch_bounds__(kThreads, 2)
+    attn_prefix_part_kernel(const __grid_constant__ CUtensorMap tm_qp, const __grid_constant__ CUtensorMap tm_qo,
+                            const __grid_constant__ CUtensorMap tm_kp, const __grid_constant__ CUtensorMap tm_vp,
+                            const __grid_constant__ CUtensorMap tm_kc, const __grid_constant__ CUtensorMap tm_vc,
+                            const Params p, int* status) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  // Queries of own items (G rows each), of a prefix item, K and V slots. The matrix unit reads 128 rows from each
+  // query tile; behind an own item's G rows it finds other data, whose rows of S nobody reads.
+  uint8_t* sQ[3] = {smem, smem + p.q_own_stride, smem + 2 * p.q_own_stride};
+  uint8_t* sK = sQ[2] + kTile;
+  uint8_t* sV = sK + kKSlots * kTile;
+  Bars* bars = reinterpret_cast<Bars*>(sV + kVSlots * kTile);
+  volatile int* abort_flag = &bars->abort;
+  const Sched& s = p.s;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kKSlots; ++i) mbar_init(&bars->k_full[i], 1), mbar_init(&bars->k_empty[i], 1);
+    for (int i = 0; i < kVSlots; ++i) mbar_init(&bars->v_full[i], 1), mbar_init(&bars->v_empty[i], 1);
+    for (int i = 0; i < 3; ++i) mbar_init(&bars->q_full[i], 1), mbar_init(&bars->q_empty[i], 1);
+    mbar_init(&bars->s_full, 1);
+    mbar_init(&bars->s_free, 4);
+    mbar_init(&bars->p_full, 4);
+    mbar_init(&bars->p_empty, 1);
+    bars->abort = 0;
+    fence_barrier_init();
+  }
+  const bool staged = s.B <= kLens;
+  if (staged)
+    for (int i = threadIdx.x; i < s.B; i += kThreads) bars->lens[i] = p.lens[i];
+  if (warp == 1) {
+    tmem_alloc(&bars->tmem_base, kTmemCols);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = bars->tmem_base;
+  const int* lens = staged ? bars->lens : p.lens;
+  Cursor c;
+  c.init(s);
+
+  if (warp == 0) {
+    if (lane == 0) {
+      uint32_t tile = 0;
+      for (bool more = c.next_item(s, lens); more; more = c.next_tile(s, lens), ++tile) {
+        if (c.j == 0) {
+          const int q = c.is_own ? (c.iown & 1) : 2;
+          const uint32_t use = c.is_own ? (uint32_t)(c.iown >> 1) : (uint32_t)c.ipre;
+          if (!wait(&bars->q_empty[q], (use & 1) ^ 1, abort_flag, status, kProducer)) break;
+          mbar_expect_tx(&bars->q_full[q], c.is_own ? p.q_own_bytes : p.q_pre_bytes);
+          tma_load_3d(sQ[q], c.is_own ? &tm_qo : &tm_qp, &bars->q_full[q], 0, c.h * s.G, c.b);
+        }
+        const uint32_t ks = tile % kKSlots, vs = tile % kVSlots;
+        if (!wait(&bars->k_empty[ks], ((tile / kKSlots) & 1) ^ 1, abort_flag, status, kProducer)) break;
+        mbar_expect_tx(&bars->k_full[ks], kTile);
+        if (c.is_own)
+          tma_load_3d(sK + ks * kTile, &tm_kc, &bars->k_full[ks], c.h * D, c.key(), c.b);
+        else
+          tma_load_2d(sK + ks * kTile, &tm_kp, &bars->k_full[ks], c.h * D, c.key());
+        if (!wait(&bars->v_empty[vs], ((tile / kVSlots) & 1) ^ 1, abort_flag, status, kProducer)) break;
+        mbar_expect_tx(&bars->v_full[vs], kTile);
+        if (c.is_own)
+          tma_load_3d(sV + vs * kTile, &tm_vc, &bars->v_full[vs], c.h * D, c.key(), c.b);
+        else
+          tma_load_2d(sV + vs * kTile, &tm_vp, &bars->v_full[vs], c.h * D, c.key());
+      }
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    constexpr uint32_t idesc_s = idesc_f16_f32(128, BKV, false, false);
+    constexpr uint32_t idesc_o = idesc_f16_f32(128, D, false, true);
+    const uint64_t dK0 = smem_desc_sw128(smem_u32(sK), 16, 1024);
+    const uint64_t dV0 = smem_desc_sw128(smem_u32(sV), 8192, 1024);
+    uint32_t ts = 0, tp = 0;  // S and P V products issued
+    // S of the cursor's tile.
+    auto issue_s = [&]() -> bool {
+      const uint32_t ks = ts % kKSlots, vs = ts % kVSlots;
+      const int q = c.is_own ? (c.iown & 1) : 2;
+      if (c.j == 0) {
+        const uint32_t use = c.is_own ? (uint32_t)(c.iown >> 1) : (uint32_t)c.ipre;
+        if (!warp_wait(&bars->q_full[q], use & 1, abort_flag, status, kMma)) return false;
+      }
+      if (!warp_wait(&bars->k_full[ks], (ts / kKSlots) & 1, abort_flag, status, kMma)) return false;
+      if (c.ends()) {
+        // The sequence ends in this tile: row `last` is the new token's.
+        if (!warp_wait(&bars->v_full[vs], (ts / kVSlots) & 1, abort_flag, status, kMma)) return false;
+        const int last = c.limit - 1 - c.key();
+        const __half* nk = p.qkv + (int64_t)c.b * p.ld_qkv + (s.H + c.h) * D;
+        const __half* nv = nk + s.Hkv * D;
+        const int64_t at = (int64_t)c.b * p.batch_stride + (int64_t)(c.limit - 1) * p.ld_cache + c.h * D;
+        if (lane < 16) {
+          const int ch = lane & 7;
+          const bool is_v = lane >= 8;
+          const uint4 u = *reinterpret_cast<const uint4*>((is_v ? nv : nk) + ch * 8);
+          uint8_t* tile = is_v ? sV + vs * kTile : sK + ks * kTile;
+          *reinterpret_cast<uint4*>(tile + last * 128 + ((ch ^ (last & 7)) << 4)) = u;
+          *reinterpret_cast<uint4*>((is_v ? p.vcache : p.kcache) + at + ch * 8) = u;
+        }
+        for (int i = (last + 1) * 8 + lane; i < BKV * 8; i += 32)
+          *reinterpret_cast<uint4*>(sV + vs * kTile + i * 16) = make_uint4(0, 0, 0, 0);
+        fence_proxy_async_smem();
+        __syncwarp();
+      }
+      if (!warp_wait(&bars->s_free, (ts & 1) ^ 1, abort_flag, status, kMma)) return false;
+      tc_fence_after();
+      if (lane == 0) {
+        const uint64_t a = smem_desc_sw128(smem_u32(sQ[q]), 16, 1024), b = desc_adv(dK0, ks * kTile);
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk)
+          umma_f16(tmem, desc_adv(a, kk * 32), desc_adv(b, kk * 32), idesc_s, kk > 0 ? 1u : 0u);
+        umma_commit(&bars->s_full);
+        umma_commit(&bars->k_empty[ks]);
+        if (c.j == c.n - 1) umma_commit(&bars->q_empty[q]);
+      }
+      __syncwarp();
+      ++ts;
+      return true;
+    };
+    Cursor cp = c;
+    bool more_s = c.next_item(s, lens);
+    bool more_p = cp.next_item(s, lens);
+    bool ok = true;
+    if (more_s) {
+      ok = issue_s();
+      more_s = c.next_tile(s, lens);
+    }
+    while (ok && more_p) {
+      // S of the next tile goes ahead of this tile's P V.
+      if (more_s) {
+        if (!(ok = issue_s())) break;
+        more_s = c.next_tile(s, lens);
+      }
+      const uint32_t vs = tp % kVSlots;
+      if (!(ok = warp_wait(&bars->v_full[vs], (tp / kVSlots) & 1, abort_flag, status, kMma))) break;
+      if (!(ok = warp_wait(&bars->p_full, tp & 1, abort_flag, status, kMma))) break;
+      tc_fence_after();
+      if (lane == 0) {
+        const uint64_t bv = desc_adv(dV0, vs * kTile);
+#pragma unroll
+        for (int kk = 0; kk < BKV / 16; ++kk)
+          umma_f16_ts(tmem + 192, tmem + 128 + kk * 8, desc_adv(bv, kk * 2048), idesc_o, (cp.j > 0 || kk > 0) ? 1u : 0u);
+        umma_commit(&bars->v_empty[vs]);
+        umma_commit(&bars->p_empty);
+      }
+      __syncwarp();
+      ++tp;
+      more_p = cp.next_tile(s, lens);
+    }
+  } else {
+    const int quarter = warp & 3;  // TMEM lanes this warp may access
+    const int r = quarter * 32 + lane;
+    const uint32_t base = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
+    constexpr float kRescaleThreshold = 8.0f;  // log2 units: P stays below 2^8 against a stale maximum
+    uint32_t g = 0;  // tiles consumed
+    bool ok = true;
+    for (bool more = c.next_item(s, lens); more && ok; more = c.next_item(s, lens)) {
+      const int seqs = c.is_own ? 1 : min(s.nb, s.B - c.b);
+      const int rows = seqs * s.G;
+      const bool active = quarter * 32 < rows;
+      float m = 0.f, l = 0.f;
+      for (int j = 0; j < c.n; ++j, ++g) {
+        if (!warp_wait(&bars->s_full, g & 1, abort_flag, status, kSoftmax)) { ok = false; break; }
+        tc_fence_after();
+        const int lim = min(c.limit - c.key0 - j * BKV, BKV);  // keys of this tile
+        float alpha = 1.f;
+        bool rescale = false;
+        if (active) {
+          float mp[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            if (q * 32 >= lim) break;
+            uint32_t sr[32];
+            tmem_ld32(base + q * 32, sr);
+            tmem_ld_wait();
+            if (q * 32 + 32 <= lim) {
+#pragma unroll
+              for (int i = 0; i < 32; ++i) mp[i & 3] = fmaxf(mp[i & 3], __uint_as_float(sr[i]));
+            } else {
+#pragma unroll
+              for (int i = 0; i < 32; ++i) mp[i & 3] = fmaxf(mp[i & 3], q * 32 + i < lim ? __uint_as_float(sr[i]) : -INFINITY);
+            }
+          }
+          const float mx = fmaxf(fmaxf(mp[0], mp[1]), fmaxf(mp[2], mp[3])) * p.scale_log2;
+          if (j == 0) {
+            m = mx;
+          } else if (mx > m + kRescaleThreshold) {
+            alpha = ex2(m - mx);
+            m = mx;
+            rescale = true;
+          }
+        }
+        // P V of the tile before must be done before P is overwritten or O rescaled.
+        if (g > 0 && !warp_wait(&bars->p_empty, (g - 1) & 1, abort_flag, status, kSoftmax)) { ok = false; break; }
+        tc_fence_after();
+        if (active) {
+          float sum[4] = {0.f, 0.f, 0.f, 0.f};
+          const float neg_m = -m;
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            uint32_t pw[16];
+            if (q * 32 >= lim) {
+#pragma unroll
+              for (int e = 0; e < 16; ++e) pw[e] = 0;
+            } else {
+              uint32_t sr[32];
+              tmem_ld32(base + q * 32, sr);
+              tmem_ld_wait();
+#pragma unroll
+              for (int e = 0; e < 16; ++e) {
+                float p0 = ex2(fmaf(__uint_as_float(sr[2 * e]), p.scale_log2, neg_m));
+                float p1 = ex2(fmaf(__uint_as_float(sr[2 * e + 1]), p.scale_log2, neg_m));
+                if (q * 32 + 32 > lim) {
+                  if (q * 32 + 2 * e >= lim) p0 = 0.f;
+                  if (q * 32 + 2 * e + 1 >= lim) p1 = 0.f;
+                }
+                sum[(2 * e) & 3] += p0;
+                sum[(2 * e + 1) & 3] += p1;
+                const __half2 hp = __floats2half2_rn(p0, p1);
+                pw[e] = *reinterpret_cast<const uint32_t*>(&hp);
+              }
+            }
+            tmem_st16(base + 128 + q * 16, pw);
+          }
+          if (__any_sync(0xffffffffu, rescale)) {
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+              uint32_t orr[32];
+              tmem_ld32(base + 192 + q * 32, orr);
+              tmem_ld_wait();
+#pragma unroll
+              for (int i = 0; i < 32; ++i) orr[i] = __float_as_uint(__uint_as_float(orr[i]) * alpha);
+              tmem_st32(base + 192 + q * 32, orr);
+            }
+          }
+          l = l * alpha + ((sum[0] + sum[1]) + (sum[2] + sum[3]));
+          tmem_st_wait();
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(&bars->s_free);
+          mbar_arrive(&bars->p_full);
+        }
+      }
+      if (!ok || !warp_wait(&bars->p_empty, (g - 1) & 1, abort_flag, status, kSoftmax)) break;
+      tc_fence_after();
+      if (active) {
+        uint32_t orr[64];
+        tmem_ld32(base + 192, *reinterpret_cast<uint32_t(*)[32]>(&orr[0]));
+        tmem_ld32(base + 224, *reinterpret_cast<uint32_t(*)[32]>(&orr[32]));
+        tmem_ld_wait();
+        if (r < rows) {
+          const int sq = r / s.G;
+          const int64_t at = ((int64_t)(c.b + sq) * s.H + c.h * s.G + (r - sq * s.G)) * s.nparts + c.part;
+          p.ml[at] = make_float2(m, l);
+          float4* dst = reinterpret_cast<float4*>(p.o + at * D);
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            dst[i] = make_float4(__uint_as_float(orr[4 * i]), __uint_as_float(orr[4 * i + 1]),
+                                 __uint_as_float(orr[4 * i + 2]), __uint_as_float(orr[4 * i + 3]));
+        }
+      }
+      // The next item's first P V waits for this warp's next arrival at p_full, after these reads.
+      tc_fence_before();
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, kTmemCols);
+  }
+}
+
+// out[b][h*64 + c] = f16(sum_s o_s[c] 2^(m_s - M) / sum_s l_s 2^(m_s - M)) over the row's parts; zeros for an idle
+// sequence. One block of 128 threads per row: warp w takes parts w, w + 4, ..., a lane two columns.
+__global__ void __launch_bounds__(128) attn_prefix_join_kernel(const Params p, int* status) {
+  __shared__ float2 wacc[4][32];
+  __shared__ float wm[4], wl[4];
+  const Sched& s = p.s;
+  const int row = blockIdx.x, b = row / s.H, hq = row - b * s.H;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int raw = p.lens[b], len = own_length(s, raw);
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  __half2* dst = reinterpret_cast<__half2*>(p.out + (int64_t)b * p.ld_out + hq * D);
+  if (len == 0) {
+    if (raw > s.max_len && threadIdx.x == 0 && hq == 0 && status) atomicExch(status, kStatusDecodeBadLength);
+    if (warp == 0) dst[lane] = __floats2half2_rn(0.f, 0.f);
+    return;
+  }
+  int npre = 0;
+  if (s.T > 0) {
+    const int unit = b / s.nb * s.Hkv + hq / s.G;
+    npre = s.block_of(unit * s.NT + s.NT - 1) - s.block_of(unit * s.NT) + 1;
+  }
+  const int nown = ((len + BKV - 1) / BKV + s.OC - 1) / s.OC, n = npre + nown;
+  const float2* ml = p.ml + (int64_t)row * s.nparts;
+  const float* o = p.o + (int64_t)row * s.nparts * D;
+  float M = -INFINITY, L = 0.f;
+  float2 acc = make_float2(0.f, 0.f);
+#pragma unroll 4
+  for (int i = warp; i < n; i += 4) {
+    const int part = i < npre ? i : s.nsp + i - npre;
+    const float2 q = ml[part];
+    const float2 v = *reinterpret_cast<const float2*>(o + (int64_t)part * D + 2 * lane);
+    const float nm = fmaxf(M, q.x);
+    const float a = M == -INFINITY ? 0.f : ex2(M - nm), w = ex2(q.x - nm);
+    L = L * a + q.y * w;
+    acc.x = acc.x * a + v.x * w;
+    acc.y = acc.y * a + v.y * w;
+    M = nm;
+  }
+  if (lane == 0) wm[warp] = M, wl[warp] = L;
+  wacc[warp][lane] = acc;
+  __syncthreads();
+  if (warp != 0) return;
+  float gm = fmaxf(fmaxf(wm[0], wm[1]), fmaxf(wm[2], wm[3]));
+  L = 0.f, acc = make_float2(0.f, 0.f);
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    if (wl[w] == 0.f) continue;  // no part
+    const float a = ex2(wm[w] - gm);
+    L += wl[w] * a;
+    acc.x += wacc[w][lane].x * a;
+    acc.y += wacc[w][lane].y * a;
+  }
+  dst[lane] = __floats2half2_rn(acc.x / L, acc.y / L);
+}
+
+// The schedule, from sizes and the SM count alone.
+bool plan(int B, int H, int Hkv, int64_t prefix_len, int64_t max_len, Sched* s, int* grid) {
+  if (B <= 0 || Hkv <= 0 || H <= 0 || H % Hkv || H / Hkv > kMaxGroup || prefix_len < 0 || max_len <= 0) return false;
+  if (prefix_len > (1 << 28) || max_len > (1 << 28) || (int64_t)B * H > (1 << 24)) return false;
+  const int blocks = 2 * num_sms();
+  s->B = B, s->H = H, s->Hkv = Hkv, s->G = H / Hkv;
+  s->nb = std::min(128 / s->G, B);
+  s->P = (int)prefix_len;
+  s->NT = (s->P + BKV - 1) / BKV;
+  const int64_t T = (int64_t)((B + s->nb - 1) / s->nb) * Hkv * s->NT;
+  const int own_tiles = (int)((max_len + BKV - 1) / BKV);
+  const int64_t own_all = (int64_t)B * Hkv * own_tiles;
+  if (T >= (1ll << 31) || own_all >= (1ll << 31)) return false;
+  s->T = (int)T;
+  s->gp = (int)std::min<int64_t>(T, blocks);
+  s->max_len = (int)max_len;
+  // Enough items to even out ragged lengths, few parts to join.
+  s->OC = (int)std::max<int64_t>(1, (own_all + 3 * blocks - 1) / (3 * blocks));
+  s->OC = std::min(s->OC, own_tiles);
+  const int chunks = (own_tiles + s->OC - 1) / s->OC;
+  s->pairs = B * Hkv;
+  s->n_own = s->pairs * chunks;
+  s->nsp = T > 0 ? (int)std::min<int64_t>(s->NT, ((int64_t)s->NT * s->gp + T - 1) / T + 1) : 0;
+  s->nparts = s->nsp + chunks;
+  *grid = (int)std::min<int64_t>(blocks, std::max<int64_t>(s->gp, T + s->n_own));
+  return true;
+}
+
+int64_t ml_bytes(const Sched& s) { return ((int64_t)s.B * s.H * s.nparts * 8 + 255) / 256 * 256; }
+
+}  // namespace pfx
+}  // namespace jx
+
+using namespace jx;
+
+extern "C" int64_t jx_attn_decode_prefix_workspace_bytes(int B, int H, int Hkv, int64_t prefix_len, int64_t max_len) {
+  pfx::Sched s;
+  int grid;
+  if (!pfx::plan(B, H, Hkv, prefix_len, max_len, &s, &grid)) return -1;
+  return pfx::ml_bytes(s) + (int64_t)B * H * s.nparts * pfx::D * 4;
+}
+
+extern "C" int jx_attn_decode_prefix(const void* qkv, int64_t ld_qkv, const void* kprefix, const void* vprefix,
+                                     int64_t ld_prefix, int64_t prefix_len, void* kcache, void* vcache, int64_t ld_cache,
+                                     int64_t cache_batch_stride, const int32_t* lens, int64_t max_len, int B, int H,
+                                     int Hkv, int Dh, float scale, void* workspace, void* out, int64_t ld_out,
+                                     jx_stream_t stream) {
+  const char* name = "jx_attn_decode_prefix";
+  JX_CHECK_ARG(Dh == 64, "%s: head_dim must be 64 (got %d)", name, Dh);
+  JX_CHECK_ARG(qkv && kcache && vcache && lens && workspace && out && (prefix_len == 0 || (kprefix && vprefix)),
+               "%s: NULL argument", name);
+  pfx::Params p{};
+  int grid;
+  JX_CHECK_ARG(pfx::plan(B, H, Hkv, prefix_len, max_len, &p.s, &grid),
+               "%s: bad shape B %d, H %d, Hkv %d (at most %d query heads per key head), prefix %lld, max_len %lld", name, B, H,
+               Hkv, pfx::kMaxGroup, (long long)prefix_len, (long long)max_len);
+  const int G = p.s.G, width = (H + 2 * Hkv) * 64;
+  JX_CHECK_ARG(aligned16(qkv) && aligned16(kcache) && aligned16(vcache) && aligned16(workspace) &&
+                   aligned16(kprefix) && aligned16(vprefix) && ((uintptr_t)out & 3) == 0,
+               "%s: operands must be 16-byte aligned", name);
+  JX_CHECK_ARG(ld_qkv % 8 == 0 && ld_qkv >= width && ld_out % 2 == 0 && ld_out >= H * 64 && ld_cache % 8 == 0 &&
+                   ld_cache >= Hkv * 64 && cache_batch_stride % 8 == 0 && cache_batch_stride >= 0 &&
+                   (prefix_len == 0 || (ld_prefix % 8 == 0 && ld_prefix >= Hkv * 64)),
+               "%s: row strides must be multiples of 8 and hold a row", name);
+  // Queries as [sequence][head][64]: one box holds G heads of one sequence, or of a row tile's sequences.
+  CUtensorMap qp, qo, kp, vp, kc, vc;
+  const uint64_t qdims[3] = {64, (uint64_t)H, (uint64_t)B}, qstr[2] = {128, (uint64_t)ld_qkv * 2};
+  const uint32_t qob[3] = {64, (uint32_t)G, 1}, qpb[3] = {64, (uint32_t)G, (uint32_t)p.s.nb};
+  const uint64_t cdims[3] = {(uint64_t)Hkv * 64, (uint64_t)max_len, (uint64_t)B};
+  const uint64_t cstr[2] = {(uint64_t)ld_cache * 2, (uint64_t)(B > 1 ? cache_batch_stride : ld_cache) * 2};
+  const uint32_t cbox[3] = {64, 128, 1};
+  bool ok = make_tmap_f16_3d(&qo, qkv, qdims, qstr, qob) && make_tmap_f16_3d(&qp, qkv, qdims, qstr, qpb) &&
+            make_tmap_f16_3d(&kc, kcache, cdims, cstr, cbox) && make_tmap_f16_3d(&vc, vcache, cdims, cstr, cbox);
+  kp = kc, vp = vc;
+  if (ok && prefix_len > 0)
+    ok = make_tmap_f16(&kp, kprefix, (uint64_t)Hkv * 64, prefix_len, ld_prefix, 64, 128) &&
+         make_tmap_f16(&vp, vprefix, (uint64_t)Hkv * 64, prefix_len, ld_prefix, 64, 128);
+  JX_CHECK_ARG(ok, "%s: cannot encode a TMA descriptor", name);
+  p.qkv = static_cast<const __half*>(qkv);
+  p.ld_qkv = ld_qkv;
+  p.kcache = static_cast<__half*>(kcache);
+  p.vcache = static_cast<__half*>(vcache);
+  p.ld_cache = ld_cache;
+  p.batch_stride = cache_batch_stride;
+  p.lens = lens;
+  p.scale_log2 = scale * 1.4426950408889634f;
+  p.ml = static_cast<float2*>(workspace);
+  p.o = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + pfx::ml_bytes(p.s));
+  p.out = static_cast<__half*>(out);
+  p.ld_out = ld_out;
+  p.q_own_bytes = G * 128;
+  p.q_own_stride = (G + 7) / 8 * 1024;
+  p.q_pre_bytes = p.s.nb * G * 128;
+  const size_t smem = 1024 + 2 * p.q_own_stride + (1 + pfx::kKSlots + pfx::kVSlots) * pfx::kTile + sizeof(pfx::Bars);
+  static std::atomic<uint64_t> done{0};
+  JX_CUDA_TRY(once_per_device(done,
+                              [] {
+                                return cudaFuncSetAttribute(pfx::attn_prefix_part_kernel,
+                                                            cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                            1024 + 2 * 8192 + 6 * pfx::kTile + (int)sizeof(pfx::Bars));
+                              }),
+              name);
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  int* status = status_ptr();
+  pfx::attn_prefix_part_kernel<<<grid, pfx::kThreads, smem, st>>>(qp, qo, kp, vp, kc, vc, p, status);
+  JX_CHECK_LAUNCH(name);
+  // The join kernel's blocks may start while the last parts are written; they wait before they read them.
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(B * H);
+  cfg.blockDim = dim3(128);
+  cfg.stream = st;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  JX_CUDA_TRY(cudaLaunchKernelEx(&cfg, pfx::attn_prefix_join_kernel, p, status), name);
+  JX_CHECK_LAUNCH(name);
+  return JX_OK;
+}

@@ -13,7 +13,7 @@ import torch
 
 from . import _lib
 
-F16, F32, I64 = torch.float16, torch.float32, torch.int64
+F16, F32, I64, I32 = torch.float16, torch.float32, torch.int64, torch.int32
 
 # When set to a list, every GEMM launch appends (algorithmic FLOPs, start event,
 # end event) recorded on the launching stream (used by bench.py's roofline).
@@ -65,6 +65,31 @@ def _check(t: torch.Tensor, dtype: torch.dtype, name: str, contiguous: bool = Tr
         raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
     if contiguous and not t.is_contiguous():
         raise ValueError(f"{name} must be contiguous")
+
+
+def _check_here(**tensors: torch.Tensor | None) -> None:
+    """Every tensor must be on the current device: the launch goes to its current stream."""
+    here = torch.cuda.current_device()
+    for name, t in tensors.items():
+        if t is not None and t.device.index != here:
+            raise ValueError(f"{name} is on {t.device}, the current device is cuda:{here}")
+
+
+def _shape(t: torch.Tensor, shape: tuple, name: str) -> None:
+    if tuple(t.shape) != shape:
+        raise ValueError(f"{name} must have shape {shape}, got {tuple(t.shape)}")
+
+
+def _logit_rows(t: torch.Tensor, name: str) -> tuple[int, int, int]:
+    """(rows, vocab, row stride) of 2-D fp16 logits whose rows start on 16-byte boundaries."""
+    _check(t, F16, name, contiguous=False)
+    if t.dim() != 2 or t.shape[1] < 1 or (t.shape[1] > 1 and t.stride(1) != 1):
+        raise ValueError(f"{name} must be 2-D with unit column stride")
+    rows, vocab = t.shape
+    ld = t.stride(0) if rows > 1 else (vocab + 7) // 8 * 8
+    if ld % 8 or ld < vocab or t.data_ptr() % 16:
+        raise ValueError(f"{name}: rows must start on 16-byte boundaries (row stride {ld})")
+    return rows, vocab, ld
 
 
 # ---------------------------------------------------------------- RMSNorm
@@ -328,6 +353,119 @@ def attn_decode(qkv: torch.Tensor, kcache: torch.Tensor, vcache: torch.Tensor, l
     return o
 
 
+def attn_decode_prefix_workspace_bytes(B: int, H: int, kv_heads: int, prefix_len: int, max_len: int) -> int:
+    n = _lib.query("jx_attn_decode_prefix_workspace_bytes", B, H, kv_heads, prefix_len, max_len)
+    if n < 0:
+        raise ValueError(f"attn_decode_prefix: unsupported shape B {B}, H {H}, kv_heads {kv_heads}, prefix {prefix_len}, "
+                         f"max_len {max_len}")
+    return n
+
+
+def attn_decode_prefix(qkv: torch.Tensor, kprefix: torch.Tensor, vprefix: torch.Tensor, prefix_len: int,
+                       kcache: torch.Tensor, vcache: torch.Tensor, lengths: torch.Tensor, H: int, D: int,
+                       kv_heads: int | None = None, max_len: int | None = None, workspace: torch.Tensor | None = None,
+                       out: torch.Tensor | None = None) -> torch.Tensor:
+    """One new token per sequence, where all sequences share the first `prefix_len` positions: that prefix is read
+    once for all of them. qkv [B, (H + 2 kv_heads)*D] (the new rows), kprefix / vprefix [>= prefix_len, kv_heads*D],
+    kcache / vcache [B, >= max_len, kv_heads*D] with each sequence's own positions. `lengths` (int32 [B], on the
+    device) counts a sequence's own positions with the new one, whose k / v are appended at lengths[b] - 1; 0
+    marks an idle sequence (zero output, nothing appended). `max_len` is their upper bound (default: the caches'
+    rows). Returns [B, H*D]. Calls that may overlap need workspaces of their own."""
+    kv = H if kv_heads is None else kv_heads
+    for name, t in (("qkv", qkv), ("kprefix", kprefix), ("vprefix", vprefix), ("kcache", kcache), ("vcache", vcache)):
+        _check(t, F16, name, contiguous=False)
+        if t.stride(-1) != 1:
+            raise ValueError(f"{name} must have unit column stride")
+    _check(lengths, I32, "lengths")
+    _check_here(qkv=qkv, kprefix=kprefix, vprefix=vprefix, kcache=kcache, vcache=vcache, lengths=lengths,
+                workspace=workspace, out=out)
+    B = qkv.shape[0]
+    max_len = kcache.shape[1] if max_len is None else max_len
+    _shape(qkv, (B, (H + 2 * kv) * D), "qkv")
+    _shape(lengths, (B,), "lengths")
+    _shape(kcache, (B, kcache.shape[1], kv * D), "kcache")
+    if kprefix.dim() != 2 or kprefix.shape[1] != kv * D or not 0 <= prefix_len <= kprefix.shape[0]:
+        raise ValueError("attn_decode_prefix: kprefix must be [>= prefix_len, kv_heads*D]")
+    if kprefix.shape != vprefix.shape or kcache.shape != vcache.shape or (
+            kprefix.stride() != vprefix.stride() or kcache.stride() != vcache.stride()):
+        raise ValueError("attn_decode_prefix: keys and values must share a layout")
+    if not 0 < max_len <= kcache.shape[1]:
+        raise ValueError("attn_decode_prefix: the caches must hold `max_len` positions")
+    (s0, s1), w = kcache.stride()[:2], kv * D
+    if B > 1 and not (min(s0, s1) >= w and (s0 >= (kcache.shape[1] - 1) * s1 + w or s1 >= (B - 1) * s0 + w)):
+        raise ValueError("attn_decode_prefix: the sequences' caches overlap")
+    need = attn_decode_prefix_workspace_bytes(B, H, kv, prefix_len, max_len)
+    if workspace is None:
+        workspace = torch.empty(need // 4 + 4, device=qkv.device, dtype=F32)
+    elif not workspace.is_contiguous() or workspace.numel() * workspace.element_size() < need:
+        raise ValueError(f"attn_decode_prefix: workspace needs {need} bytes")
+    if out is None:
+        out = torch.empty(B, H * D, device=qkv.device, dtype=F16)
+    else:
+        _check(out, F16, "out", contiguous=False)
+        _shape(out, (B, H * D), "out")
+    row = lambda t, i, w: t.stride(i) if t.shape[i] > 1 else w  # noqa: E731  (a single row's stride says nothing)
+    _lib.call("jx_attn_decode_prefix", qkv.data_ptr(), row(qkv, 0, qkv.shape[1]), kprefix.data_ptr(), vprefix.data_ptr(),
+              row(kprefix, 0, kv * D), prefix_len, kcache.data_ptr(), vcache.data_ptr(), row(kcache, 1, kv * D),
+              row(kcache, 0, 0), lengths.data_ptr(), max_len, B, H, kv, D, 1.0 / math.sqrt(D), workspace.data_ptr(),
+              out.data_ptr(), row(out, 0, H * D), _stream())
+    return out
+
+
+# ---------------------------------------------------------------- next tokens
+def sample(logits16: torch.Tensor, uniforms: torch.Tensor, temperature: float | torch.Tensor = 1.0,
+           top_k: int | torch.Tensor = 0, top_p: float | torch.Tensor = 1.0, min_p: float | torch.Tensor = 0.0,
+           tokens: torch.Tensor | None = None, logprobs: torch.Tensor | None = None):
+    """Draws one token per row of fp16 logits [rows, vocab] with the given uniform numbers (f32 [rows], in [0, 1)):
+    returns (tokens int64 [rows], logprobs f32 [rows]). Temperature, then top-k, then top-p over what top-k left,
+    then min-p (relative to the largest probability); among equal logits the lower index ranks first. temperature
+    0 is greedy; top_k 0, top_p 1 and min_p 0 are off. Each setting is a number, or a device tensor with one value
+    per row (f32; top_k int32). A row with a NaN or without a finite logit gives token -1 and a NaN."""
+    rows, vocab, ld = _logit_rows(logits16, "logits16")
+    _check(uniforms, F32, "uniforms")
+    _shape(uniforms, (rows,), "uniforms")
+    per_row = []
+    for name, v, dtype in (("temperature", temperature, F32), ("top_k", top_k, I32), ("top_p", top_p, F32),
+                           ("min_p", min_p, F32)):
+        if isinstance(v, torch.Tensor):
+            _check(v, dtype, name)
+            _shape(v, (rows,), name)
+            per_row += [v, 0]
+        else:
+            if v != v or (name == "temperature" and v < 0):
+                raise ValueError(f"sample: bad {name} {v}")
+            per_row += [None, min(max(int(v), 0), 2**31 - 1) if dtype == I32 else float(v)]
+    tokens = torch.empty(rows, device=logits16.device, dtype=I64) if tokens is None else tokens
+    logprobs = torch.empty(rows, device=logits16.device, dtype=F32) if logprobs is None else logprobs
+    _check(tokens, I64, "tokens")
+    _check(logprobs, F32, "logprobs")
+    _shape(tokens, (rows,), "tokens")
+    _shape(logprobs, (rows,), "logprobs")
+    t, t_s, k, k_s, p, p_s, m, m_s = per_row
+    _check_here(logits16=logits16, uniforms=uniforms, temperature=t, top_k=k, top_p=p, min_p=m, tokens=tokens,
+                logprobs=logprobs)
+    if rows:
+        _lib.call("jx_sample", logits16.data_ptr(), rows, vocab, ld, uniforms.data_ptr(), _ptr(t), t_s, _ptr(k), k_s,
+                  _ptr(p), p_s, _ptr(m), m_s, tokens.data_ptr(), logprobs.data_ptr(), _stream())
+    return tokens, logprobs
+
+
+def top_logits(logits16: torch.Tensor, k: int, values: torch.Tensor | None = None, ids: torch.Tensor | None = None):
+    """The k largest fp16 logits of each row, largest first, the lower index first among equal ones (NaN last):
+    (values f16 [rows, k], ids int64 [rows, k]); k at most min(vocab, 1024)."""
+    rows, vocab, ld = _logit_rows(logits16, "logits16")
+    values = torch.empty(rows, k, device=logits16.device, dtype=F16) if values is None else values
+    ids = torch.empty(rows, k, device=logits16.device, dtype=I64) if ids is None else ids
+    _check(values, F16, "values")
+    _check(ids, I64, "ids")
+    _shape(values, (rows, k), "values")
+    _shape(ids, (rows, k), "ids")
+    _check_here(logits16=logits16, values=values, ids=ids)
+    if rows:
+        _lib.call("jx_top_logits", logits16.data_ptr(), rows, vocab, ld, k, values.data_ptr(), ids.data_ptr(), _stream())
+    return values, ids
+
+
 # ---------------------------------------------------------------- cross-entropy
 def ce_fwd(logits16: torch.Tensor, targets: torch.Tensor, ignore_index: int = -100, lse=None, row_loss=None):
     _check(targets, I64, "targets")
@@ -392,6 +530,75 @@ def ce_bwd(logits16, targets, lse, grad_loss: torch.Tensor, count: torch.Tensor,
     rows, vocab = logits16.shape
     _lib.call("jx_ce_bwd", logits16.data_ptr(), rows, vocab, _ld(logits16), targets.data_ptr(), ignore_index,
               lse.data_ptr(), grad_loss.data_ptr(), count.data_ptr(), _stream())
+
+
+# ---------------------------------------------------------------- distillation
+def _teacher(logits16, teacher_ids, teacher_logits, targets):
+    rows, vocab, ld = _logit_rows(logits16, "logits16")
+    _check(teacher_ids, I64, "teacher_ids")
+    if not isinstance(teacher_logits, torch.Tensor) or teacher_logits.dtype not in (F16, F32):
+        raise TypeError("teacher_logits must be a float16 or float32 tensor")
+    _check(teacher_logits, teacher_logits.dtype, "teacher_logits")
+    _check(targets, I64, "targets")
+    if teacher_ids.dim() != 2:
+        raise ValueError("teacher_ids must be [rows, K]")
+    K = teacher_ids.shape[1]
+    _shape(teacher_ids, (rows, K), "teacher_ids")
+    _shape(teacher_logits, (rows, K), "teacher_logits")
+    _shape(targets, (rows,), "targets")
+    _check_here(logits16=logits16, teacher_ids=teacher_ids, teacher_logits=teacher_logits, targets=targets)
+    return rows, vocab, ld, K
+
+
+def distill_fwd(logits16: torch.Tensor, teacher_ids: torch.Tensor, teacher_logits: torch.Tensor, targets: torch.Tensor,
+                temperature: float = 1.0, alpha: float = 1.0, ignore_index: int = -100,
+                parts: torch.Tensor | None = None, stats: torch.Tensor | None = None,
+                row_loss: torch.Tensor | None = None):
+    """Per-row distillation loss from a teacher's K top logits, mixed with the cross-entropy of the targets:
+    alpha temperature^2 KL(p || q) + (1 - alpha) CE, p the teacher's softmax over its used slots (id >= 0), q the
+    student's over the vocabulary, both at `temperature`. logits16 [rows, vocab] fp16, teacher_ids int64 [rows, K],
+    teacher_logits fp16 or fp32 [rows, K], targets int64 [rows] (ignore_index rows give 0). `parts` from
+    gemm_f16_ce_parts for these logits saves the pass over them at temperature 1. Returns (stats f32 [3, rows],
+    row_loss f32 [rows]); ce_loss(row_loss, targets, ignore_index) is the mean."""
+    rows, vocab, ld, K = _teacher(logits16, teacher_ids, teacher_logits, targets)
+    stats = torch.empty(3, rows, device=logits16.device, dtype=F32) if stats is None else stats
+    row_loss = torch.empty(rows, device=logits16.device, dtype=F32) if row_loss is None else row_loss
+    _check(stats, F32, "stats")
+    _check(row_loss, F32, "row_loss")
+    _shape(stats, (3, rows), "stats")
+    _shape(row_loss, (rows,), "row_loss")
+    if parts is not None:
+        _check(parts, F32, "parts")
+        if parts.numel() < rows * ce_parts_blocks(vocab) * 2:
+            raise ValueError("parts is too small")
+    _check_here(parts=parts, stats=stats, row_loss=row_loss)
+    _lib.call("jx_distill_fwd", logits16.data_ptr(), rows, vocab, ld, teacher_ids.data_ptr(), teacher_logits.data_ptr(),
+              int(teacher_logits.dtype == F16), K, targets.data_ptr(), ignore_index, float(temperature), float(alpha),
+              _ptr(parts), stats.data_ptr(), row_loss.data_ptr(), _stream())
+    return stats, row_loss
+
+
+def distill_bwd(logits16: torch.Tensor, teacher_ids: torch.Tensor, teacher_logits: torch.Tensor, targets: torch.Tensor,
+                stats: torch.Tensor, grad_loss: torch.Tensor, count: torch.Tensor, temperature: float = 1.0,
+                alpha: float = 1.0, ignore_index: int = -100, out: torch.Tensor | None = None) -> torch.Tensor:
+    """Gradient of the mean of distill_fwd's row losses (over `count` rows, a device scalar), times `grad_loss`,
+    with respect to the logits: fp16 [rows, vocab], into `out`, or over the logits themselves without one."""
+    rows, vocab, ld, K = _teacher(logits16, teacher_ids, teacher_logits, targets)
+    out = logits16 if out is None else out
+    orows, ovocab, ld_out = _logit_rows(out, "out")
+    if (orows, ovocab) != (rows, vocab):
+        raise ValueError(f"out must have shape {(rows, vocab)}, got {(orows, ovocab)}")
+    _check(stats, F32, "stats")
+    _shape(stats, (3, rows), "stats")
+    _check(grad_loss, F32, "grad_loss")
+    _check(count, F32, "count")
+    if grad_loss.numel() != 1 or count.numel() != 1:
+        raise ValueError("grad_loss and count must hold one value")
+    _check_here(stats=stats, grad_loss=grad_loss, count=count, out=out)
+    _lib.call("jx_distill_bwd", logits16.data_ptr(), rows, vocab, ld, teacher_ids.data_ptr(), teacher_logits.data_ptr(),
+              int(teacher_logits.dtype == F16), K, targets.data_ptr(), ignore_index, float(temperature), float(alpha),
+              stats.data_ptr(), grad_loss.data_ptr(), count.data_ptr(), out.data_ptr(), ld_out, _stream())
+    return out
 
 
 # ---------------------------------------------------------------- optimizer

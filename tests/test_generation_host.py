@@ -1,0 +1,122 @@
+"""Host-side checks of the shared-prefix attention, sampling, top-logit and distillation entry points: arguments that
+are refused before anything is launched, and the workspace query. Pointers are small aligned numbers that nothing
+reads."""
+import pytest
+import torch
+
+A = 256  # a non-NULL, 16-byte aligned pointer
+
+
+def _call(name, *args):
+    from midstream_llm_b200 import _lib
+    _lib.call(name, *args)
+
+
+def _prefix(**kw):
+    a = dict(qkv=A, ld_qkv=768, kp=A, vp=A, ld_p=256, P=100, kc=A, vc=A, ld_c=256, bs=25600, lens=A, max_len=100, B=2, H=4,
+             kv=4, D=64, scale=0.125, ws=A, out=A, ld_out=256, stream=None)
+    a.update(kw)
+    return tuple(a.values())
+
+
+@pytest.mark.parametrize("kw,text", [
+    (dict(D=128), "head_dim must be 64"), (dict(qkv=None), "NULL"), (dict(lens=None), "NULL"), (dict(kp=None), "NULL"),
+    (dict(B=0), "bad shape"), (dict(H=5, kv=2), "bad shape"), (dict(H=130, kv=1), "bad shape"), (dict(P=-1), "bad shape"),
+    (dict(max_len=0), "bad shape"), (dict(P=1 << 40), "bad shape"), (dict(qkv=A + 8), "16-byte"), (dict(ws=A + 4), "16-byte"),
+    (dict(ld_qkv=764), "strides"), (dict(ld_qkv=760), "strides"), (dict(ld_c=248), "strides"), (dict(ld_p=260), "strides"),
+    (dict(bs=12), "strides"), (dict(ld_out=255), "strides"),
+])
+def test_prefix_attention_refuses(kw, text):
+    from midstream_llm_b200 import _lib
+    with pytest.raises(_lib.JxError, match=text):
+        _call("jx_attn_decode_prefix", *_prefix(**kw))
+
+
+def test_prefix_workspace_query():
+    from midstream_llm_b200 import _lib, ops
+    need = lambda *a: _lib.query("jx_attn_decode_prefix_workspace_bytes", *a)  # noqa: E731
+    assert need(0, 4, 4, 10, 10) == need(1, 4, 3, 10, 10) == need(1, 4, 4, -1, 10) == need(1, 4, 4, 10, 0) == -1
+    # every row has room for at least one part of the prefix and one of its own keys: (m, l) and 64 sums
+    for B, H, kv, P, S in ((1, 4, 4, 1, 1), (16, 16, 16, 1791, 257), (64, 16, 4, 40000, 1000), (300, 2, 1, 129, 5)):
+        assert need(B, H, kv, P, S) >= B * H * 2 * (8 + 256)
+        assert need(B, H, kv, 0, S) >= B * H * (8 + 256)
+    with pytest.raises(ValueError, match="unsupported shape"):
+        ops.attn_decode_prefix_workspace_bytes(2, 130, 1, 10, 10)
+
+
+@pytest.mark.parametrize("kw,text", [
+    (dict(x=None), "NULL"), (dict(u=None), "NULL"), (dict(tok=None), "NULL"), (dict(rows=0), "bad shape"),
+    (dict(V=0), "bad shape"), (dict(V=(1 << 20) + 1, ld=(1 << 20) + 8), "bad shape"), (dict(ld=992), "bad shape"),
+    (dict(ld=1004), "ld%8"), (dict(x=A + 2), "16B"),
+])
+def test_sample_refuses(kw, text):
+    from midstream_llm_b200 import _lib
+    a = dict(x=A, rows=3, V=1000, ld=1000, u=A, T=None, Ts=1.0, k=None, ks=0, p=None, ps=1.0, m=None, ms=0.0, tok=A, lp=None,
+             stream=None)
+    a.update(kw)
+    with pytest.raises(_lib.JxError, match=text):
+        _call("jx_sample", *a.values())
+
+
+@pytest.mark.parametrize("kw,text", [
+    (dict(k=0), "k must be"), (dict(k=1001), "k must be"), (dict(V=4000, ld=4000, k=1025), "k must be"), (dict(v=None), "NULL"),
+    (dict(rows=-1), "bad shape"), (dict(ld=1004), "ld%8"),
+])
+def test_top_logits_refuses(kw, text):
+    from midstream_llm_b200 import _lib
+    a = dict(x=A, rows=3, V=1000, ld=1000, k=5, v=A, i=A, stream=None)
+    a.update(kw)
+    with pytest.raises(_lib.JxError, match=text):
+        _call("jx_top_logits", *a.values())
+
+
+@pytest.mark.parametrize("kw,text", [
+    (dict(x=None), "NULL"), (dict(ids=None), "NULL"), (dict(stats=None), "NULL"), (dict(K=0), "teacher slots"),
+    (dict(K=1025), "teacher slots"), (dict(tau=0.0), "temperature"), (dict(tau=float("nan")), "temperature"),
+    (dict(alpha=-0.1), "alpha"), (dict(alpha=float("nan")), "alpha"), (dict(rows=0), "bad shape"), (dict(ld=1004), "ld%8"),
+])
+def test_distill_refuses(kw, text):
+    from midstream_llm_b200 import _lib
+    a = dict(x=A, rows=3, V=1000, ld=1000, ids=A, t=A, f16=1, K=4, y=A, ignore=-100, tau=1.0, alpha=1.0)
+    a.update({k: v for k, v in kw.items() if k in a})
+    s = kw.get("stats", A)
+    with pytest.raises(_lib.JxError, match=text):
+        _call("jx_distill_fwd", *a.values(), None, s, A, None)
+    with pytest.raises(_lib.JxError, match=text):
+        _call("jx_distill_bwd", *a.values(), s, A, A, A, 1000, None)
+
+
+def test_distill_backward_refuses_other_strides_in_place():
+    from midstream_llm_b200 import _lib
+    with pytest.raises(_lib.JxError, match="in place"):
+        _call("jx_distill_bwd", A, 3, 1000, 1008, A, A, 1, 4, A, -100, 1.0, 1.0, A, A, A, A, 1000, None)
+
+
+def test_wrappers_refuse_cpu_tensors():
+    from midstream_llm_b200 import ops
+    x, u = torch.zeros(2, 8, dtype=torch.float16), torch.zeros(2)
+    ids = torch.zeros(2, 3, dtype=torch.int64)
+    for call in (lambda: ops.sample(x, u), lambda: ops.top_logits(x, 2), lambda: ops.distill_fwd(x, ids, x[:, :3], ids[:, 0]),
+                 lambda: ops.attn_decode_prefix(x, x, x, 1, x, x, u.int(), 4, 64)):
+        with pytest.raises(RuntimeError, match="CUDA"):
+            call()
+
+
+def test_prefix_schedule_gives_every_tile_to_one_block():
+    """The rule that cuts the prefix tiles among blocks, restated: runs that cover the line, at least one tile each,
+    and no more blocks on a unit than the workspace has parts for."""
+    import random
+    r = random.Random(0)
+    for _ in range(2000):
+        NT, units, blocks = r.randint(1, 300), r.randint(1, 70), r.choice([2, 20, 296])
+        T = NT * units
+        gp = min(T, blocks)
+        starts = [c * T // gp for c in range(gp + 1)]
+        assert starts[0] == 0 and starts[-1] == T and all(b > a for a, b in zip(starts, starts[1:]))
+        block_of = lambda x: ((x + 1) * gp - 1) // T  # noqa: E731
+        for x in {0, T - 1, *(r.randrange(T) for _ in range(5))}:
+            c = block_of(x)
+            assert starts[c] <= x < starts[c + 1]
+        room = min(NT, (NT * gp + T - 1) // T + 1)
+        for u in range(units):
+            assert block_of(u * NT + NT - 1) - block_of(u * NT) + 1 <= room
