@@ -5,12 +5,16 @@
 // (Midstream-LLM src/jishui/generate_torch.py:279-285); decode_attn.cu is the form for caches that share nothing.
 //
 // With G query heads per key / value head, the queries of all sequences at one key / value head are rows of one
-// matrix, so the prefix is read once for up to 128 rows and its scores are matrix products: for every 128 keys
-//   S = Q K^T  (tcgen05, M 128 rows, N 128 keys, K 64, Q and K in shared memory)   -> TMEM
-//   P = exp2(S scale - m) as fp16, with a lazily updated row maximum m             -> TMEM
-//   O += P V   (tcgen05, M 128, N 64, K 128, P from TMEM, V from shared memory)    -> TMEM
-// A sequence's own keys go through the same pipeline with only its G heads as rows: the matrix unit has far
-// more than the time that the 32 KB of a tile take from memory, whatever part of its rows is used.
+// matrix, so the prefix is read once for up to 64 rows and its scores are matrix products. They are formed
+// transposed, with the keys along the matrix unit's 128 rows: then a thread owns one key, and the softmax's work is
+// in proportion to the query rows and spread over all four warps however few they are. For every 128 keys
+//   S^T = K Q^T        (tcgen05, M 128 keys, N 16-64 rows, K 64, both from shared memory)          -> TMEM
+//   P   = exp2(S scale - m) as fp16, against a reference m per row                                 -> shared memory
+//   [O^T; l] += [V^T; 1] P  (tcgen05, M 128 = 64 head columns and the sum's row, N rows, K 128 keys) -> TMEM
+// m is the row's maximum over the first tile and is raised only when a later P passes 2^8 (a rare step that
+// rescales O^T), so no other tile needs a maximum across threads. The sum l comes out of the same product from
+// the same rounded P, by a block of ones behind V^T. A sequence's own keys take the same way with its G heads
+// as rows.
 //
 // Work: the prefix tiles of all (row tile, key / value head) units stand in one line that is cut into equal runs, one
 // a block, so that each unit is split over a few blocks; the (sequence, head, chunk) items of the own keys
@@ -21,7 +25,7 @@
 //   warp 0    TMA producer: Q of the item, K and V tiles (2 and 3 slots of 16 KB),
 //   warp 1    MMA issuer; before the tile that holds a sequence's end it puts the new key and value into the
 //             tile (and the cache) and clears the values behind them, since 0 * garbage may be NaN,
-//   warps 2-5 softmax, one row per thread, and the parts' output.
+//   warps 2-5 softmax, one key per thread, and the parts' output.
 #include <algorithm>
 #include <atomic>
 
@@ -33,12 +37,14 @@ namespace pfx {
 
 constexpr int D = 64;
 constexpr int BKV = 128;
+constexpr int kRows = 64;  // query rows of a tile at most
 constexpr int kThreads = 192;
-constexpr uint32_t kTile = BKV * D * 2;  // 16 KiB
+constexpr uint32_t kTile = BKV * D * 2;   // 16 KiB
+constexpr uint32_t kQTile = kRows * D * 2;  // 8 KiB
+constexpr uint32_t kOnes = 2048;          // 16 keys x 64 ones
 constexpr int kKSlots = 2, kVSlots = 3;
-constexpr int kMaxGroup = 64;
-constexpr int kLens = 1024;  // lengths kept in shared memory
-constexpr uint32_t kTmemCols = 256;  // S [0,128), P (fp16 pairs) [128,192), O [192,256)
+constexpr int kLens = 512;  // lengths kept in shared memory
+constexpr uint32_t kTmemCols = 256;  // S^T [0,64) and [64,128), [O^T; l] [128,192)
 
 enum Status : int { kProducer = 601, kMma = 602, kSoftmax = 603 };
 
@@ -48,7 +54,8 @@ struct Sched {
   int P, NT;           // prefix keys and tiles of one unit
   int T, gp;           // prefix tiles in all, and blocks that share them
   int max_len, OC;     // own keys: upper bound, tiles per item
-  int pairs, n_own;    // B * Hkv, items
+  int chunks;          // items of one (sequence, key / value head)
+  int step_b, step_h;  // (sequence, head) distance of a block's consecutive items: grid = step_b Hkv + step_h
   int nparts;          // parts a row has room for
   int nsp;             // of those, for the prefix
 
@@ -61,7 +68,7 @@ __device__ __forceinline__ int own_length(const Sched& s, int raw) { return raw 
 // The tiles of one block in order. Every role walks its own copy.
 struct Cursor {
   int t, t1;    // prefix tiles left
-  int own;      // next item of own keys
+  int ob, oh, oc;  // sequence, head and chunk of the next item of own keys
   int b, h;     // first sequence of the row tile, or the sequence; key / value head
   int key0, n, j, limit;  // first key, tiles, current tile, end of the keys
   int part, ipre, iown;   // part index; prefix / own items begun before
@@ -74,10 +81,17 @@ struct Cursor {
       t = (int)((int64_t)c * s.T / s.gp);
       t1 = (int)((int64_t)(c + 1) * s.T / s.gp);
     }
-    own = gridDim.x - 1 - c;  // dealt from the last block on: those may have no prefix tiles
+    const int own = gridDim.x - 1 - c;  // dealt from the last block on: those may have no prefix tiles
+    ob = own / s.Hkv;
+    oh = own - ob * s.Hkv;
+    oc = ob / s.B;
+    ob -= oc * s.B;
     ipre = iown = -1;
+    n = j = 0;
   }
-  __device__ __forceinline__ bool next_item(const Sched& s, const int* lens) {
+  // The next tile; false at the end.
+  __device__ __forceinline__ bool advance(const Sched& s, const int* lens) {
+    if (++j < n) return true;
     j = 0;
     if (t < t1) {
       const int unit = t / s.NT, first = t - unit * s.NT;
@@ -92,11 +106,13 @@ struct Cursor {
       t += n;
       return true;
     }
-    while (own < s.n_own) {
-      const int chunk = own / s.pairs, pair = own - chunk * s.pairs;
-      own += gridDim.x;
-      b = pair / s.Hkv;
-      h = pair - b * s.Hkv;
+    while (oc < s.chunks) {
+      b = ob, h = oh;
+      const int chunk = oc;
+      oh += s.step_h;
+      ob += s.step_b;
+      if (oh >= s.Hkv) oh -= s.Hkv, ++ob;
+      while (ob >= s.B) ob -= s.B, ++oc;
       limit = own_length(s, lens[b]);
       key0 = chunk * s.OC * BKV;
       if (key0 >= limit) continue;
@@ -108,9 +124,7 @@ struct Cursor {
     }
     return false;
   }
-  __device__ __forceinline__ bool next_tile(const Sched& s, const int* lens) {
-    return ++j < n || next_item(s, lens);
-  }
+  __device__ __forceinline__ int rows(const Sched& s) const { return is_own ? s.G : min(s.nb, s.B - b) * s.G; }
   __device__ __forceinline__ int key() const { return key0 + j * BKV; }
   __device__ __forceinline__ bool ends() const { return is_own && key() + BKV >= limit; }
 };
@@ -118,13 +132,18 @@ struct Cursor {
 struct Bars {
   uint64_t k_full[kKSlots], k_empty[kKSlots], v_full[kVSlots], v_empty[kVSlots];
   uint64_t q_full[3], q_empty[3];  // own items alternate between 0 and 1, prefix items use 2
-  uint64_t s_full, s_free, p_full, p_empty;
+  uint64_t s_full[2], s_free[2], p_full, p_empty;
   uint32_t tmem_base;
   int abort;
+  alignas(16) float m[kRows];        // reference of each row, log2 units; +inf for columns without a row
+  alignas(16) float alpha[kRows];    // factor of a raised reference
+  alignas(16) float wmax[4][kRows];  // each warp's maxima
+  int at[kRows];                     // place of each row's part in the workspace
   int lens[kLens];
 };
 
 __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* status, int code) {
+  if (mbar_try_wait(bar, parity)) return true;
   const long long start = clock64();
   for (uint32_t i = 0;; ++i) {
     if (mbar_try_wait(bar, parity)) return true;
@@ -139,14 +158,30 @@ __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, volatile in
   }
 }
 
-// Lane 0 polls, the warp follows.
+// Every lane polls.
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* status,
                                           int code) {
-  int ok = 1;
-  if ((threadIdx.x & 31) == 0) ok = wait(bar, parity, abort_flag, status, code) ? 1 : 0;
-  ok = __shfl_sync(0xffffffffu, ok, 0);
-  __syncwarp();
-  return ok != 0;
+  return __all_sync(0xffffffffu, wait(bar, parity, abort_flag, status, code));
+}
+
+// Barrier of the four softmax warps; true if any thread's flag is set.
+__device__ __forceinline__ bool softmax_any(bool flag) {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.u32 p, %1, 0;\n\t"
+      "barrier.cta.red.or.pred q, 1, 128, p;\n\t"
+      "selp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(r)
+      : "r"((uint32_t)flag)
+      : "memory");
+  return r != 0;
+}
+
+__device__ __forceinline__ float redux_max(float v) {
+  float r;
+  asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+  return r;
 }
 
 __device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, uint64_t* bar, int x, int y, int z) {
@@ -179,6 +214,147 @@ struct Params {
   uint32_t q_own_bytes, q_own_stride, q_pre_bytes;
 };
 
+template <int N>
+__device__ __forceinline__ void load_cols(uint32_t addr, uint32_t (&r)[N]) {
+  if constexpr (N == 8) {
+    tmem_ld8(addr, r);
+  } else if constexpr (N == 16) {
+    tmem_ld16(addr, r);
+  } else {
+#pragma unroll
+    for (int q = 0; q < N / 32; ++q) tmem_ld32(addr + q * 32, *reinterpret_cast<uint32_t(*)[32]>(&r[q * 32]));
+  }
+  tmem_ld_wait();
+}
+
+// The tiles of one item, by the four softmax warps: thread = key, W columns of which the first `rows` are rows.
+// `g` counts tiles over all items. Columns behind the rows hold garbage on all ways and are never looked at; their
+// reference is +inf, so that they pass no bound.
+template <int W>
+__device__ __forceinline__ bool softmax_item(const Params& p, Cursor& c, const int rows, uint32_t& g, Bars* bars, uint8_t* sP,
+                                             uint32_t tmem, int* status) {
+  volatile int* abort_flag = &bars->abort;
+  const Sched& s = p.s;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int quarter = warp & 3;  // TMEM lanes this warp may access
+  const int key = quarter * 32 + lane;
+  const uint32_t base = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
+  uint8_t* prow = sP + key * 128;
+  const float scale = p.scale_log2;
+  for (c.j = 0; c.j < c.n; ++c.j, ++g) {
+    const int x = g & 1;
+    if (!warp_wait(&bars->s_full[x], (g >> 1) & 1, abort_flag, status, kSoftmax)) return false;
+    tc_fence_after();
+    uint32_t sr[W];
+    load_cols(base + x * 64, sr);
+    tc_fence_before();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&bars->s_free[x]);  // the scores are in registers
+    if (c.key() + BKV > c.limit && c.key() + key >= c.limit) {  // a key past the end
+#pragma unroll
+      for (int i = 0; i < W; ++i) sr[i] = 0xff800000u;
+    }
+    uint32_t pw[W / 2];
+    // P of this thread's key; true if one of them passes the bound.
+    auto probabilities = [&]() -> bool {
+      float top[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int i = 0; i < W; i += 4) {
+        const float4 m = *reinterpret_cast<const float4*>(&bars->m[i]);
+        const float p0 = ex2(fmaf(__uint_as_float(sr[i]), scale, -m.x));
+        const float p1 = ex2(fmaf(__uint_as_float(sr[i + 1]), scale, -m.y));
+        const float p2 = ex2(fmaf(__uint_as_float(sr[i + 2]), scale, -m.z));
+        const float p3 = ex2(fmaf(__uint_as_float(sr[i + 3]), scale, -m.w));
+        top[(i >> 2) & 3] = fmaxf(top[(i >> 2) & 3], fmaxf(fmaxf(p0, p1), fmaxf(p2, p3)));
+        const __half2 h0 = __floats2half2_rn(p0, p1), h1 = __floats2half2_rn(p2, p3);
+        pw[i / 2] = *reinterpret_cast<const uint32_t*>(&h0);
+        pw[i / 2 + 1] = *reinterpret_cast<const uint32_t*>(&h1);
+      }
+      return fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) > 256.f;
+    };
+    bool raise = c.j == 0;
+    if (!raise) raise = softmax_any(probabilities());
+    if (raise) {
+      // Maxima over the tile's keys, per warp, then over the warps.
+#pragma unroll
+      for (int i = 0; i < W; i += 4) {
+        float4 w;
+        w.x = redux_max(__uint_as_float(sr[i]));
+        w.y = redux_max(__uint_as_float(sr[i + 1]));
+        w.z = redux_max(__uint_as_float(sr[i + 2]));
+        w.w = redux_max(__uint_as_float(sr[i + 3]));
+        if (lane == 0) *reinterpret_cast<float4*>(&bars->wmax[quarter][i]) = w;
+      }
+      softmax_any(false);
+      const int i = threadIdx.x - 64;
+      if (i < W) {
+        float mx = INFINITY;
+        if (i < rows) {
+          mx = fmaxf(fmaxf(bars->wmax[0][i], bars->wmax[1][i]), fmaxf(bars->wmax[2][i], bars->wmax[3][i])) * scale;
+          if (c.j > 0) {
+            const float old = bars->m[i];
+            mx = fmaxf(mx, old);
+            bars->alpha[i] = ex2(old - mx);
+          } else {
+            const int sq = i / s.G;
+            bars->at[i] = ((c.b + sq) * s.H + c.h * s.G + i - sq * s.G) * s.nparts + c.part;
+          }
+        }
+        bars->m[i] = mx;
+      }
+      softmax_any(false);
+      probabilities();
+    }
+    // The product of the tile before must be done before P is overwritten or [O^T; l] rescaled.
+    if (g > 0 && !warp_wait(&bars->p_empty, (g - 1) & 1, abort_flag, status, kSoftmax)) return false;
+    if (raise && c.j > 0) {
+      tc_fence_after();
+#pragma unroll
+      for (int q = 0; q < W; q += 8) {
+        uint32_t orr[8];
+        load_cols(base + 128 + q, orr);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) orr[i] = __float_as_uint(__uint_as_float(orr[i]) * bars->alpha[q + i]);
+        tmem_st8(base + 128 + q, orr);
+      }
+      tmem_st_wait();
+      tc_fence_before();
+    }
+#pragma unroll
+    for (int q = 0; q < W / 8; ++q)
+      *reinterpret_cast<uint4*>(prow + ((q ^ (key & 7)) << 4)) =
+          make_uint4(pw[q * 4], pw[q * 4 + 1], pw[q * 4 + 2], pw[q * 4 + 3]);
+    fence_proxy_async_smem();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&bars->p_full);
+  }
+  // The item's part: columns of [O^T; l], 64 values from two warps, the sum from the third.
+  if (!warp_wait(&bars->p_empty, (g - 1) & 1, abort_flag, status, kSoftmax)) return false;
+  tc_fence_after();
+  if (quarter < 3) {
+#pragma unroll
+    for (int q = 0; q < W; q += 8) {
+      uint32_t orr[8];
+      load_cols(base + 128 + q, orr);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int r = q + i;
+        if (r < rows) {
+          const int64_t at = bars->at[r];
+          if (quarter < 2)
+            p.o[at * D + key] = __uint_as_float(orr[i]);
+          else if (lane == 0)
+            p.ml[at] = make_float2(bars->m[r], __uint_as_float(orr[i]));
+        }
+      }
+    }
+  }
+  // The next item's first product with V waits for this warp's next arrival at p_full, after these reads.
+  tc_fence_before();
+  c.j = c.n - 1;
+  return true;
+}
+
 __global__ void __launch_bounds__(kThreads, 2)
     attn_prefix_part_kernel(const __grid_constant__ CUtensorMap tm_qp, const __grid_constant__ CUtensorMap tm_qo,
                             const __grid_constant__ CUtensorMap tm_kp, const __grid_constant__ CUtensorMap tm_vp,
@@ -186,12 +362,16 @@ __global__ void __launch_bounds__(kThreads, 2)
                             const Params p, int* status) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  // Queries of own items (G rows each), of a prefix item, K and V slots. The matrix unit reads 128 rows from each
-  // query tile; behind an own item's G rows it finds other data, whose rows of S nobody reads.
-  uint8_t* sQ[3] = {smem, smem + p.q_own_stride, smem + 2 * p.q_own_stride};
-  uint8_t* sK = sQ[2] + kTile;
+  // Queries of own items (two, G rows each), of a prefix item, K and V slots, P, ones. The matrix unit reads the
+  // rows of a query tile in sixteens; behind an own item's G rows it finds other data, which only reaches columns
+  // of S^T and O^T that nobody reads.
+  uint8_t* sQ = smem;
+  uint8_t* sQp = smem + 2 * p.q_own_stride;
+  uint8_t* sK = sQp + kQTile;
   uint8_t* sV = sK + kKSlots * kTile;
-  Bars* bars = reinterpret_cast<Bars*>(sV + kVSlots * kTile);
+  uint8_t* sP = sV + kVSlots * kTile;
+  uint8_t* s1 = sP + kTile;
+  Bars* bars = reinterpret_cast<Bars*>(s1 + kOnes);
   volatile int* abort_flag = &bars->abort;
   const Sched& s = p.s;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -200,8 +380,7 @@ __global__ void __launch_bounds__(kThreads, 2)
     for (int i = 0; i < kKSlots; ++i) mbar_init(&bars->k_full[i], 1), mbar_init(&bars->k_empty[i], 1);
     for (int i = 0; i < kVSlots; ++i) mbar_init(&bars->v_full[i], 1), mbar_init(&bars->v_empty[i], 1);
     for (int i = 0; i < 3; ++i) mbar_init(&bars->q_full[i], 1), mbar_init(&bars->q_empty[i], 1);
-    mbar_init(&bars->s_full, 1);
-    mbar_init(&bars->s_free, 4);
+    for (int i = 0; i < 2; ++i) mbar_init(&bars->s_full[i], 1), mbar_init(&bars->s_free[i], 4);
     mbar_init(&bars->p_full, 4);
     mbar_init(&bars->p_empty, 1);
     bars->abort = 0;
@@ -210,6 +389,8 @@ __global__ void __launch_bounds__(kThreads, 2)
   const bool staged = s.B <= kLens;
   if (staged)
     for (int i = threadIdx.x; i < s.B; i += kThreads) bars->lens[i] = p.lens[i];
+  for (int i = threadIdx.x; i < (int)kOnes / 4; i += kThreads) reinterpret_cast<uint32_t*>(s1)[i] = 0x3c003c00u;
+  fence_proxy_async_smem();
   if (warp == 1) {
     tmem_alloc(&bars->tmem_base, kTmemCols);
     tmem_relinquish();
@@ -224,14 +405,14 @@ __global__ void __launch_bounds__(kThreads, 2)
 
   if (warp == 0) {
     if (lane == 0) {
-      uint32_t tile = 0;
-      for (bool more = c.next_item(s, lens); more; more = c.next_tile(s, lens), ++tile) {
+      for (uint32_t tile = 0; c.advance(s, lens); ++tile) {
         if (c.j == 0) {
           const int q = c.is_own ? (c.iown & 1) : 2;
           const uint32_t use = c.is_own ? (uint32_t)(c.iown >> 1) : (uint32_t)c.ipre;
           if (!wait(&bars->q_empty[q], (use & 1) ^ 1, abort_flag, status, kProducer)) break;
           mbar_expect_tx(&bars->q_full[q], c.is_own ? p.q_own_bytes : p.q_pre_bytes);
-          tma_load_3d(sQ[q], c.is_own ? &tm_qo : &tm_qp, &bars->q_full[q], 0, c.h * s.G, c.b);
+          tma_load_3d(q == 2 ? sQp : sQ + q * p.q_own_stride, c.is_own ? &tm_qo : &tm_qp, &bars->q_full[q], 0, c.h * s.G,
+                      c.b);
         }
         const uint32_t ks = tile % kKSlots, vs = tile % kVSlots;
         if (!wait(&bars->k_empty[ks], ((tile / kKSlots) & 1) ^ 1, abort_flag, status, kProducer)) break;
@@ -250,201 +431,96 @@ __global__ void __launch_bounds__(kThreads, 2)
     }
     __syncwarp();
   } else if (warp == 1) {
-    constexpr uint32_t idesc_s = idesc_f16_f32(128, BKV, false, false);
-    constexpr uint32_t idesc_o = idesc_f16_f32(128, D, false, true);
     const uint64_t dK0 = smem_desc_sw128(smem_u32(sK), 16, 1024);
-    const uint64_t dV0 = smem_desc_sw128(smem_u32(sV), 8192, 1024);
-    uint32_t ts = 0, tp = 0;  // S and P V products issued
-    // S of the cursor's tile.
-    auto issue_s = [&]() -> bool {
+    const uint64_t dP0 = smem_desc_sw128(smem_u32(sP), 8192, 1024);
+    // Of the last issued S^T, for its product with V: the row tile's width and whether it begins an item.
+    uint32_t width = 16;
+    bool first = true;
+    auto issue_s = [&](uint32_t ts, int x) -> bool {  // x = ts & 1
       const uint32_t ks = ts % kKSlots, vs = ts % kVSlots;
       const int q = c.is_own ? (c.iown & 1) : 2;
+      width = (uint32_t)(c.rows(s) + 15) & ~15u;
+      first = c.j == 0;
       if (c.j == 0) {
         const uint32_t use = c.is_own ? (uint32_t)(c.iown >> 1) : (uint32_t)c.ipre;
         if (!warp_wait(&bars->q_full[q], use & 1, abort_flag, status, kMma)) return false;
       }
+      const bool ends = c.ends();
+      const bool is_v = lane >= 8;
+      const int ch = lane & 7;
+      uint4 fresh = make_uint4(0, 0, 0, 0);  // lanes 0-7: the new key, 8-15: the new value
+      if (ends && lane < 16)
+        fresh = *reinterpret_cast<const uint4*>(p.qkv + (int64_t)c.b * p.ld_qkv + (s.H + c.h + (is_v ? s.Hkv : 0)) * D + ch * 8);
       if (!warp_wait(&bars->k_full[ks], (ts / kKSlots) & 1, abort_flag, status, kMma)) return false;
-      if (c.ends()) {
+      if (ends) {
         // The sequence ends in this tile: row `last` is the new token's.
         if (!warp_wait(&bars->v_full[vs], (ts / kVSlots) & 1, abort_flag, status, kMma)) return false;
         const int last = c.limit - 1 - c.key();
-        const __half* nk = p.qkv + (int64_t)c.b * p.ld_qkv + (s.H + c.h) * D;
-        const __half* nv = nk + s.Hkv * D;
-        const int64_t at = (int64_t)c.b * p.batch_stride + (int64_t)(c.limit - 1) * p.ld_cache + c.h * D;
         if (lane < 16) {
-          const int ch = lane & 7;
-          const bool is_v = lane >= 8;
-          const uint4 u = *reinterpret_cast<const uint4*>((is_v ? nv : nk) + ch * 8);
           uint8_t* tile = is_v ? sV + vs * kTile : sK + ks * kTile;
-          *reinterpret_cast<uint4*>(tile + last * 128 + ((ch ^ (last & 7)) << 4)) = u;
-          *reinterpret_cast<uint4*>((is_v ? p.vcache : p.kcache) + at + ch * 8) = u;
+          *reinterpret_cast<uint4*>(tile + last * 128 + ((ch ^ (last & 7)) << 4)) = fresh;
+          *reinterpret_cast<uint4*>((is_v ? p.vcache : p.kcache) + (int64_t)c.b * p.batch_stride +
+                                    (int64_t)(c.limit - 1) * p.ld_cache + c.h * D + ch * 8) = fresh;
         }
         for (int i = (last + 1) * 8 + lane; i < BKV * 8; i += 32)
           *reinterpret_cast<uint4*>(sV + vs * kTile + i * 16) = make_uint4(0, 0, 0, 0);
         fence_proxy_async_smem();
         __syncwarp();
       }
-      if (!warp_wait(&bars->s_free, (ts & 1) ^ 1, abort_flag, status, kMma)) return false;
+      if (!warp_wait(&bars->s_free[x], ((ts >> 1) & 1) ^ 1, abort_flag, status, kMma)) return false;
       tc_fence_after();
       if (lane == 0) {
-        const uint64_t a = smem_desc_sw128(smem_u32(sQ[q]), 16, 1024), b = desc_adv(dK0, ks * kTile);
+        const uint32_t idesc = idesc_f16_f32(BKV, 0, false, false) | (width >> 3) << 17;
+        const uint64_t a = desc_adv(dK0, ks * kTile);
+        const uint64_t b = smem_desc_sw128(smem_u32(q == 2 ? sQp : sQ + q * p.q_own_stride), 16, 1024);
 #pragma unroll
         for (int kk = 0; kk < D / 16; ++kk)
-          umma_f16(tmem, desc_adv(a, kk * 32), desc_adv(b, kk * 32), idesc_s, kk > 0 ? 1u : 0u);
-        umma_commit(&bars->s_full);
+          umma_f16(tmem + x * 64, desc_adv(a, kk * 32), desc_adv(b, kk * 32), idesc, kk > 0 ? 1u : 0u);
+        umma_commit(&bars->s_full[x]);
         umma_commit(&bars->k_empty[ks]);
         if (c.j == c.n - 1) umma_commit(&bars->q_empty[q]);
       }
       __syncwarp();
-      ++ts;
       return true;
     };
-    Cursor cp = c;
-    bool more_s = c.next_item(s, lens);
-    bool more_p = cp.next_item(s, lens);
-    bool ok = true;
-    if (more_s) {
-      ok = issue_s();
-      more_s = c.next_tile(s, lens);
-    }
-    while (ok && more_p) {
-      // S of the next tile goes ahead of this tile's P V.
-      if (more_s) {
-        if (!(ok = issue_s())) break;
-        more_s = c.next_tile(s, lens);
-      }
+    bool more = c.advance(s, lens);
+    bool ok = !more || issue_s(0, 0);
+    for (uint32_t tp = 0; ok && more; ++tp) {
+      const uint32_t pv_width = width;
+      const bool pv_first = first;
+      // S^T of the next tile goes ahead of this tile's product with V.
+      more = c.advance(s, lens);
+      if (more && !(ok = issue_s(tp + 1, (tp + 1) & 1))) break;
       const uint32_t vs = tp % kVSlots;
       if (!(ok = warp_wait(&bars->v_full[vs], (tp / kVSlots) & 1, abort_flag, status, kMma))) break;
       if (!(ok = warp_wait(&bars->p_full, tp & 1, abort_flag, status, kMma))) break;
       tc_fence_after();
       if (lane == 0) {
-        const uint64_t bv = desc_adv(dV0, vs * kTile);
+        const uint32_t idesc = idesc_f16_f32(128, 0, true, true) | (pv_width >> 3) << 17;
+        const uint32_t v = smem_u32(sV + vs * kTile), ones = smem_u32(s1);
 #pragma unroll
         for (int kk = 0; kk < BKV / 16; ++kk)
-          umma_f16_ts(tmem + 192, tmem + 128 + kk * 8, desc_adv(bv, kk * 2048), idesc_o, (cp.j > 0 || kk > 0) ? 1u : 0u);
+          // Rows 0-63 of A are V^T of 16 keys, rows 64-127, one leading offset on, ones.
+          umma_f16(tmem + 128, smem_desc_sw128(v + kk * 2048, ones - (v + kk * 2048), 1024), desc_adv(dP0, kk * 2048), idesc,
+                   (!pv_first || kk > 0) ? 1u : 0u);
         umma_commit(&bars->v_empty[vs]);
         umma_commit(&bars->p_empty);
       }
       __syncwarp();
-      ++tp;
-      more_p = cp.next_tile(s, lens);
     }
   } else {
-    const int quarter = warp & 3;  // TMEM lanes this warp may access
-    const int r = quarter * 32 + lane;
-    const uint32_t base = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
-    constexpr float kRescaleThreshold = 8.0f;  // log2 units: P stays below 2^8 against a stale maximum
-    uint32_t g = 0;  // tiles consumed
     bool ok = true;
-    for (bool more = c.next_item(s, lens); more && ok; more = c.next_item(s, lens)) {
-      const int seqs = c.is_own ? 1 : min(s.nb, s.B - c.b);
-      const int rows = seqs * s.G;
-      const bool active = quarter * 32 < rows;
-      float m = 0.f, l = 0.f;
-      for (int j = 0; j < c.n; ++j, ++g) {
-        if (!warp_wait(&bars->s_full, g & 1, abort_flag, status, kSoftmax)) { ok = false; break; }
-        tc_fence_after();
-        const int lim = min(c.limit - c.key0 - j * BKV, BKV);  // keys of this tile
-        float alpha = 1.f;
-        bool rescale = false;
-        if (active) {
-          float mp[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            if (q * 32 >= lim) break;
-            uint32_t sr[32];
-            tmem_ld32(base + q * 32, sr);
-            tmem_ld_wait();
-            if (q * 32 + 32 <= lim) {
-#pragma unroll
-              for (int i = 0; i < 32; ++i) mp[i & 3] = fmaxf(mp[i & 3], __uint_as_float(sr[i]));
-            } else {
-#pragma unroll
-              for (int i = 0; i < 32; ++i) mp[i & 3] = fmaxf(mp[i & 3], q * 32 + i < lim ? __uint_as_float(sr[i]) : -INFINITY);
-            }
-          }
-          const float mx = fmaxf(fmaxf(mp[0], mp[1]), fmaxf(mp[2], mp[3])) * p.scale_log2;
-          if (j == 0) {
-            m = mx;
-          } else if (mx > m + kRescaleThreshold) {
-            alpha = ex2(m - mx);
-            m = mx;
-            rescale = true;
-          }
-        }
-        // P V of the tile before must be done before P is overwritten or O rescaled.
-        if (g > 0 && !warp_wait(&bars->p_empty, (g - 1) & 1, abort_flag, status, kSoftmax)) { ok = false; break; }
-        tc_fence_after();
-        if (active) {
-          float sum[4] = {0.f, 0.f, 0.f, 0.f};
-          const float neg_m = -m;
-#pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            uint32_t pw[16];
-            if (q * 32 >= lim) {
-#pragma unroll
-              for (int e = 0; e < 16; ++e) pw[e] = 0;
-            } else {
-              uint32_t sr[32];
-              tmem_ld32(base + q * 32, sr);
-              tmem_ld_wait();
-#pragma unroll
-              for (int e = 0; e < 16; ++e) {
-                float p0 = ex2(fmaf(__uint_as_float(sr[2 * e]), p.scale_log2, neg_m));
-                float p1 = ex2(fmaf(__uint_as_float(sr[2 * e + 1]), p.scale_log2, neg_m));
-                if (q * 32 + 32 > lim) {
-                  if (q * 32 + 2 * e >= lim) p0 = 0.f;
-                  if (q * 32 + 2 * e + 1 >= lim) p1 = 0.f;
-                }
-                sum[(2 * e) & 3] += p0;
-                sum[(2 * e + 1) & 3] += p1;
-                const __half2 hp = __floats2half2_rn(p0, p1);
-                pw[e] = *reinterpret_cast<const uint32_t*>(&hp);
-              }
-            }
-            tmem_st16(base + 128 + q * 16, pw);
-          }
-          if (__any_sync(0xffffffffu, rescale)) {
-#pragma unroll
-            for (int q = 0; q < 2; ++q) {
-              uint32_t orr[32];
-              tmem_ld32(base + 192 + q * 32, orr);
-              tmem_ld_wait();
-#pragma unroll
-              for (int i = 0; i < 32; ++i) orr[i] = __float_as_uint(__uint_as_float(orr[i]) * alpha);
-              tmem_st32(base + 192 + q * 32, orr);
-            }
-          }
-          l = l * alpha + ((sum[0] + sum[1]) + (sum[2] + sum[3]));
-          tmem_st_wait();
-        }
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) {
-          mbar_arrive(&bars->s_free);
-          mbar_arrive(&bars->p_full);
-        }
-      }
-      if (!ok || !warp_wait(&bars->p_empty, (g - 1) & 1, abort_flag, status, kSoftmax)) break;
-      tc_fence_after();
-      if (active) {
-        uint32_t orr[64];
-        tmem_ld32(base + 192, *reinterpret_cast<uint32_t(*)[32]>(&orr[0]));
-        tmem_ld32(base + 224, *reinterpret_cast<uint32_t(*)[32]>(&orr[32]));
-        tmem_ld_wait();
-        if (r < rows) {
-          const int sq = r / s.G;
-          const int64_t at = ((int64_t)(c.b + sq) * s.H + c.h * s.G + (r - sq * s.G)) * s.nparts + c.part;
-          p.ml[at] = make_float2(m, l);
-          float4* dst = reinterpret_cast<float4*>(p.o + at * D);
-#pragma unroll
-          for (int i = 0; i < 16; ++i)
-            dst[i] = make_float4(__uint_as_float(orr[4 * i]), __uint_as_float(orr[4 * i + 1]),
-                                 __uint_as_float(orr[4 * i + 2]), __uint_as_float(orr[4 * i + 3]));
-        }
-      }
-      // The next item's first P V waits for this warp's next arrival at p_full, after these reads.
-      tc_fence_before();
+    for (uint32_t g = 0; ok && c.advance(s, lens);) {
+      const int rows = c.rows(s);
+      // Straight code for a few widths: branches per row cost more than the columns they save.
+      if (rows <= 8)
+        ok = softmax_item<8>(p, c, rows, g, bars, sP, tmem, status);
+      else if (rows <= 16)
+        ok = softmax_item<16>(p, c, rows, g, bars, sP, tmem, status);
+      else if (rows <= 32)
+        ok = softmax_item<32>(p, c, rows, g, bars, sP, tmem, status);
+      else
+        ok = softmax_item<64>(p, c, rows, g, bars, sP, tmem, status);
     }
   }
   tc_fence_before();
@@ -512,11 +588,11 @@ __global__ void __launch_bounds__(128) attn_prefix_join_kernel(const Params p, i
 
 // The schedule, from sizes and the SM count alone.
 bool plan(int B, int H, int Hkv, int64_t prefix_len, int64_t max_len, Sched* s, int* grid) {
-  if (B <= 0 || Hkv <= 0 || H <= 0 || H % Hkv || H / Hkv > kMaxGroup || prefix_len < 0 || max_len <= 0) return false;
+  if (B <= 0 || Hkv <= 0 || H <= 0 || H % Hkv || H / Hkv > kRows || prefix_len < 0 || max_len <= 0) return false;
   if (prefix_len > (1 << 28) || max_len > (1 << 28) || (int64_t)B * H > (1 << 24)) return false;
   const int blocks = 2 * num_sms();
   s->B = B, s->H = H, s->Hkv = Hkv, s->G = H / Hkv;
-  s->nb = std::min(128 / s->G, B);
+  s->nb = std::min(kRows / s->G, B);
   s->P = (int)prefix_len;
   s->NT = (s->P + BKV - 1) / BKV;
   const int64_t T = (int64_t)((B + s->nb - 1) / s->nb) * Hkv * s->NT;
@@ -529,12 +605,13 @@ bool plan(int B, int H, int Hkv, int64_t prefix_len, int64_t max_len, Sched* s, 
   // Enough items to even out ragged lengths, few parts to join.
   s->OC = (int)std::max<int64_t>(1, (own_all + 3 * blocks - 1) / (3 * blocks));
   s->OC = std::min(s->OC, own_tiles);
-  const int chunks = (own_tiles + s->OC - 1) / s->OC;
-  s->pairs = B * Hkv;
-  s->n_own = s->pairs * chunks;
+  s->chunks = (own_tiles + s->OC - 1) / s->OC;
   s->nsp = T > 0 ? (int)std::min<int64_t>(s->NT, ((int64_t)s->NT * s->gp + T - 1) / T + 1) : 0;
-  s->nparts = s->nsp + chunks;
-  *grid = (int)std::min<int64_t>(blocks, std::max<int64_t>(s->gp, T + s->n_own));
+  s->nparts = s->nsp + s->chunks;
+  if ((int64_t)B * H * s->nparts >= (1ll << 31)) return false;
+  *grid = (int)std::min<int64_t>(blocks, std::max<int64_t>(s->gp, T + (int64_t)B * Hkv * s->chunks));
+  s->step_b = *grid / Hkv;
+  s->step_h = *grid % Hkv;
   return true;
 }
 
@@ -565,7 +642,7 @@ extern "C" int jx_attn_decode_prefix(const void* qkv, int64_t ld_qkv, const void
   int grid;
   JX_CHECK_ARG(pfx::plan(B, H, Hkv, prefix_len, max_len, &p.s, &grid),
                "%s: bad shape B %d, H %d, Hkv %d (at most %d query heads per key head), prefix %lld, max_len %lld", name, B, H,
-               Hkv, pfx::kMaxGroup, (long long)prefix_len, (long long)max_len);
+               Hkv, pfx::kRows, (long long)prefix_len, (long long)max_len);
   const int G = p.s.G, width = (H + 2 * Hkv) * 64;
   JX_CHECK_ARG(aligned16(qkv) && aligned16(kcache) && aligned16(vcache) && aligned16(workspace) &&
                    aligned16(kprefix) && aligned16(vprefix) && ((uintptr_t)out & 3) == 0,
@@ -603,13 +680,15 @@ extern "C" int jx_attn_decode_prefix(const void* qkv, int64_t ld_qkv, const void
   p.q_own_bytes = G * 128;
   p.q_own_stride = (G + 7) / 8 * 1024;
   p.q_pre_bytes = p.s.nb * G * 128;
-  const size_t smem = 1024 + 2 * p.q_own_stride + (1 + pfx::kKSlots + pfx::kVSlots) * pfx::kTile + sizeof(pfx::Bars);
+  constexpr size_t kFixed = 1024 + pfx::kQTile + (pfx::kKSlots + pfx::kVSlots + 1) * pfx::kTile + pfx::kOnes + sizeof(pfx::Bars);
+  static_assert(kFixed + 2 * 1024 + 1024 <= 233472 / 2, "two blocks an SM with up to eight heads a key / value head");
+  const size_t smem = kFixed + 2 * p.q_own_stride;
   static std::atomic<uint64_t> done{0};
   JX_CUDA_TRY(once_per_device(done,
                               [] {
                                 return cudaFuncSetAttribute(pfx::attn_prefix_part_kernel,
                                                             cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                                            1024 + 2 * 8192 + 6 * pfx::kTile + (int)sizeof(pfx::Bars));
+                                                            (int)(kFixed + 2 * pfx::kQTile));
                               }),
               name);
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
