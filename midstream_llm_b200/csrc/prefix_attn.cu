@@ -13,13 +13,18 @@
 //   [O^T; l] += [V^T; 1] P  (tcgen05, M 128 = 64 head columns and the sum's row, N rows, K 128 keys) -> TMEM
 // m is the row's maximum over the first tile and is raised only when a later P passes 2^8 (a rare step that
 // rescales O^T), so no other tile needs a maximum across threads. The sum l comes out of the same product from
-// the same rounded P, by a block of ones behind V^T. A sequence's own keys take the same way with its G heads
-// as rows.
+// the same rounded P, by a block of ones behind V^T.
 //
-// Work: the prefix tiles of all (row tile, key / value head) units stand in one line that is cut into equal runs, one
-// a block, so that each unit is split over a few blocks; the (sequence, head, chunk) items of the own keys
-// follow, dealt round robin. Each part leaves (m, l, o[64]) of its rows in the workspace, the second kernel joins
-// them. The schedule is fixed by the sizes, so results repeat bit for bit.
+// A sequence's own keys belong to no other, so a product has only its G heads as rows, and an item as short as a few
+// keys still pays the whole chain from TMA to the output (about 3 us). With up to four heads a key head they are
+// therefore scored by the second kernel, which joins the parts anyway, in plain fp32 arithmetic (one block per
+// sequence and key / value head, many blocks an SM; 64 sequences of 16 heads with a single own token: 21.5 ->
+// SHORTUS us). Larger groups, and few sequences with long own parts, which have to be split, take the matrix way.
+//
+// Work of the first kernel: the prefix tiles of all (row tile, key / value head) units stand in one line that is cut
+// into equal runs, one a block, so that each unit is split over a few blocks; the (sequence, head, chunk) items of
+// own keys, where it has them, follow, dealt round robin. Each part leaves (m, l, o[64]) of its rows in the
+// workspace, the second kernel joins them. The schedule is fixed by the sizes, so results repeat bit for bit.
 //
 // 192 threads, two blocks an SM (256 TMEM columns each):
 //   warp 0    TMA producer: Q of the item, K and V tiles (2 and 3 slots of 16 KB),
@@ -52,15 +57,20 @@ struct Sched {
   int B, G, Hkv, H;
   int nb;              // sequences per row tile
   int P, NT;           // prefix keys and tiles of one unit
-  int T, gp;           // prefix tiles in all, and blocks that share them
+  int T, gp;           // prefix tiles in all, and blocks that share them:
+  int per, more;       // `per` each, one more for the first `more` blocks
   int max_len, OC;     // own keys: upper bound, tiles per item
   int chunks;          // items of one (sequence, key / value head)
   int step_b, step_h;  // (sequence, head) distance of a block's consecutive items: grid = step_b Hkv + step_h
+  bool plain;          // own keys are left to the second kernel (chunks is 0)
   int nparts;          // parts a row has room for
   int nsp;             // of those, for the prefix
 
-  // Block that has prefix tile x: block c has [c T / gp, (c + 1) T / gp).
-  __host__ __device__ int block_of(int x) const { return (int)((((int64_t)x + 1) * gp - 1) / T); }
+  // Block that has prefix tile x.
+  __device__ int block_of(int x) const {
+    const int big = more * (per + 1);
+    return x < big ? x / (per + 1) : more + (x - big) / per;
+  }
 };
 
 __device__ __forceinline__ int own_length(const Sched& s, int raw) { return raw > 0 && raw <= s.max_len ? raw : 0; }
@@ -78,8 +88,8 @@ struct Cursor {
     const int c = blockIdx.x;
     t = t1 = 0;
     if (c < s.gp) {
-      t = (int)((int64_t)c * s.T / s.gp);
-      t1 = (int)((int64_t)(c + 1) * s.T / s.gp);
+      t = c * s.per + min(c, s.more);
+      t1 = t + s.per + (c < s.more ? 1 : 0);
     }
     const int own = gridDim.x - 1 - c;  // dealt from the last block on: those may have no prefix tiles
     ob = own / s.Hkv;
@@ -138,7 +148,7 @@ struct Bars {
   alignas(16) float m[kRows];        // reference of each row, log2 units; +inf for columns without a row
   alignas(16) float alpha[kRows];    // factor of a raised reference
   alignas(16) float wmax[4][kRows];  // each warp's maxima
-  int at[kRows];                     // place of each row's part in the workspace
+  alignas(16) int at[kRows];         // place of each row's part in the workspace
   int lens[kLens];
 };
 
@@ -191,6 +201,9 @@ __device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, u
       "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z)
       : "memory");
 }
+
+// Until the kernel before this one is done and what it wrote is visible.
+__device__ __forceinline__ void prior_kernel_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
 __device__ __forceinline__ float ex2(float x) {
   float y;
@@ -247,10 +260,8 @@ __device__ __forceinline__ bool softmax_item(const Params& p, Cursor& c, const i
     tc_fence_after();
     uint32_t sr[W];
     load_cols(base + x * 64, sr);
-    tc_fence_before();
-    __syncwarp();
-    if (lane == 0) mbar_arrive(&bars->s_free[x]);  // the scores are in registers
-    if (c.key() + BKV > c.limit && c.key() + key >= c.limit) {  // a key past the end
+    const bool past = c.key() + key >= c.limit;  // a key past the end
+    if (past) {
 #pragma unroll
       for (int i = 0; i < W; ++i) sr[i] = 0xff800000u;
     }
@@ -275,15 +286,19 @@ __device__ __forceinline__ bool softmax_item(const Params& p, Cursor& c, const i
     bool raise = c.j == 0;
     if (!raise) raise = softmax_any(probabilities());
     if (raise) {
-      // Maxima over the tile's keys, per warp, then over the warps.
+      // Maxima over the tile's keys, per warp, then over the warps. A loop, like every part that runs once an item: cold
+      // straight code costs more in instruction fetches than it saves.
+#pragma unroll 1
+      for (int i = 0; i < W; i += 8) {
+        uint32_t u[8];
+        load_cols(base + x * 64 + i, u);
+        float w[8];
 #pragma unroll
-      for (int i = 0; i < W; i += 4) {
-        float4 w;
-        w.x = redux_max(__uint_as_float(sr[i]));
-        w.y = redux_max(__uint_as_float(sr[i + 1]));
-        w.z = redux_max(__uint_as_float(sr[i + 2]));
-        w.w = redux_max(__uint_as_float(sr[i + 3]));
-        if (lane == 0) *reinterpret_cast<float4*>(&bars->wmax[quarter][i]) = w;
+        for (int k = 0; k < 8; ++k) w[k] = redux_max(past ? -INFINITY : __uint_as_float(u[k]));
+        if (lane == 0) {
+          *reinterpret_cast<float4*>(&bars->wmax[quarter][i]) = make_float4(w[0], w[1], w[2], w[3]);
+          *reinterpret_cast<float4*>(&bars->wmax[quarter][i + 4]) = make_float4(w[4], w[5], w[6], w[7]);
+        }
       }
       softmax_any(false);
       const int i = threadIdx.x - 64;
@@ -305,11 +320,14 @@ __device__ __forceinline__ bool softmax_item(const Params& p, Cursor& c, const i
       softmax_any(false);
       probabilities();
     }
+    tc_fence_before();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&bars->s_free[x]);  // the scores have been read
     // The product of the tile before must be done before P is overwritten or [O^T; l] rescaled.
     if (g > 0 && !warp_wait(&bars->p_empty, (g - 1) & 1, abort_flag, status, kSoftmax)) return false;
     if (raise && c.j > 0) {
       tc_fence_after();
-#pragma unroll
+#pragma unroll 1
       for (int q = 0; q < W; q += 8) {
         uint32_t orr[8];
         load_cols(base + 128 + q, orr);
@@ -332,20 +350,22 @@ __device__ __forceinline__ bool softmax_item(const Params& p, Cursor& c, const i
   if (!warp_wait(&bars->p_empty, (g - 1) & 1, abort_flag, status, kSoftmax)) return false;
   tc_fence_after();
   if (quarter < 3) {
-#pragma unroll
-    for (int q = 0; q < W; q += 8) {
+#pragma unroll 1
+    for (int q = 0; q < rows; q += 8) {
       uint32_t orr[8];
       load_cols(base + 128 + q, orr);
+      int at[8];
+      *reinterpret_cast<int4*>(&at[0]) = *reinterpret_cast<const int4*>(&bars->at[q]);
+      *reinterpret_cast<int4*>(&at[4]) = *reinterpret_cast<const int4*>(&bars->at[q + 4]);
+      if (quarter < 2) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int r = q + i;
-        if (r < rows) {
-          const int64_t at = bars->at[r];
-          if (quarter < 2)
-            p.o[at * D + key] = __uint_as_float(orr[i]);
-          else if (lane == 0)
-            p.ml[at] = make_float2(bars->m[r], __uint_as_float(orr[i]));
-        }
+        for (int i = 0; i < 8; ++i)
+          if (q + i < rows) p.o[(int64_t)at[i] * D + key] = __uint_as_float(orr[i]);
+      } else {  // every lane has every sum: lane i takes row q + i
+        uint32_t l = orr[0];
+#pragma unroll
+        for (int i = 1; i < 8; ++i) l = lane == i ? orr[i] : l;
+        if (lane < 8 && q + lane < rows) p.ml[bars->at[q + lane]] = make_float2(bars->m[q + lane], __uint_as_float(l));
       }
     }
   }
@@ -376,6 +396,10 @@ __global__ void __launch_bounds__(kThreads, 2)
   const Sched& s = p.s;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
+  if (threadIdx.x == 32) {
+    tma_prefetch_desc(&tm_qp), tma_prefetch_desc(&tm_kp), tma_prefetch_desc(&tm_vp);
+    if (s.chunks > 0) tma_prefetch_desc(&tm_qo), tma_prefetch_desc(&tm_kc), tma_prefetch_desc(&tm_vc);
+  }
   if (threadIdx.x == 0) {
     for (int i = 0; i < kKSlots; ++i) mbar_init(&bars->k_full[i], 1), mbar_init(&bars->k_empty[i], 1);
     for (int i = 0; i < kVSlots; ++i) mbar_init(&bars->v_full[i], 1), mbar_init(&bars->v_empty[i], 1);
@@ -386,15 +410,17 @@ __global__ void __launch_bounds__(kThreads, 2)
     bars->abort = 0;
     fence_barrier_init();
   }
-  const bool staged = s.B <= kLens;
-  if (staged)
-    for (int i = threadIdx.x; i < s.B; i += kThreads) bars->lens[i] = p.lens[i];
-  for (int i = threadIdx.x; i < (int)kOnes / 4; i += kThreads) reinterpret_cast<uint32_t*>(s1)[i] = 0x3c003c00u;
-  fence_proxy_async_smem();
   if (warp == 1) {
     tmem_alloc(&bars->tmem_base, kTmemCols);
     tmem_relinquish();
   }
+  for (int i = threadIdx.x; i < (int)kOnes / 4; i += kThreads) reinterpret_cast<uint32_t*>(s1)[i] = 0x3c003c00u;
+  fence_proxy_async_smem();
+  prior_kernel_wait();  // what is above may run while the kernel before finishes
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the second kernel's blocks may use what is free
+  const bool staged = s.B <= kLens;
+  if (staged)
+    for (int i = threadIdx.x; i < s.B; i += kThreads) bars->lens[i] = p.lens[i];
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -405,28 +431,52 @@ __global__ void __launch_bounds__(kThreads, 2)
 
   if (warp == 0) {
     if (lane == 0) {
-      for (uint32_t tile = 0; c.advance(s, lens); ++tile) {
-        if (c.j == 0) {
+      // K and V take turns as their slots come free: V's are held longer, and K must not wait behind them.
+      bool more_k = c.advance(s, lens), more_v = more_k;
+      Cursor v = c;
+      uint32_t nk = 0, nv = 0;
+      long long since = clock64();
+      while (more_k || more_v) {
+        bool idle = true;
+        const uint32_t ks = nk % kKSlots, vs = nv % kVSlots;
+        if (more_k && mbar_test_wait(&bars->k_empty[ks], ((nk / kKSlots) & 1) ^ 1)) {
           const int q = c.is_own ? (c.iown & 1) : 2;
           const uint32_t use = c.is_own ? (uint32_t)(c.iown >> 1) : (uint32_t)c.ipre;
-          if (!wait(&bars->q_empty[q], (use & 1) ^ 1, abort_flag, status, kProducer)) break;
-          mbar_expect_tx(&bars->q_full[q], c.is_own ? p.q_own_bytes : p.q_pre_bytes);
-          tma_load_3d(q == 2 ? sQp : sQ + q * p.q_own_stride, c.is_own ? &tm_qo : &tm_qp, &bars->q_full[q], 0, c.h * s.G,
-                      c.b);
+          if (c.j > 0 || mbar_test_wait(&bars->q_empty[q], (use & 1) ^ 1)) {
+            if (c.j == 0) {
+              mbar_expect_tx(&bars->q_full[q], c.is_own ? p.q_own_bytes : p.q_pre_bytes);
+              tma_load_3d(q == 2 ? sQp : sQ + q * p.q_own_stride, c.is_own ? &tm_qo : &tm_qp, &bars->q_full[q], 0, c.h * s.G,
+                          c.b);
+            }
+            mbar_expect_tx(&bars->k_full[ks], kTile);
+            if (c.is_own)
+              tma_load_3d(sK + ks * kTile, &tm_kc, &bars->k_full[ks], c.h * D, c.key(), c.b);
+            else
+              tma_load_2d(sK + ks * kTile, &tm_kp, &bars->k_full[ks], c.h * D, c.key());
+            more_k = c.advance(s, lens);
+            ++nk;
+            idle = false;
+          }
         }
-        const uint32_t ks = tile % kKSlots, vs = tile % kVSlots;
-        if (!wait(&bars->k_empty[ks], ((tile / kKSlots) & 1) ^ 1, abort_flag, status, kProducer)) break;
-        mbar_expect_tx(&bars->k_full[ks], kTile);
-        if (c.is_own)
-          tma_load_3d(sK + ks * kTile, &tm_kc, &bars->k_full[ks], c.h * D, c.key(), c.b);
-        else
-          tma_load_2d(sK + ks * kTile, &tm_kp, &bars->k_full[ks], c.h * D, c.key());
-        if (!wait(&bars->v_empty[vs], ((tile / kVSlots) & 1) ^ 1, abort_flag, status, kProducer)) break;
-        mbar_expect_tx(&bars->v_full[vs], kTile);
-        if (c.is_own)
-          tma_load_3d(sV + vs * kTile, &tm_vc, &bars->v_full[vs], c.h * D, c.key(), c.b);
-        else
-          tma_load_2d(sV + vs * kTile, &tm_vp, &bars->v_full[vs], c.h * D, c.key());
+        if (more_v && mbar_test_wait(&bars->v_empty[vs], ((nv / kVSlots) & 1) ^ 1)) {
+          mbar_expect_tx(&bars->v_full[vs], kTile);
+          if (v.is_own)
+            tma_load_3d(sV + vs * kTile, &tm_vc, &bars->v_full[vs], v.h * D, v.key(), v.b);
+          else
+            tma_load_2d(sV + vs * kTile, &tm_vp, &bars->v_full[vs], v.h * D, v.key());
+          more_v = v.advance(s, lens);
+          ++nv;
+          idle = false;
+        }
+        if (!idle) {
+          since = clock64();
+        } else if (*abort_flag) {
+          break;
+        } else if (clock64() - since > (1ll << 32)) {
+          *abort_flag = 1;
+          if (status) atomicExch(status, kProducer);
+          break;
+        }
       }
     }
     __syncwarp();
@@ -540,7 +590,7 @@ __global__ void __launch_bounds__(128) attn_prefix_join_kernel(const Params p, i
   const int row = blockIdx.x, b = row / s.H, hq = row - b * s.H;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int raw = p.lens[b], len = own_length(s, raw);
-  asm volatile("griddepcontrol.wait;" ::: "memory");
+  prior_kernel_wait();
   __half2* dst = reinterpret_cast<__half2*>(p.out + (int64_t)b * p.ld_out + hq * D);
   if (len == 0) {
     if (raw > s.max_len && threadIdx.x == 0 && hq == 0 && status) atomicExch(status, kStatusDecodeBadLength);
@@ -586,6 +636,185 @@ __global__ void __launch_bounds__(128) attn_prefix_join_kernel(const Params p, i
   dst[lane] = __floats2half2_rn(acc.x / L, acc.y / L);
 }
 
+// The same with the own keys: a block per (sequence, key / value head), NT threads. A warp takes 4 U keys at a time, eight
+// lanes to a key (16 bytes each), four keys side by side, and every lane group keeps its own running (m, l, o) of the
+// keys it has seen; the prefix's parts are then added by warps (a lane two columns), and all partial results meet in
+// shared memory. Only the parts wait for the first kernel, so a block begins while that still runs.
+template <int G, int NT, int U>
+__global__ void __launch_bounds__(NT) attn_prefix_own_kernel(const Params p, int* status) {
+  constexpr int NW = NT / 32;
+  __shared__ float so[2 * NW][G][D];
+  __shared__ float sm[2 * NW][G], sl[2 * NW][G];
+  const Sched& s = p.s;
+  const int b = blockIdx.x / s.Hkv, h = blockIdx.x - b * s.Hkv;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int raw = p.lens[b], len = own_length(s, raw);
+  __half* dst = p.out + (int64_t)b * p.ld_out + h * G * D;
+  if (len == 0) {
+    if (raw > s.max_len && threadIdx.x == 0 && h == 0 && status) atomicExch(status, kStatusDecodeBadLength);
+    for (int i = threadIdx.x; i < G * D; i += NT) dst[i] = __ushort_as_half(0);
+    prior_kernel_wait();
+    return;
+  }
+  const __half* row = p.qkv + (int64_t)b * p.ld_qkv;
+  __half* kc = p.kcache + (int64_t)b * p.batch_stride + h * D;
+  __half* vc = p.vcache + (int64_t)b * p.batch_stride + h * D;
+  const __half* nk = row + (s.H + h) * D;
+  const __half* nv = nk + s.Hkv * D;
+  const int part = (lane & 7) * 8;
+  float q[G][8], m[G], l[G], o[G][8];
+#pragma unroll
+  for (int g = 0; g < G; ++g) {
+    const uint4 u = *reinterpret_cast<const uint4*>(row + (h * G + g) * D + part);
+    const __half2* hq = reinterpret_cast<const __half2*>(&u);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float2 f = __half22float2(hq[j]);
+      q[g][2 * j] = f.x * p.scale_log2, q[g][2 * j + 1] = f.y * p.scale_log2;
+    }
+    m[g] = -INFINITY, l[g] = 0.f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) o[g][j] = 0.f;
+  }
+  // The new key and value: appended, and read from their row of qkv below.
+  if (threadIdx.x < 16) {
+    const int ch = (threadIdx.x & 7) * 8;
+    const bool is_v = threadIdx.x >= 8;
+    *reinterpret_cast<uint4*>((is_v ? vc : kc) + (int64_t)(len - 1) * p.ld_cache + ch) =
+        *reinterpret_cast<const uint4*>((is_v ? nv : nk) + ch);
+  }
+  for (int k0 = warp * 4 * U; k0 < len; k0 += NW * 4 * U) {
+    uint4 ku[U], vu[U];
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      const int k = k0 + i * 4 + (lane >> 3);
+      ku[i] = vu[i] = make_uint4(0, 0, 0, 0);
+      if (k < len) {
+        const bool fresh = k == len - 1;
+        ku[i] = *reinterpret_cast<const uint4*>((fresh ? nk : kc + (int64_t)k * p.ld_cache) + part);
+        vu[i] = *reinterpret_cast<const uint4*>((fresh ? nv : vc + (int64_t)k * p.ld_cache) + part);
+      }
+    }
+    float sc[G][U];
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      const __half2* hk = reinterpret_cast<const __half2*>(&ku[i]);
+      float f[8];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float2 x = __half22float2(hk[j]);
+        f[2 * j] = x.x, f[2 * j + 1] = x.y;
+      }
+#pragma unroll
+      for (int g = 0; g < G; ++g) {
+        float a = 0.f, c = 0.f;
+#pragma unroll
+        for (int j = 0; j < 8; j += 2) a = fmaf(q[g][j], f[j], a), c = fmaf(q[g][j + 1], f[j + 1], c);
+        sc[g][i] = a + c;
+      }
+    }
+#pragma unroll
+    for (int x = 1; x < 8; x <<= 1)
+#pragma unroll
+      for (int g = 0; g < G; ++g)
+#pragma unroll
+        for (int i = 0; i < U; ++i) sc[g][i] += __shfl_xor_sync(0xffffffffu, sc[g][i], x);
+#pragma unroll
+    for (int g = 0; g < G; ++g) {
+      float nm = m[g];
+#pragma unroll
+      for (int i = 0; i < U; ++i) {
+        if (k0 + i * 4 + (lane >> 3) >= len) sc[g][i] = -INFINITY;
+        nm = fmaxf(nm, sc[g][i]);
+      }
+      const float a = nm == -INFINITY ? 1.f : ex2(m[g] - nm);  // no key of this lane group yet
+      l[g] *= a;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) o[g][j] *= a;
+      m[g] = nm;
+#pragma unroll
+      for (int i = 0; i < U; ++i) {
+        sc[g][i] = nm == -INFINITY ? 0.f : ex2(sc[g][i] - nm);
+        l[g] += sc[g][i];
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      const __half2* hv = reinterpret_cast<const __half2*>(&vu[i]);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float2 x = __half22float2(hv[j]);
+#pragma unroll
+        for (int g = 0; g < G; ++g) {
+          o[g][2 * j] = fmaf(sc[g][i], x.x, o[g][2 * j]);
+          o[g][2 * j + 1] = fmaf(sc[g][i], x.y, o[g][2 * j + 1]);
+        }
+      }
+    }
+  }
+  // The four lane groups of the warp, then the warp's result to shared memory.
+#pragma unroll
+  for (int g = 0; g < G; ++g) {
+    float wm = fmaxf(m[g], __shfl_xor_sync(0xffffffffu, m[g], 8));
+    wm = fmaxf(wm, __shfl_xor_sync(0xffffffffu, wm, 16));
+    const float a = m[g] == -INFINITY ? 0.f : ex2(m[g] - wm);
+    l[g] *= a;
+    l[g] += __shfl_xor_sync(0xffffffffu, l[g], 8);
+    l[g] += __shfl_xor_sync(0xffffffffu, l[g], 16);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      o[g][j] *= a;
+      o[g][j] += __shfl_xor_sync(0xffffffffu, o[g][j], 8);
+      o[g][j] += __shfl_xor_sync(0xffffffffu, o[g][j], 16);
+    }
+    if (lane < 8) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) so[warp][g][part + j] = o[g][j];
+    }
+    if (lane == 0) sm[warp][g] = wm, sl[warp][g] = l[g];
+  }
+  prior_kernel_wait();
+  int npre = 0;
+  if (s.T > 0) {
+    const int unit = b / s.nb * s.Hkv + h;
+    npre = s.block_of(unit * s.NT + s.NT - 1) - s.block_of(unit * s.NT) + 1;
+  }
+#pragma unroll
+  for (int g = 0; g < G; ++g) {
+    const int64_t at = ((int64_t)b * s.H + h * G + g) * s.nparts;
+    float M = -INFINITY, L = 0.f;
+    float2 acc = make_float2(0.f, 0.f);
+#pragma unroll 4
+    for (int i = warp; i < npre; i += NW) {
+      const float2 ml = p.ml[at + i];
+      const float2 v = *reinterpret_cast<const float2*>(p.o + (at + i) * D + 2 * lane);
+      const float nm = fmaxf(M, ml.x);
+      const float a = M == -INFINITY ? 0.f : ex2(M - nm), w = ex2(ml.x - nm);
+      L = L * a + ml.y * w;
+      acc.x = acc.x * a + v.x * w;
+      acc.y = acc.y * a + v.y * w;
+      M = nm;
+    }
+    *reinterpret_cast<float2*>(&so[NW + warp][g][2 * lane]) = acc;
+    if (lane == 0) sm[NW + warp][g] = M, sl[NW + warp][g] = L;
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < G * D; i += NT) {
+    const int g = i / D, d = i % D;
+    float M = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < 2 * NW; ++w) M = fmaxf(M, sm[w][g]);
+    float L = 0.f, a = 0.f;
+#pragma unroll
+    for (int w = 0; w < 2 * NW; ++w) {
+      const float e = sm[w][g] == -INFINITY ? 0.f : ex2(sm[w][g] - M);
+      L = fmaf(sl[w][g], e, L);
+      a = fmaf(so[w][g][d], e, a);
+    }
+    dst[i] = __float2half_rn(a / L);
+  }
+}
+
 // The schedule, from sizes and the SM count alone.
 bool plan(int B, int H, int Hkv, int64_t prefix_len, int64_t max_len, Sched* s, int* grid) {
   if (B <= 0 || Hkv <= 0 || H <= 0 || H % Hkv || H / Hkv > kRows || prefix_len < 0 || max_len <= 0) return false;
@@ -601,17 +830,23 @@ bool plan(int B, int H, int Hkv, int64_t prefix_len, int64_t max_len, Sched* s, 
   if (T >= (1ll << 31) || own_all >= (1ll << 31)) return false;
   s->T = (int)T;
   s->gp = (int)std::min<int64_t>(T, blocks);
+  s->per = s->gp > 0 ? s->T / s->gp : 0;
+  s->more = s->gp > 0 ? s->T % s->gp : 0;
   s->max_len = (int)max_len;
+  // One block per pair reads at most 512 keys, or there are pairs enough to fill the GPU; up to four heads' state in
+  // registers.
+  s->plain = s->G <= 4 && (max_len <= 512 || (int64_t)B * Hkv >= blocks);
   // Enough items to even out ragged lengths, few parts to join.
   s->OC = (int)std::max<int64_t>(1, (own_all + 3 * blocks - 1) / (3 * blocks));
   s->OC = std::min(s->OC, own_tiles);
-  s->chunks = (own_tiles + s->OC - 1) / s->OC;
-  s->nsp = T > 0 ? (int)std::min<int64_t>(s->NT, ((int64_t)s->NT * s->gp + T - 1) / T + 1) : 0;
+  s->chunks = s->plain ? 0 : (own_tiles + s->OC - 1) / s->OC;
+  s->nsp = T > 0 ? std::min(s->NT, (s->NT - 1 + s->per - 1) / s->per + 1) : 0;  // blocks that a unit may be split over
   s->nparts = s->nsp + s->chunks;
   if ((int64_t)B * H * s->nparts >= (1ll << 31)) return false;
   *grid = (int)std::min<int64_t>(blocks, std::max<int64_t>(s->gp, T + (int64_t)B * Hkv * s->chunks));
   s->step_b = *grid / Hkv;
   s->step_h = *grid % Hkv;
+  if (s->nparts == 0) s->nparts = 1;
   return true;
 }
 
@@ -693,19 +928,39 @@ extern "C" int jx_attn_decode_prefix(const void* qkv, int64_t ld_qkv, const void
               name);
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   int* status = status_ptr();
-  pfx::attn_prefix_part_kernel<<<grid, pfx::kThreads, smem, st>>>(qp, qo, kp, vp, kc, vc, p, status);
-  JX_CHECK_LAUNCH(name);
-  // The join kernel's blocks may start while the last parts are written; they wait before they read them.
+  // Both kernels may be set up while the one before them finishes; they wait before they read what it wrote.
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(B * H);
-  cfg.blockDim = dim3(128);
   cfg.stream = st;
   cudaLaunchAttribute attr;
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr.val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  JX_CUDA_TRY(cudaLaunchKernelEx(&cfg, pfx::attn_prefix_join_kernel, p, status), name);
+  if (grid > 0) {
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(pfx::kThreads);
+    cfg.dynamicSmemBytes = smem;
+    JX_CUDA_TRY(cudaLaunchKernelEx(&cfg, pfx::attn_prefix_part_kernel, qp, qo, kp, vp, kc, vc, p, status), name);
+    JX_CHECK_LAUNCH(name);
+  } else {
+    cfg.numAttrs = 0;  // no prefix: the second kernel alone, which reads before it waits
+  }
+  cfg.dynamicSmemBytes = 0;
+  if (p.s.plain) {
+    // Eight warps where one head's sequences may have more than 128 keys of their own, else four; two steps' keys in
+    // flight with several heads, whose state takes the registers.
+    const int NT = G == 1 && max_len > 128 ? 256 : 128;
+    void (*own[4])(const pfx::Params, int*) = {
+        NT == 256 ? pfx::attn_prefix_own_kernel<1, 256, 4> : pfx::attn_prefix_own_kernel<1, 128, 4>,
+        pfx::attn_prefix_own_kernel<2, 128, 2>, pfx::attn_prefix_own_kernel<3, 128, 2>, pfx::attn_prefix_own_kernel<4, 128, 2>};
+    cfg.gridDim = dim3(B * Hkv);
+    cfg.blockDim = dim3(NT);
+    JX_CUDA_TRY(cudaLaunchKernelEx(&cfg, own[G - 1], p, status), name);
+  } else {
+    cfg.gridDim = dim3(B * H);
+    cfg.blockDim = dim3(128);
+    JX_CUDA_TRY(cudaLaunchKernelEx(&cfg, pfx::attn_prefix_join_kernel, p, status), name);
+  }
   JX_CHECK_LAUNCH(name);
   return JX_OK;
 }

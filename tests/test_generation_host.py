@@ -36,9 +36,9 @@ def test_prefix_workspace_query():
     from midstream_llm_b200 import _lib, ops
     need = lambda *a: _lib.query("jx_attn_decode_prefix_workspace_bytes", *a)  # noqa: E731
     assert need(0, 4, 4, 10, 10) == need(1, 4, 3, 10, 10) == need(1, 4, 4, -1, 10) == need(1, 4, 4, 10, 0) == -1
-    # every row has room for at least one part of the prefix and one of its own keys: (m, l) and 64 sums
+    # every row has room for at least one part: (m, l) and 64 sums
     for B, H, kv, P, S in ((1, 4, 4, 1, 1), (16, 16, 16, 1791, 257), (64, 16, 4, 40000, 1000), (300, 2, 1, 129, 5)):
-        assert need(B, H, kv, P, S) >= B * H * 2 * (8 + 256)
+        assert need(B, H, kv, P, S) >= B * H * (8 + 256)
         assert need(B, H, kv, 0, S) >= B * H * (8 + 256)
     with pytest.raises(ValueError, match="unsupported shape"):
         ops.attn_decode_prefix_workspace_bytes(2, 130, 1, 10, 10)
@@ -111,12 +111,14 @@ def test_prefix_schedule_gives_every_tile_to_one_block():
         NT, units, blocks = r.randint(1, 300), r.randint(1, 70), r.choice([2, 20, 296])
         T = NT * units
         gp = min(T, blocks)
-        starts = [c * T // gp for c in range(gp + 1)]
+        per, more = T // gp, T % gp
+        starts = [c * per + min(c, more) for c in range(gp + 1)]
         assert starts[0] == 0 and starts[-1] == T and all(b > a for a, b in zip(starts, starts[1:]))
-        block_of = lambda x: ((x + 1) * gp - 1) // T  # noqa: E731
+        big = more * (per + 1)
+        block_of = lambda x: x // (per + 1) if x < big else more + (x - big) // per  # noqa: E731
         for x in {0, T - 1, *(r.randrange(T) for _ in range(5))}:
             c = block_of(x)
             assert starts[c] <= x < starts[c + 1]
-        room = min(NT, (NT * gp + T - 1) // T + 1)
+        room = min(NT, -(-(NT - 1) // per) + 1)
         for u in range(units):
             assert block_of(u * NT + NT - 1) - block_of(u * NT) + 1 <= room
