@@ -26,11 +26,13 @@
 // own keys, where it has them, follow, dealt round robin. Each part leaves (m, l, o[64]) of its rows in the
 // workspace, the second kernel joins them. The schedule is fixed by the sizes, so results repeat bit for bit.
 //
-// 192 threads, two blocks an SM (256 TMEM columns each):
+// 224 threads, two blocks an SM (256 TMEM columns each):
 //   warp 0    TMA producer: Q of the item, K and V tiles (2 and 3 slots of 16 KB),
-//   warp 1    MMA issuer; before the tile that holds a sequence's end it puts the new key and value into the
-//             tile (and the cache) and clears the values behind them, since 0 * garbage may be NaN,
-//   warps 2-5 softmax, one key per thread, and the parts' output.
+//   warp 1    issues the first products; before the tile that holds a sequence's end it puts the new key and value
+//             into the tile (and the cache) and clears the values behind them, since 0 * garbage may be NaN,
+//   warps 2-5 softmax, one key per thread, and the parts' output,
+//   warp 6    issues the second products (one thread issuing both was the slowest link: its twelve products, their
+//             waits and commits followed each other, PVUS us against SPLITUS us at 64 rows of 32749 keys).
 #include <algorithm>
 #include <atomic>
 
@@ -43,7 +45,7 @@ namespace pfx {
 constexpr int D = 64;
 constexpr int BKV = 128;
 constexpr int kRows = 64;  // query rows of a tile at most
-constexpr int kThreads = 192;
+constexpr int kThreads = 224;
 constexpr uint32_t kTile = BKV * D * 2;   // 16 KiB
 constexpr uint32_t kQTile = kRows * D * 2;  // 8 KiB
 constexpr uint32_t kOnes = 2048;          // 16 keys x 64 ones
@@ -145,7 +147,7 @@ struct Bars {
   uint64_t s_full[2], s_free[2], p_full, p_empty;
   uint32_t tmem_base;
   int abort;
-  alignas(16) float m[kRows];        // reference of each row, log2 units; +inf for columns without a row
+  alignas(16) float m[kRows];        // minus each row's reference, log2 units; -inf for columns without a row
   alignas(16) float alpha[kRows];    // factor of a raised reference
   alignas(16) float wmax[4][kRows];  // each warp's maxima
   alignas(16) int at[kRows];         // place of each row's part in the workspace
@@ -186,6 +188,13 @@ __device__ __forceinline__ bool softmax_any(bool flag) {
       : "r"((uint32_t)flag)
       : "memory");
   return r != 0;
+}
+
+// max(a, b, c) in one instruction (sm_100).
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
 }
 
 __device__ __forceinline__ float redux_max(float v) {
@@ -261,30 +270,30 @@ __device__ __forceinline__ bool softmax_item(const Params& p, Cursor& c, const i
     uint32_t sr[W];
     load_cols(base + x * 64, sr);
     const bool past = c.key() + key >= c.limit;  // a key past the end
-    if (past) {
+    // The scores become exponents against the references; true if one passes the bound.
+    auto exponents = [&]() -> bool {
+      float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+      constexpr int B = W < 16 ? W : 16;  // columns whose references are read ahead of their use
+      const float2 sc = make_float2(scale, scale);
 #pragma unroll
-      for (int i = 0; i < W; ++i) sr[i] = 0xff800000u;
-    }
-    uint32_t pw[W / 2];
-    // P of this thread's key; true if one of them passes the bound.
-    auto probabilities = [&]() -> bool {
-      float top[4] = {0.f, 0.f, 0.f, 0.f};
+      for (int i0 = 0; i0 < W; i0 += B) {
+        float4 m[B / 4];
 #pragma unroll
-      for (int i = 0; i < W; i += 4) {
-        const float4 m = *reinterpret_cast<const float4*>(&bars->m[i]);
-        const float p0 = ex2(fmaf(__uint_as_float(sr[i]), scale, -m.x));
-        const float p1 = ex2(fmaf(__uint_as_float(sr[i + 1]), scale, -m.y));
-        const float p2 = ex2(fmaf(__uint_as_float(sr[i + 2]), scale, -m.z));
-        const float p3 = ex2(fmaf(__uint_as_float(sr[i + 3]), scale, -m.w));
-        top[(i >> 2) & 3] = fmaxf(top[(i >> 2) & 3], fmaxf(fmaxf(p0, p1), fmaxf(p2, p3)));
-        const __half2 h0 = __floats2half2_rn(p0, p1), h1 = __floats2half2_rn(p2, p3);
-        pw[i / 2] = *reinterpret_cast<const uint32_t*>(&h0);
-        pw[i / 2 + 1] = *reinterpret_cast<const uint32_t*>(&h1);
+        for (int i = 0; i < B / 4; ++i) m[i] = *reinterpret_cast<const float4*>(&bars->m[i0 + 4 * i]);
+#pragma unroll
+        for (int i = 0; i < B / 4; ++i) {
+          uint32_t* r = &sr[i0 + 4 * i];
+          const float2 y0 = __ffma2_rn(make_float2(__uint_as_float(r[0]), __uint_as_float(r[1])), sc, make_float2(m[i].x, m[i].y));
+          const float2 y1 = __ffma2_rn(make_float2(__uint_as_float(r[2]), __uint_as_float(r[3])), sc, make_float2(m[i].z, m[i].w));
+          top[i & 3] = max3(max3(top[i & 3], y0.x, y0.y), y1.x, y1.y);
+          r[0] = __float_as_uint(y0.x), r[1] = __float_as_uint(y0.y);
+          r[2] = __float_as_uint(y1.x), r[3] = __float_as_uint(y1.y);
+        }
       }
-      return fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) > 256.f;
+      return !past && fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) > 8.f;
     };
     bool raise = c.j == 0;
-    if (!raise) raise = softmax_any(probabilities());
+    if (!raise) raise = softmax_any(exponents());
     if (raise) {
       // Maxima over the tile's keys, per warp, then over the warps. A loop, like every part that runs once an item: cold
       // straight code costs more in instruction fetches than it saves.
@@ -307,7 +316,7 @@ __device__ __forceinline__ bool softmax_item(const Params& p, Cursor& c, const i
         if (i < rows) {
           mx = fmaxf(fmaxf(bars->wmax[0][i], bars->wmax[1][i]), fmaxf(bars->wmax[2][i], bars->wmax[3][i])) * scale;
           if (c.j > 0) {
-            const float old = bars->m[i];
+            const float old = -bars->m[i];
             mx = fmaxf(mx, old);
             bars->alpha[i] = ex2(old - mx);
           } else {
@@ -315,10 +324,11 @@ __device__ __forceinline__ bool softmax_item(const Params& p, Cursor& c, const i
             bars->at[i] = ((c.b + sq) * s.H + c.h * s.G + i - sq * s.G) * s.nparts + c.part;
           }
         }
-        bars->m[i] = mx;
+        bars->m[i] = -mx;
       }
       softmax_any(false);
-      probabilities();
+      load_cols(base + x * 64, sr);
+      exponents();
     }
     tc_fence_before();
     __syncwarp();
@@ -339,9 +349,16 @@ __device__ __forceinline__ bool softmax_item(const Params& p, Cursor& c, const i
       tc_fence_before();
     }
 #pragma unroll
-    for (int q = 0; q < W / 8; ++q)
-      *reinterpret_cast<uint4*>(prow + ((q ^ (key & 7)) << 4)) =
-          make_uint4(pw[q * 4], pw[q * 4 + 1], pw[q * 4 + 2], pw[q * 4 + 3]);
+    for (int q = 0; q < W / 8; ++q) {
+      uint32_t pw[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float p0 = ex2(__uint_as_float(sr[q * 8 + 2 * e])), p1 = ex2(__uint_as_float(sr[q * 8 + 2 * e + 1]));
+        const __half2 hp = __floats2half2_rn(p0, p1);
+        pw[e] = past ? 0u : *reinterpret_cast<const uint32_t*>(&hp);
+      }
+      *reinterpret_cast<uint4*>(prow + ((q ^ (key & 7)) << 4)) = make_uint4(pw[0], pw[1], pw[2], pw[3]);
+    }
     fence_proxy_async_smem();
     __syncwarp();
     if (lane == 0) mbar_arrive(&bars->p_full);
@@ -365,7 +382,7 @@ __device__ __forceinline__ bool softmax_item(const Params& p, Cursor& c, const i
         uint32_t l = orr[0];
 #pragma unroll
         for (int i = 1; i < 8; ++i) l = lane == i ? orr[i] : l;
-        if (lane < 8 && q + lane < rows) p.ml[bars->at[q + lane]] = make_float2(bars->m[q + lane], __uint_as_float(l));
+        if (lane < 8 && q + lane < rows) p.ml[bars->at[q + lane]] = make_float2(-bars->m[q + lane], __uint_as_float(l));
       }
     }
   }
@@ -482,18 +499,14 @@ __global__ void __launch_bounds__(kThreads, 2)
     __syncwarp();
   } else if (warp == 1) {
     const uint64_t dK0 = smem_desc_sw128(smem_u32(sK), 16, 1024);
-    const uint64_t dP0 = smem_desc_sw128(smem_u32(sP), 8192, 1024);
-    // Of the last issued S^T, for its product with V: the row tile's width and whether it begins an item.
-    uint32_t width = 16;
-    bool first = true;
-    auto issue_s = [&](uint32_t ts, int x) -> bool {  // x = ts & 1
+    const uint64_t dQ0 = smem_desc_sw128(smem_u32(sQ), 16, 1024), dQp = smem_desc_sw128(smem_u32(sQp), 16, 1024);
+    for (uint32_t ts = 0; c.advance(s, lens); ++ts) {
+      const int x = ts & 1;
       const uint32_t ks = ts % kKSlots, vs = ts % kVSlots;
       const int q = c.is_own ? (c.iown & 1) : 2;
-      width = (uint32_t)(c.rows(s) + 15) & ~15u;
-      first = c.j == 0;
       if (c.j == 0) {
         const uint32_t use = c.is_own ? (uint32_t)(c.iown >> 1) : (uint32_t)c.ipre;
-        if (!warp_wait(&bars->q_full[q], use & 1, abort_flag, status, kMma)) return false;
+        if (!warp_wait(&bars->q_full[q], use & 1, abort_flag, status, kMma)) break;
       }
       const bool ends = c.ends();
       const bool is_v = lane >= 8;
@@ -501,10 +514,10 @@ __global__ void __launch_bounds__(kThreads, 2)
       uint4 fresh = make_uint4(0, 0, 0, 0);  // lanes 0-7: the new key, 8-15: the new value
       if (ends && lane < 16)
         fresh = *reinterpret_cast<const uint4*>(p.qkv + (int64_t)c.b * p.ld_qkv + (s.H + c.h + (is_v ? s.Hkv : 0)) * D + ch * 8);
-      if (!warp_wait(&bars->k_full[ks], (ts / kKSlots) & 1, abort_flag, status, kMma)) return false;
+      if (!warp_wait(&bars->k_full[ks], (ts / kKSlots) & 1, abort_flag, status, kMma)) break;
       if (ends) {
         // The sequence ends in this tile: row `last` is the new token's.
-        if (!warp_wait(&bars->v_full[vs], (ts / kVSlots) & 1, abort_flag, status, kMma)) return false;
+        if (!warp_wait(&bars->v_full[vs], (ts / kVSlots) & 1, abort_flag, status, kMma)) break;
         const int last = c.limit - 1 - c.key();
         if (lane < 16) {
           uint8_t* tile = is_v ? sV + vs * kTile : sK + ks * kTile;
@@ -517,12 +530,12 @@ __global__ void __launch_bounds__(kThreads, 2)
         fence_proxy_async_smem();
         __syncwarp();
       }
-      if (!warp_wait(&bars->s_free[x], ((ts >> 1) & 1) ^ 1, abort_flag, status, kMma)) return false;
+      if (!warp_wait(&bars->s_free[x], ((ts >> 1) & 1) ^ 1, abort_flag, status, kMma)) break;
       tc_fence_after();
       if (lane == 0) {
-        const uint32_t idesc = idesc_f16_f32(BKV, 0, false, false) | (width >> 3) << 17;
+        const uint32_t idesc = idesc_f16_f32(BKV, 0, false, false) | ((uint32_t)(c.rows(s) + 15) >> 4) << 18;
         const uint64_t a = desc_adv(dK0, ks * kTile);
-        const uint64_t b = smem_desc_sw128(smem_u32(q == 2 ? sQp : sQ + q * p.q_own_stride), 16, 1024);
+        const uint64_t b = q == 2 ? dQp : desc_adv(dQ0, q * p.q_own_stride);
 #pragma unroll
         for (int kk = 0; kk < D / 16; ++kk)
           umma_f16(tmem + x * 64, desc_adv(a, kk * 32), desc_adv(b, kk * 32), idesc, kk > 0 ? 1u : 0u);
@@ -531,33 +544,30 @@ __global__ void __launch_bounds__(kThreads, 2)
         if (c.j == c.n - 1) umma_commit(&bars->q_empty[q]);
       }
       __syncwarp();
-      return true;
-    };
-    bool more = c.advance(s, lens);
-    bool ok = !more || issue_s(0, 0);
-    for (uint32_t tp = 0; ok && more; ++tp) {
-      const uint32_t pv_width = width;
-      const bool pv_first = first;
-      // S^T of the next tile goes ahead of this tile's product with V.
-      more = c.advance(s, lens);
-      if (more && !(ok = issue_s(tp + 1, (tp + 1) & 1))) break;
-      const uint32_t vs = tp % kVSlots;
-      if (!(ok = warp_wait(&bars->v_full[vs], (tp / kVSlots) & 1, abort_flag, status, kMma))) break;
-      if (!(ok = warp_wait(&bars->p_full, tp & 1, abort_flag, status, kMma))) break;
-      tc_fence_after();
-      if (lane == 0) {
-        const uint32_t idesc = idesc_f16_f32(128, 0, true, true) | (pv_width >> 3) << 17;
-        const uint32_t v = smem_u32(sV + vs * kTile), ones = smem_u32(s1);
+    }
+  } else if (warp == 6) {
+    if (lane == 0) {
+      const uint64_t dP0 = smem_desc_sw128(smem_u32(sP), 8192, 1024);
+      // A of the second product for slot 0 and keys 0-15: rows 0-63 are V^T, rows 64-127, one leading offset on, ones.
+      // 16 keys (2 KB) or a slot further, the start moves up and the leading offset down by as much, both in units of 16.
+      const uint64_t dV0 = smem_desc_sw128(smem_u32(sV), smem_u32(s1) - smem_u32(sV), 1024);
+      constexpr uint64_t kStep = 2048 / 16, kSlot = kTile / 16;
+      for (uint32_t tp = 0; c.advance(s, lens); ++tp) {
+        const uint32_t vs = tp % kVSlots;
+        const uint32_t idesc = idesc_f16_f32(128, 0, true, true) | ((uint32_t)(c.rows(s) + 15) >> 4) << 18;
+        const uint64_t dv = dV0 + vs * (kSlot - (kSlot << 16));
+        if (!wait(&bars->v_full[vs], (tp / kVSlots) & 1, abort_flag, status, kMma)) break;
+        if (!wait(&bars->p_full, tp & 1, abort_flag, status, kMma)) break;
+        tc_fence_after();
 #pragma unroll
         for (int kk = 0; kk < BKV / 16; ++kk)
-          // Rows 0-63 of A are V^T of 16 keys, rows 64-127, one leading offset on, ones.
-          umma_f16(tmem + 128, smem_desc_sw128(v + kk * 2048, ones - (v + kk * 2048), 1024), desc_adv(dP0, kk * 2048), idesc,
-                   (!pv_first || kk > 0) ? 1u : 0u);
+          umma_f16(tmem + 128, dv + kk * (kStep - (kStep << 16)), desc_adv(dP0, kk * 2048), idesc,
+                   (c.j > 0 || kk > 0) ? 1u : 0u);
         umma_commit(&bars->v_empty[vs]);
         umma_commit(&bars->p_empty);
       }
-      __syncwarp();
     }
+    __syncwarp();
   } else {
     bool ok = true;
     for (uint32_t g = 0; ok && c.advance(s, lens);) {
