@@ -15,11 +15,29 @@ namespace kd {
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kMaxSlots = 1024;
+constexpr int kSeen = 1024;
 
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+
+// What a row's softmax at temperature 1 costs next to the one at tau: nothing (kOne: tau = 1, alpha = 1 or given block
+// statistics), multiplications (tau = 2, 3, 4: exp(z) is a power of exp(z / tau)) or a second exponential (kBoth). The
+// exponential unit takes 2000 cycles of an SM for 32000 logits where memory takes 2700, so a second one would set the
+// time (16384 x 32000: kBoth BOTHUS us, kPow2 POWUS us).
+enum Mode : int { kOne = 0, kBoth = 1, kPow2 = 2, kPow3 = 3, kPow4 = 4 };
+
+inline Mode mode_of(float tau, bool two) {
+  if (!two) return kOne;
+  return tau == 2.f ? kPow2 : tau == 3.f ? kPow3 : tau == 4.f ? kPow4 : kBoth;
+}
+
+template <int MODE>
+__device__ __forceinline__ float power(float w) {
+  const float w2 = w * w;
+  return MODE == kPow2 ? w2 : MODE == kPow3 ? w2 * w : w2 * w2;
 }
 
 struct Params {
@@ -57,6 +75,15 @@ __device__ __forceinline__ uint4 load8(const __half* row, int64_t first, int voc
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
+// ln(s) with the exponent split off, so that the fp32 logarithm's error is that of a number below 0.35.
+__device__ __forceinline__ double log_wide(float s) {
+  if (!(s > 1e-30f && s < 1e30f)) return (double)logf(s);
+  int e = (__float_as_int(s) >> 23) - 127;
+  float m = __int_as_float((__float_as_int(s) & 0x7fffff) | 0x3f800000);
+  if (m > 1.41421356f) m *= 0.5f, ++e;
+  return e * 0.69314718055994530942 + (double)logf(m);
+}
+
 __device__ __forceinline__ double warp_sum_d(double v) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
@@ -92,7 +119,7 @@ __device__ __forceinline__ void finish_row(const Params& p, int64_t row, double 
   nan = __any_sync(0xffffffffu, nan || bad_id);
   if (lane != 0) return;
   const bool used = tm != -INFINITY || nan;
-  const double lse_t = used ? (double)tm / p.tau + log((double)s) : -INFINITY;
+  const double lse_t = used ? (double)tm / p.tau + log_wide(s) : -INFINITY;
   double kl = 0.0;
   if (used) kl = d / s / p.tau + lse - lse_t;
   const int64_t y = p.targets[row];
@@ -146,7 +173,7 @@ __device__ __forceinline__ double parts_lse(const float2* parts, int nblk, float
   const float gm = warp_max(m);
   if (m != -INFINITY) s *= ex2((m - gm) * kLog2e);
   *gmax = gm;
-  return (double)gm + log((double)warp_sum(s));
+  return (double)gm + log_wide(warp_sum(s));
 }
 
 // Temperature 1 with the head's block statistics: the logits are read at the slots and the target only. One
@@ -171,10 +198,12 @@ __global__ void __launch_bounds__(kPartWarps * 32) distill_parts_kernel(const Pa
 }
 
 // One block per row, one pass over the logits: each thread keeps a running maximum of what it has read and the
-// sums against it. kTwo: the sum at temperature 1 as well.
-template <int NT, int VPT, bool kTwo>
+// sums against it. Small blocks, so that the few warps of a row's end (a chain of about a thousand cycles over the
+// slots) are covered by the other rows on the SM; rows of few-row calls are spread over more threads.
+template <int NT, int VPT, int MODE>
 __global__ void __launch_bounds__(NT, 1024 / NT) distill_fwd_kernel(const Params p, float* __restrict__ row_loss,
                                                                     int* status) {
+  constexpr bool kTwo = MODE != kOne;
   extern __shared__ float slots[];  // [2][K]
   __shared__ float rm[NT / 32], rs[NT / 32], rs1[NT / 32];
   __shared__ double rlse1;
@@ -224,8 +253,12 @@ __global__ void __launch_bounds__(NT, 1024 / NT) distill_fwd_kernel(const Params
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const float2 f = __half22float2(h[j]);
-        a[j] += ex2(fmaf(f.x, c, mc)) + ex2(fmaf(f.y, c, mc));
-        if constexpr (kTwo) b[j] += ex2(fmaf(f.x, kLog2e, mc1)) + ex2(fmaf(f.y, kLog2e, mc1));
+        const float w0 = ex2(fmaf(f.x, c, mc)), w1 = ex2(fmaf(f.y, c, mc));
+        a[j] += w0 + w1;
+        if constexpr (MODE == kBoth)
+          b[j] += ex2(fmaf(f.x, kLog2e, mc1)) + ex2(fmaf(f.y, kLog2e, mc1));
+        else if constexpr (kTwo)
+          b[j] += power<MODE>(w0) + power<MODE>(w1);
       }
     }
     s += (a[0] + a[1]) + (a[2] + a[3]);
@@ -263,8 +296,8 @@ __global__ void __launch_bounds__(NT, 1024 / NT) distill_fwd_kernel(const Params
   }
   s = warp_sum(s);
   s1 = warp_sum(s1);
-  const double lse = (double)gm / p.tau + log((double)s);
-  const double lse1 = kTwo ? (double)gm + log((double)s1) : p.parts ? rlse1 : lse;
+  const double lse = (double)gm / p.tau + log_wide(s);
+  const double lse1 = kTwo ? (double)gm + log_wide(s1) : p.parts ? rlse1 : lse;
   const int64_t y = p.targets[row];
   const float zy = y >= 0 && y < p.vocab ? __half2float(z[y]) : 0.f;
   finish_row(p, row, lse, lse1, slots, slots + p.K, rbad != 0, zy, row_loss, status);
@@ -273,11 +306,13 @@ __global__ void __launch_bounds__(NT, 1024 / NT) distill_fwd_kernel(const Params
 // The gradient. One block per row; the slots' logits are read before anything is stored (out may be the logits).
 // Every element gets the dense part, then the slots' elements and the target's are stored once more with
 // their own terms, each by the first slot that names it, so that each is rounded once.
-template <int NT, int VPT, bool kTwo>
+template <int NT, int VPT, int MODE>
 __global__ void __launch_bounds__(NT, 1024 / NT) distill_bwd_kernel(const Params p, const float* __restrict__ grad_loss,
                                                                     const float* __restrict__ count, __half* out,
                                                                     int64_t ld_out) {
   extern __shared__ float slots[];  // t, z, then ids: [3][K + 1]
+  __shared__ uint32_t seen[kSeen];  // a bit per id (modulo 32 kSeen): tells whether two slots may name the same
+  __shared__ int repeated;
   const int tid = threadIdx.x;
   const int64_t row = blockIdx.x;
   const __half* z = p.logits + row * p.ld;
@@ -302,17 +337,23 @@ __global__ void __launch_bounds__(NT, 1024 / NT) distill_bwd_kernel(const Params
   float* delta = slots;            // what a slot adds to its element's gradient
   float* slot_z = slots + K + 1;
   int* slot_id = reinterpret_cast<int*>(slots + 2 * (K + 1));
+  for (int i = tid; i < kSeen; i += NT) seen[i] = 0;
   load_slots<NT>(p, row, z, delta, slot_z, slot_id, tid, nullptr);
   // Slot K: the target.
   if (tid == 0) {
+    repeated = 0;
     slot_id[K] = (int)y;
     slot_z[K] = __half2float(z[y]);
     delta[K] = -gb;
   }
   const float c = kLog2e / p.tau, b = -lse * kLog2e, b1 = -lse1 * kLog2e;
+  // q1 = exp(z - lse1) = q^tau exp(tau lse - lse1); the last factor is at most vocab^(tau - 1).
+  const float gpow = MODE == kOne || MODE == kBoth ? 0.f : gb * expf(fmaf(p.tau, lse, -lse1));
   auto dense = [&](float x) {
-    if constexpr (kTwo) return fmaf(gb, ex2(fmaf(x, kLog2e, b1)), ga * ex2(fmaf(x, c, b)));
-    return (ga + gb) * ex2(fmaf(x, c, b));  // tau = 1, or gb = 0
+    const float w = ex2(fmaf(x, c, b));
+    if constexpr (MODE == kOne) return (ga + gb) * w;  // tau = 1, or gb = 0
+    if constexpr (MODE == kBoth) return fmaf(gb, ex2(fmaf(x, kLog2e, b1)), ga * w);
+    return fmaf(gpow, power<MODE>(w), ga * w);
   };
   for (int base = 0; base < nvec; base += NT * VPT) {
     uint4 v[VPT];
@@ -323,6 +364,10 @@ __global__ void __launch_bounds__(NT, 1024 / NT) distill_bwd_kernel(const Params
       for (int k = tid; k < K; k += NT) {
         const float t = delta[k];
         delta[k] = t == -INFINITY ? 0.f : -ga * exp2f((t / p.tau - lse_t) * kLog2e);
+      }
+      for (int k = tid; k <= K; k += NT) {
+        const int id = slot_id[k];
+        if (id >= 0 && (atomicOr(&seen[(id >> 5) % kSeen], 1u << (id & 31)) >> (id & 31) & 1u)) repeated = 1;
       }
     }
 #pragma unroll
@@ -349,15 +394,18 @@ __global__ void __launch_bounds__(NT, 1024 / NT) distill_bwd_kernel(const Params
   for (int k = tid; k <= K; k += NT) {
     const int id = slot_id[k];
     if (id < 0) continue;
-    float d = 0.f;
+    float d = delta[k];
     bool mine = true;
-    for (int j = 0; j <= K; ++j) {
-      if (slot_id[j] != id) continue;
-      if (j < k) {
-        mine = false;
-        break;
+    if (repeated) {
+      d = 0.f;
+      for (int j = 0; j <= K; ++j) {
+        if (slot_id[j] != id) continue;
+        if (j < k) {
+          mine = false;
+          break;
+        }
+        d += delta[j];
       }
-      d += delta[j];
     }
     if (mine) o[id] = __float2half_rn(dense(slot_z[k]) + d);
   }
@@ -380,8 +428,37 @@ int check(const kd::Params& p, const char* name) {
   return JX_OK;
 }
 
-// A block of 512 threads holds rows of up to 32768 logits in registers; for short rows one of 128.
-constexpr int kShortRow = 8192;
+// Threads of a row's block: 128, or 512 where fewer rows than that fill the SMs (1000 x 24000, loss and gradient: SMALLUS
+// against WIDEUS us; 16384 x 32000: see above) and the row is long enough for them.
+bool wide_block(int64_t rows, int vocab) { return rows < 4 * num_sms() && vocab > 8192; }
+
+template <int NT>
+void launch_fwd(const kd::Params& p, kd::Mode mode, float* row_loss, cudaStream_t s) {
+  const unsigned grid = (unsigned)p.rows;
+  const size_t smem = 2 * p.K * sizeof(float);
+  int* status = status_ptr();
+  switch (mode) {
+    case kd::kOne: kd::distill_fwd_kernel<NT, 8, kd::kOne><<<grid, NT, smem, s>>>(p, row_loss, status); break;
+    case kd::kBoth: kd::distill_fwd_kernel<NT, 8, kd::kBoth><<<grid, NT, smem, s>>>(p, row_loss, status); break;
+    case kd::kPow2: kd::distill_fwd_kernel<NT, 8, kd::kPow2><<<grid, NT, smem, s>>>(p, row_loss, status); break;
+    case kd::kPow3: kd::distill_fwd_kernel<NT, 8, kd::kPow3><<<grid, NT, smem, s>>>(p, row_loss, status); break;
+    case kd::kPow4: kd::distill_fwd_kernel<NT, 8, kd::kPow4><<<grid, NT, smem, s>>>(p, row_loss, status); break;
+  }
+}
+
+template <int NT>
+void launch_bwd(const kd::Params& p, kd::Mode mode, const float* grad_loss, const float* count, __half* out, int64_t ld_out,
+                cudaStream_t s) {
+  const unsigned grid = (unsigned)p.rows;
+  const size_t smem = 3 * (p.K + 1) * sizeof(float);
+  switch (mode) {
+    case kd::kOne: kd::distill_bwd_kernel<NT, 8, kd::kOne><<<grid, NT, smem, s>>>(p, grad_loss, count, out, ld_out); break;
+    case kd::kBoth: kd::distill_bwd_kernel<NT, 8, kd::kBoth><<<grid, NT, smem, s>>>(p, grad_loss, count, out, ld_out); break;
+    case kd::kPow2: kd::distill_bwd_kernel<NT, 8, kd::kPow2><<<grid, NT, smem, s>>>(p, grad_loss, count, out, ld_out); break;
+    case kd::kPow3: kd::distill_bwd_kernel<NT, 8, kd::kPow3><<<grid, NT, smem, s>>>(p, grad_loss, count, out, ld_out); break;
+    case kd::kPow4: kd::distill_bwd_kernel<NT, 8, kd::kPow4><<<grid, NT, smem, s>>>(p, grad_loss, count, out, ld_out); break;
+  }
+}
 
 }  // namespace
 
@@ -402,15 +479,10 @@ extern "C" int jx_distill_fwd(const void* logits16, int64_t rows, int vocab, int
     return JX_OK;
   }
   const bool two = alpha < 1.f && temperature != 1.f && !parts;
-  const size_t smem = 2 * K * sizeof(float);
-  const unsigned grid = (unsigned)rows;
-  if (vocab <= kShortRow) {
-    if (two) kd::distill_fwd_kernel<128, 8, true><<<grid, 128, smem, s>>>(p, row_loss, status_ptr());
-    else kd::distill_fwd_kernel<128, 8, false><<<grid, 128, smem, s>>>(p, row_loss, status_ptr());
-  } else {
-    if (two) kd::distill_fwd_kernel<512, 8, true><<<grid, 512, smem, s>>>(p, row_loss, status_ptr());
-    else kd::distill_fwd_kernel<512, 8, false><<<grid, 512, smem, s>>>(p, row_loss, status_ptr());
-  }
+  if (wide_block(rows, vocab))
+    launch_fwd<512>(p, kd::mode_of(temperature, two), row_loss, s);
+  else
+    launch_fwd<128>(p, kd::mode_of(temperature, two), row_loss, s);
   JX_CHECK_LAUNCH("jx_distill_fwd");
   return JX_OK;
 }
@@ -428,17 +500,12 @@ extern "C" int jx_distill_bwd(const void* logits16, int64_t rows, int vocab, int
   JX_CHECK_ARG(ld_out % 8 == 0 && ld_out >= vocab && aligned16(out16), "jx_distill_bwd: ld_out%%8 and 16B alignment required");
   JX_CHECK_ARG(out16 != logits16 || ld_out == ld, "jx_distill_bwd: in place, the row strides must be the same");
   const bool two = alpha < 1.f && temperature != 1.f;
-  const size_t smem = 3 * (K + 1) * sizeof(float);
-  const unsigned grid = (unsigned)rows;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   __half* out = static_cast<__half*>(out16);
-  if (vocab <= kShortRow) {
-    if (two) kd::distill_bwd_kernel<128, 8, true><<<grid, 128, smem, s>>>(p, grad_loss, count, out, ld_out);
-    else kd::distill_bwd_kernel<128, 8, false><<<grid, 128, smem, s>>>(p, grad_loss, count, out, ld_out);
-  } else {
-    if (two) kd::distill_bwd_kernel<512, 8, true><<<grid, 512, smem, s>>>(p, grad_loss, count, out, ld_out);
-    else kd::distill_bwd_kernel<512, 8, false><<<grid, 512, smem, s>>>(p, grad_loss, count, out, ld_out);
-  }
+  if (wide_block(rows, vocab))
+    launch_bwd<512>(p, kd::mode_of(temperature, two), grad_loss, count, out, ld_out, s);
+  else
+    launch_bwd<128>(p, kd::mode_of(temperature, two), grad_loss, count, out, ld_out, s);
   JX_CHECK_LAUNCH("jx_distill_bwd");
   return JX_OK;
 }
