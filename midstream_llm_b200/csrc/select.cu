@@ -32,26 +32,37 @@ __device__ __forceinline__ uint32_t key_bits(uint32_t key) { return (key & 0x800
 
 __device__ __forceinline__ __half key_half(uint32_t key) { return __ushort_as_half((unsigned short)key_bits(key)); }
 
-// Eight consecutive logits; elements at and past `vocab` read as NaN, which no comparison selects. A row
-// starts on a 16-byte boundary; only whole vectors are read as one.
+// Eight consecutive logits; elements at and past `vocab` read as `fill` (twice the same half: a NaN, which no
+// comparison selects, or -inf). A row starts on a 16-byte boundary; only whole vectors are read as one.
+constexpr uint32_t kFillNan = 0xffffu, kFillNegInf = 0xfc00u;
+
 struct Vec {
   uint32_t w[4];
   __device__ __forceinline__ uint32_t bits(int j) const { return (w[j >> 1] >> ((j & 1) * 16)) & 0xffffu; }
 };
 
-__device__ __forceinline__ Vec load_vec(const __half* row, int64_t first, int vocab) {
+template <uint32_t kFill>
+__device__ __noinline__ Vec load_part(const __half* row, int64_t first, int vocab) {
+  const unsigned short* p = reinterpret_cast<const unsigned short*>(row);
   Vec v;
-  if (first + 8 <= vocab) {
-    const uint4 u = __ldg(reinterpret_cast<const uint4*>(row + first));
-    v.w[0] = u.x, v.w[1] = u.y, v.w[2] = u.z, v.w[3] = u.w;
-  } else {
-    const unsigned short* p = reinterpret_cast<const unsigned short*>(row);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const uint32_t lo = first + 2 * j < vocab ? p[first + 2 * j] : 0xffffu;
-      const uint32_t hi = first + 2 * j + 1 < vocab ? p[first + 2 * j + 1] : 0xffffu;
-      v.w[j] = lo | (hi << 16);
-    }
+  for (int j = 0; j < 4; ++j) {
+    const uint32_t lo = first + 2 * j < vocab ? p[first + 2 * j] : kFill;
+    const uint32_t hi = first + 2 * j + 1 < vocab ? p[first + 2 * j + 1] : kFill;
+    v.w[j] = lo | (hi << 16);
+  }
+  return v;
+}
+
+template <uint32_t kFill>
+__device__ __forceinline__ Vec load_vec(const __half* row, int i, int vocab) {  // vector i
+  Vec v;
+  v.w[0] = v.w[1] = v.w[2] = v.w[3] = kFill * 0x10001u;
+  if (i < vocab >> 3) {
+    const uint4 u = __ldg(reinterpret_cast<const uint4*>(row) + i);
+    v.w[0] = u.x, v.w[1] = u.y, v.w[2] = u.z, v.w[3] = u.w;
+  } else if (i * 8 < vocab) {
+    v = load_part<kFill>(row, 8 * i, vocab);
   }
   return v;
 }
@@ -69,13 +80,19 @@ __device__ __forceinline__ __half max_of(__half2 m) { return __hmax(__low2half(m
 __device__ __forceinline__ uint32_t vec_ge(const Vec& v, __half2 limit) {
   uint32_t m = 0;
 #pragma unroll
-  for (int j = 0; j < 4; ++j) m |= (__hge2_mask(as_half2(v.w[j]), limit) & 0x10001u) << j;
+  for (int j = 0; j < 4; ++j) m |= __hge2_mask(as_half2(v.w[j]), limit) & (0x10001u << j);
   // bits 0..3: elements 0, 2, 4, 6; bits 16..19: elements 1, 3, 5, 7
   return m;
 }
 __device__ __forceinline__ uint32_t ge_bit(int j) { return (j & 1) ? 0x10000u << (j >> 1) : 1u << (j >> 1); }
 
 // ---------------------------------------------------------------------------------------------------------
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
 // Block helpers. Every thread of the block calls them.
 // ---------------------------------------------------------------------------------------------------------
 template <int NT>
@@ -125,20 +142,20 @@ __device__ __forceinline__ T block_scan(T v, T* red, T* total) {
 // Top logits: the k largest of a row in rank order.
 //
 // One block per row with the row in registers (rows longer than NT * 8 * VPT elements are read again for the
-// second pass). The k-th largest of any part of the row is a lower bound of the k-th largest of all of it, so
-// the maxima of the threads (or of the 8-element vectors where k is large) go into a histogram of their
-// keys' upper 11 bits and the bin that holds the k-th of them gives a limit that little more than k elements
-// pass. Those are collected, ranked among themselves and written. A row where more than kCand elements pass
-// (many equal values) takes the exact way: two histograms find the threshold key, values at it are taken
-// in index order.
+// second pass). The k-th largest of the threads' maxima is a limit that at least k elements pass, and in general few
+// more: a histogram of the maxima, in bins of 16 keys down from the largest, gives it to within a bin. The few vectors that
+// hold such elements go to shared memory, their elements above the limit are collected, ranked among themselves by
+// counting and written. A row where too many pass (many equal values) or k is large against the threads takes
+// the exact way: two histograms of all keys find the threshold, values at it are taken in index order.
 // ---------------------------------------------------------------------------------------------------------
 constexpr int kBins = 2048;     // upper 11 bits of a key
 constexpr int kCand = 2048;     // candidates a block can hold
+constexpr int kVecs = 512;      // vectors with candidates
 constexpr int kMaxTop = 1024;
 
 // With hist[bin] counting keys, finds the bin (from the top) in which the k-th key falls and how many keys lie
 // in higher bins; found[0] = -1 if there are fewer than k keys in all.
-template <int NT>
+template <int NT, int kBins = sel::kBins>
 __device__ __forceinline__ void find_bin(const uint32_t* hist, uint32_t k, uint32_t* red, int* found) {
   constexpr int PER = kBins / NT;
   uint32_t c[PER], sum = 0;
@@ -163,138 +180,193 @@ __device__ __forceinline__ void find_bin(const uint32_t* hist, uint32_t k, uint3
   __syncthreads();
 }
 
-template <int NT, int VPT>
+// A candidate: key and complemented index, so that larger means earlier in rank. 32 bits where the index fits 16.
+template <typename C>
+struct CandidateOf {
+  static constexpr int kShift = sizeof(C) * 4;
+  static constexpr C kMask = (C(1) << kShift) - 1;
+  static __device__ __forceinline__ C make(uint32_t key, uint32_t index) { return (C)key << kShift | (kMask - (C)index); }
+  static __device__ __forceinline__ uint32_t key(C c) { return (uint32_t)(c >> kShift); }
+  static __device__ __forceinline__ uint32_t index(C c) { return (uint32_t)(kMask - (c & kMask)); }
+};
+
+// The exact way: k candidates in any order. Rare, so plain.
+template <int NT, typename C>
+__device__ __noinline__ void exact_candidates(const unsigned short* row, int vocab, uint32_t k, uint32_t* hist, uint32_t* red,
+                                              int* found, C* cand, uint32_t* ncand) {
+  const int tid = threadIdx.x;
+  __syncthreads();
+  for (int i = tid; i < kBins; i += NT) hist[i] = 0;
+  if (tid == 0) *ncand = 0;
+  __syncthreads();
+  for (int i = tid; i < vocab; i += NT) atomicAdd(&hist[order_key(row[i]) >> 5], 1u);
+  __syncthreads();
+  find_bin<NT>(hist, k, red, found);
+  const uint32_t bin = (uint32_t)found[0];
+  uint32_t left = k - (uint32_t)found[1];
+  __syncthreads();
+  for (int i = tid; i < kBins; i += NT) hist[i] = 0;
+  __syncthreads();
+  for (int i = tid; i < vocab; i += NT) {
+    const uint32_t key = order_key(row[i]);
+    if (key >> 5 == bin) atomicAdd(&hist[key & 31u], 1u);
+  }
+  __syncthreads();
+  uint32_t sub = 31;
+  while (hist[sub] < left) left -= hist[sub--];
+  const uint32_t tau = (bin << 5) | sub;
+  uint32_t taken = 0;
+  for (int base = 0; base < vocab; base += NT) {
+    const int i = base + tid;
+    const uint32_t key = i < vocab ? order_key(row[i]) : 0u;
+    const uint32_t tie = i < vocab && key == tau ? 1u : 0u;
+    uint32_t total = 0, before = 0;
+    if (taken < left) before = taken + block_scan<NT>(tie, red, &total);
+    if (i < vocab && (key > tau || (tie && taken < left && before < left)))
+      cand[atomicAdd(ncand, 1u)] = CandidateOf<C>::make(key, (uint32_t)i);
+    taken += total;
+  }
+  __syncthreads();
+}
+
+template <int NT, int VPT, typename C>
 __global__ void __launch_bounds__(NT, 1024 / NT)
     top_logits_kernel(const __half* __restrict__ logits, int64_t ld, int vocab, int k, __half* __restrict__ values,
                       int64_t* __restrict__ ids) {
-  __shared__ uint32_t hist[kBins];
-  __shared__ u64 cand[kCand];
+  constexpr int NW = NT / 32;
+  typedef CandidateOf<C> Cand;
+  constexpr int kOwn = kVecs / NW;  // vectors a warp can hold
+  __shared__ union {
+    struct {
+      uint4 v[kVecs];
+      int index[kVecs];
+    } vec;
+    uint32_t hist[kBins];
+  } s;
+  __shared__ __align__(16) C cand[kCand];
   __shared__ uint32_t red[32];
   __shared__ int found[2];
   __shared__ uint32_t ncand;
-  const int tid = threadIdx.x;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const __half* row = logits + (int64_t)blockIdx.x * ld;
   const int nvec = (vocab + 7) / 8;
   const int nchunk = (nvec + NT * VPT - 1) / (NT * VPT);
 
-  for (int i = tid; i < kBins; i += NT) hist[i] = 0;
-  if (tid == 0) ncand = 0;
-  __syncthreads();
-
-  // Maxima into the histogram: one a thread, or one a vector where k is large against their number.
-  const bool fine = (int64_t)k * 4 > min(nvec, NT);
   Vec v[VPT];
   __half2 tmax = __half2half2(__ushort_as_half(0xffffu));
   for (int c = 0; c < nchunk; ++c) {
 #pragma unroll
-    for (int i = 0; i < VPT; ++i) v[i] = load_vec(row, 8 * (int64_t)((c * VPT + i) * NT + tid), vocab);
+    for (int i = 0; i < VPT; ++i) v[i] = load_vec<kFillNan>(row, (c * VPT + i) * NT + tid, vocab);
 #pragma unroll
-    for (int i = 0; i < VPT; ++i) {
-      const __half2 m = vec_max2(v[i]);
-      if (fine) {
-        const uint32_t key = order_key(__half_as_ushort(max_of(m)));
-        if (key) atomicAdd(&hist[key >> 5], 1u);
-      }
-      tmax = __hmax2(tmax, m);
+    for (int i = 0; i < VPT; ++i) tmax = __hmax2(tmax, vec_max2(v[i]));
+  }
+  // The limit.
+  constexpr int kTopBins = 1024;
+  const uint32_t tkey = order_key(__half_as_ushort(max_of(tmax)));
+  for (int i = tid; i < kTopBins; i += NT) s.hist[i] = 0;
+  if (tid == 0) ncand = 0;
+  const uint32_t mkey = block_max<NT>(tkey, red);
+  uint32_t lkey = 0;
+  if (k <= min(nvec, NT)) {
+    const uint32_t d = (mkey - tkey) >> 4;
+    if (tkey && d < kTopBins) atomicAdd(&s.hist[kTopBins - 1 - d], 1u);
+    __syncthreads();
+    find_bin<NT, kTopBins>(s.hist, (uint32_t)k, red, found);
+    if (found[0] >= 0) {
+      const uint32_t down = (uint32_t)(kTopBins - found[0]) * 16 - 1;  // to the bin's lowest key
+      lkey = mkey > down ? mkey - down : 0u;
     }
   }
-  if (!fine) {
-    const uint32_t key = order_key(__half_as_ushort(max_of(tmax)));
-    if (key) atomicAdd(&hist[key >> 5], 1u);
-  }
-  __syncthreads();
-  find_bin<NT>(hist, (uint32_t)k, red, found);
-  // Fewer maxima than k: every element is a candidate (NaN too), if they fit.
-  const bool all = found[0] < 0;
-  const __half2 limit = __half2half2(key_half(all ? kKeyNegInf : max((uint32_t)found[0] << 5, kKeyNegInf)));
+  // Without a limit every element of a short row is a candidate (NaN too).
+  const bool all = lkey <= kKeyNegInf;
+  const __half limit = key_half(max(lkey, kKeyNegInf));
   uint32_t n = kCand + 1;
-  if (!all || vocab <= kCand) {
+  if (!all || nvec * 8 <= kCand) {
+    // Each warp gathers its vectors and looks through them by itself.
+    const uint32_t below = (1u << lane) - 1u;
+    uint32_t nv = 0;
     for (int c = 0; c < nchunk; ++c) {
       if (nchunk > 1) {
 #pragma unroll
-        for (int i = 0; i < VPT; ++i) v[i] = load_vec(row, 8 * (int64_t)((c * VPT + i) * NT + tid), vocab);
+        for (int i = 0; i < VPT; ++i) v[i] = load_vec<kFillNan>(row, (c * VPT + i) * NT + tid, vocab);
       }
 #pragma unroll
       for (int i = 0; i < VPT; ++i) {
-        const int64_t first = 8 * (int64_t)((c * VPT + i) * NT + tid);
-        const uint32_t m = all ? 0xf000fu : vec_ge(v[i], limit);
-        if (m) {
-#pragma unroll
-          for (int j = 0; j < 8; ++j)
-            if ((m & ge_bit(j)) && first + j < vocab) {
-              const uint32_t p = atomicAdd(&ncand, 1u);
-              if (p < kCand) cand[p] = ((u64)order_key(v[i].bits(j)) << 32) | (0xffffffffu - (uint32_t)(first + j));
-            }
+        const int at = (c * VPT + i) * NT + tid;
+        const bool hit = all ? at < nvec : __hge(max_of(vec_max2(v[i])), limit);
+        const uint32_t hits = __ballot_sync(0xffffffffu, hit);
+        if (hits) {
+          const uint32_t p = nv + __popc(hits & below);
+          if (hit && p < kOwn) {
+            s.vec.v[warp * kOwn + p] = make_uint4(v[i].w[0], v[i].w[1], v[i].w[2], v[i].w[3]);
+            s.vec.index[warp * kOwn + p] = at;
+          }
+          nv += __popc(hits);
         }
+      }
+    }
+    __syncwarp();
+    if (nv > kOwn) {
+      if (lane == 0) atomicAdd(&ncand, kCand + 1u);  // too many: the exact way
+    } else {
+      const unsigned short* h = reinterpret_cast<const unsigned short*>(&s.vec.v[warp * kOwn]);
+#pragma unroll 1
+      for (uint32_t e = lane; e < (nv * 8 + 31 & ~31u); e += 32) {
+        uint32_t key = 0, index = 0xffffffffu;
+        if (e < nv * 8) {
+          key = order_key(h[e]);
+          index = (uint32_t)s.vec.index[warp * kOwn + (e >> 3)] * 8 + (e & 7);
+        }
+        const bool in = (all || key >= lkey) && index < (uint32_t)vocab;
+        const uint32_t ins = __ballot_sync(0xffffffffu, in);
+        uint32_t p = 0;
+        if (lane == 0 && ins) p = atomicAdd(&ncand, (uint32_t)__popc(ins));
+        p = __shfl_sync(0xffffffffu, p, 0) + __popc(ins & below);
+        if (in && p < kCand) cand[p] = Cand::make(key, index);
       }
     }
     __syncthreads();
     n = ncand;
   }
   if (n > kCand) {
-    // The exact way: threshold key from histograms over the whole row, then the keys above it and, in index
-    // order, as many at it as are left to take.
-    __syncthreads();
-    for (int i = tid; i < kBins; i += NT) hist[i] = 0;
-    if (tid == 0) ncand = 0;
-    __syncthreads();
-    const unsigned short* p = reinterpret_cast<const unsigned short*>(row);
-    for (int i = tid; i < vocab; i += NT) atomicAdd(&hist[order_key(p[i]) >> 5], 1u);
-    __syncthreads();
-    find_bin<NT>(hist, (uint32_t)k, red, found);
-    const uint32_t bin = (uint32_t)found[0];
-    uint32_t left = (uint32_t)k - (uint32_t)found[1];
-    __syncthreads();
-    for (int i = tid; i < kBins; i += NT) hist[i] = 0;
-    __syncthreads();
-    for (int i = tid; i < vocab; i += NT) {
-      const uint32_t key = order_key(p[i]);
-      if (key >> 5 == bin) atomicAdd(&hist[key & 31u], 1u);
-    }
-    __syncthreads();
-    uint32_t sub = 31;
-    while (hist[sub] < left) left -= hist[sub--];
-    const uint32_t tau = (bin << 5) | sub;
-    uint32_t taken = 0;
-    for (int base = 0; base < vocab; base += NT) {
-      const int i = base + tid;
-      const uint32_t key = i < vocab ? order_key(p[i]) : 0u;
-      const uint32_t tie = i < vocab && key == tau ? 1u : 0u;
-      uint32_t total = 0, before = 0;
-      if (taken < left) before = taken + block_scan<NT>(tie, red, &total);
-      if (i < vocab && (key > tau || (tie && taken < left && before < left)))
-        cand[atomicAdd(&ncand, 1u)] = ((u64)key << 32) | (0xffffffffu - (uint32_t)i);
-      taken += total;
-    }
-    __syncthreads();
-    n = ncand;  // k
+    exact_candidates<NT, C>(reinterpret_cast<const unsigned short*>(row), vocab, (uint32_t)k, s.hist, red, found, cand, &ncand);
+    n = (uint32_t)k;
   }
   __half* vout = values + (int64_t)blockIdx.x * k;
   int64_t* iout = ids + (int64_t)blockIdx.x * k;
-  auto write = [&](uint32_t rank, u64 c) {
-    vout[rank] = key_half((uint32_t)(c >> 32));
-    iout[rank] = (int64_t)(0xffffffffu - (uint32_t)c);
+  auto write = [&](uint32_t rank, C c) {
+    vout[rank] = key_half(Cand::key(c));
+    iout[rank] = (int64_t)Cand::index(c);
   };
+  // Padded with zeros (which no candidate is), to the vectors of the count or the power of two of the sort.
+  uint32_t size = (n + 3) & ~3u;
+  if (n > 256)
+    for (size = 512; size < n;) size <<= 1;
+  if (n + tid < size) cand[n + tid] = 0;
+  for (uint32_t i = n + tid + NT; i < size; i += NT) cand[i] = 0;
+  __syncthreads();
   if (n <= 256) {
     // Few: the rank of each is the number of larger ones (no two are equal: the index is part of them).
-    for (uint32_t i = tid; i < n; i += NT) {
-      const u64 mine = cand[i];
+    if (tid < (int)n) {
+      const C mine = cand[tid];
       uint32_t rank = 0;
-      for (uint32_t j = 0; j < n; ++j) rank += cand[j] > mine;
+      constexpr int kPer = 16 / sizeof(C);
+      for (uint32_t j = 0; j < size; j += kPer) {
+        const uint4 u = *reinterpret_cast<const uint4*>(&cand[j]);
+        const C* o = reinterpret_cast<const C*>(&u);
+#pragma unroll
+        for (int e = 0; e < kPer; ++e) rank += o[e] > mine;
+      }
       if (rank < (uint32_t)k) write(rank, mine);
     }
   } else {
-    // Bitonic sort, largest first, padded with zeros to a power of two (no candidate is 0).
-    uint32_t size = 512;
-    while (size < n) size <<= 1;
-    for (uint32_t i = n + tid; i < size; i += NT) cand[i] = 0;
-    __syncthreads();
+    // Bitonic sort, largest first.
     for (uint32_t len = 2; len <= size; len <<= 1) {
       for (uint32_t half = len >> 1; half > 0; half >>= 1) {
         for (uint32_t t = tid; t < size / 2; t += NT) {
           const uint32_t i = 2 * half * (t / half) + t % half, j = i + half;
           const bool down = (i & len) == 0;
-          const u64 a = cand[i], b = cand[j];
+          const C a = cand[i], b = cand[j];
           if ((a < b) == down) {
             cand[i] = b;
             cand[j] = a;
@@ -318,22 +390,30 @@ __global__ void __launch_bounds__(NT, 1024 / NT)
 // weights are 64-bit integers round(e * 2^42), from exponentials in double precision. Integer sums do not
 // depend on their order, so results repeat bit for bit.
 //
-// One block per row. The maximum first; it gives a limit below which an element cannot be kept, or only as part
-// of a sum:
+// One block per row, which reads it twice (from memory, then from the caches): for the maximum, and to copy what
+// can matter, in index order, to lists in shared memory (one for each warp's stretch of the row), so that the
+// exponentials run on full warps. Below a limit an element cannot be kept, or only its part of a sum counts:
 //   - e < 2^-43: its weight rounds to 0;
-//   - top-k: below a limit from the threads' maxima, as in top_logits_kernel;
+//   - top-k: below a limit that a histogram of the threads' maxima gives, or of the maxima of the 8-element vectors
+//     where k is large;
 //   - top-p without top-k: e < (1 - top_p) / V, since all such elements together weigh less than what top-p
-//     drops (the maximum alone weighs 1). Their sum, a part of the total of at most 1 - top_p, is taken in fp32;
-//     its error (about 1e-9 of the total, from arguments with an exact difference and a two-part 1 / T) only
-//     moves the place of the cut, by less than a thousandth of the tokens' weight there.
-// The elements above the limit are copied, in index order, to a list in shared memory, so that the exponentials
-// run on full warps. A histogram of the list's keys (counts and weights) gives the threshold key; then the kept
-// weights are summed per 256 list places, and the group where the running sum passes its target is walked
-// by one warp. A list that does not fit is replaced by the whole row, read again from memory (L2) by each step.
-constexpr int kSegs = 4096;                // segments of 256 elements: vocabularies up to 2^20
-constexpr int kList = 32768;               // list places
+//     drops (the maximum alone weighs 1). That limit is low, so a higher one is tried first, which a part of the row
+//     says leaves three quarters of 1 - top_p below; whether it does is seen from the sums, and if not, the
+//     safe one is taken. What lies below the limit is summed in fp32; the error (about 1e-9 of the total, from
+//     arguments with an exact difference and a two-part 1 / T) only moves the place of the cut, by less than a
+//     thousandth of the tokens' weight there.
+// A histogram of the list's keys gives the threshold: counts alone where a bin is one key (its weight is the
+// count times one exponential), else counts and weights, the latter in four 11-bit limbs, since shared memory adds 32
+// bits at a time. Then the kept weights are summed per 256 list places, and the group where the running sum passes
+// its target is walked by one warp. Lists that do not fit are replaced by the whole row. All of this runs
+// once a row, mostly as cold code, so it is written in loops rather than unrolled.
+constexpr int kFine = 8192;      // bins of one key
+constexpr int kCoarse = 2048;    // bins of several
+constexpr int kGroups = 4096;    // groups of 256 elements of a whole row: vocabularies up to 2^20
+constexpr int kList = 24576;     // list places, over all warps
 constexpr double kUnit = 4398046511104.0;  // 2^42: weights of a row of 2^20 elements sum to at most 2^62
 constexpr int kExpTab = 64;
+constexpr int kGuess = 8;        // limits tried, 2.5 octaves of weight apart
 
 struct SampleParams {
   const __half* logits;
@@ -357,17 +437,18 @@ struct Exp {
   double c;        // 64 log2(e) / T
   const double* tab;
 
+  // kAny: also for values whose weight rounds to 0, down to -inf.
+  template <bool kAny>
   __device__ __forceinline__ double value(uint32_t h) const {
     // A half's bits moved to a double's places are the value times 2^-1008, subnormals too.
     const double x = __hiloint2double((int)((h & 0x8000u) << 16 | (h & 0x7fffu) << 10), 0);
     const double y = fma(x, 0x1p1008, -m) * c;  // 64 log2(e_i), exact difference
-    if (!(y > -64.0 * 60.0)) return 0.0;
+    if (kAny && !(y > -64.0 * 60.0)) return 0.0;
     const double t = y + 0x1.8p52;  // rounds to an integer, which sits in the low word
     const int n = __double2loint(t);
     const double r = y - (t - 0x1.8p52);
-    const double b = 0.010830424696249145;  // ln 2 / 64
-    const double z = r * b;
-    const double p = fma(z, fma(z, fma(z, fma(z, 1.0 / 24.0, 1.0 / 6.0), 0.5), 1.0), 1.0);
+    constexpr double b = 0.010830424696249145;  // ln 2 / 64
+    const double p = fma(r, fma(r, fma(r, fma(r, b * b * b * b / 24.0, b * b * b / 6.0), b * b / 2.0), b), 1.0);
     const double w = tab[n & (kExpTab - 1)];
     return __hiloint2double(__double2hiint(w) + ((n >> 6) << 20), __double2loint(w)) * p;
   }
@@ -382,31 +463,47 @@ struct SampleShared {
   union {
     unsigned short list[kList];
     struct {
-      u64 mass[kSegs];
-      uint32_t ties[kSegs];
+      u64 mass[kGroups];
+      uint32_t ties[kGroups];
     } row;  // groups of the whole row, where there is no list
   };
   union {
+    uint32_t fine[kFine];
     struct {
-      u64 mass[kBins];
-      uint32_t count[kBins];
-    } hist;
+      uint32_t count[kCoarse];
+      uint32_t limb[4][kCoarse];
+    } coarse;
     struct {
       u64 mass[kList / 256];
       uint32_t ties[kList / 256];
     } group;
   };
-  uint32_t seg[kSegs];  // list place of each segment's first entry
-  uint32_t sub[32];
+  uint32_t listed[32];  // entries of each warp's list
+  uint32_t sub[64];
   double tab[kExpTab];
   u64 red64[32];
   uint32_t red[32];
-  float redf[32];
+  float redf[32][kGuess + 1];
   uint32_t key, left, bin;
   u64 before;
 };
+static_assert(2 * (sizeof(SampleShared) + 1024) <= 233472, "two blocks an SM");
 
-template <int NT, int VPT, bool kRegs>
+// Weight of a logit in units of 2^-42, as an integer.
+struct Weights {
+  Exp ex;
+  uint32_t mkey;
+  __device__ __forceinline__ u64 of(uint32_t bits, uint32_t key) const {  // key >= the least lkey
+    return key == mkey ? (u64)kUnit : to_units(ex.value<false>(bits));
+  }
+};
+
+// The same as a call, for any key: an infinite maximum leaves every finite logit without weight.
+__device__ __noinline__ u64 weight_of_key(const Weights& w, uint32_t key) {
+  return key == w.mkey ? (u64)kUnit : w.mkey == 0xfc00u ? 0ull : to_units(w.ex.value<true>(key_bits(key)));
+}
+
+template <int NT>
 __global__ void __launch_bounds__(NT, 1024 / NT) sample_kernel(const SampleParams a) {
   extern __shared__ __align__(16) uint8_t smem_raw[];
   SampleShared& s = *reinterpret_cast<SampleShared*>(smem_raw);
@@ -416,39 +513,39 @@ __global__ void __launch_bounds__(NT, 1024 / NT) sample_kernel(const SampleParam
   const __half* row = a.logits + r * a.ld;
   const int vocab = a.vocab;
   const int nvec = (vocab + 7) / 8;
-  const int nchunk = kRegs ? 1 : (nvec + NT * VPT - 1) / (NT * VPT);
-  Vec v[VPT];
-  auto load = [&](int c) {
-#pragma unroll
-    for (int i = 0; i < VPT; ++i) v[i] = load_vec(row, 8 * (int64_t)((c * VPT + i) * NT + tid), vocab);
-  };
-  load(0);
-  const float T = a.temperature ? a.temperature[r] : a.temperature_s;
+  constexpr int kOwn = kList / NW;               // places of a warp's list
+  const int stretch = (nvec + NW - 1) / NW;      // vectors of a warp's part of the row
+  const int v0 = warp * stretch, v1 = min(v0 + stretch, nvec);
+  auto vec = [&](int i) { return load_vec<kFillNegInf>(row, i, vocab); };
+  const float Tr = a.temperature ? a.temperature[r] : a.temperature_s;
+  // Past these bounds the weights no longer change: fp16 logits differ by 6e-8 to 131008, or not at all.
+  const float T = Tr > 1e30f ? 1e30f : Tr > 0.f && Tr < 1e-9f ? 1e-9f : Tr;
   const int top_k = a.top_k ? a.top_k[r] : a.top_k_s;
   const float top_p = a.top_p ? a.top_p[r] : a.top_p_s;
   const float min_p = a.min_p ? a.min_p[r] : a.min_p_s;
   if (tid < kExpTab) s.tab[tid] = exp2((double)tid / kExpTab) * kUnit;
 
-  // Maximum, and whether a NaN stands in the row (a position past the end reads as one, and is not asked).
-  __half2 tmax = __half2half2(__ushort_as_half(0xffffu));
-  bool nan = false;
-  for (int c = 0; c < nchunk; ++c) {
-    if (c) load(c);
-#pragma unroll
-    for (int i = 0; i < VPT; ++i) {
-      const int64_t first = 8 * (int64_t)((c * VPT + i) * NT + tid);
-      tmax = __hmax2(tmax, vec_max2(v[i]));
-      uint32_t bad = 0;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) bad |= __hneu2_mask(as_half2(v[i].w[j]), as_half2(v[i].w[j]));
-      if (bad) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) nan |= first + j < vocab && (v[i].bits(j) & 0x7fffu) > 0x7c00u;
-      }
-    }
+  const bool use_k = top_k > 0 && top_k < vocab;
+  const bool use_p = top_p < 1.f;
+  // A limit for top-k comes from a histogram of maxima: of the threads, or of the vectors if those are few against k.
+  const bool by_thread = use_k && top_k <= min(nvec, NT) / 4, by_vector = use_k && !by_thread && top_k <= nvec / 4;
+  if (by_thread || by_vector) {
+    for (int i = tid; i < kBins; i += NT) s.fine[i] = 0;
+    if (by_vector) __syncthreads();  // else block_max has one before the first use
   }
-  const uint32_t tkey = order_key(__half_as_ushort(max_of(tmax)));
-  const uint32_t mkey = block_max<NT>(nan ? 0xffffu : tkey, s.red);
+
+  // The maximum, NaN if one stands in the row.
+  __half2 tmax = __half2half2(__ushort_as_half((unsigned short)kFillNegInf));
+#pragma unroll 4
+  for (int i = tid; i < nvec; i += NT) {
+    const Vec v = vec(i);
+    const __half2 m = __hmax2_nan(__hmax2_nan(as_half2(v.w[0]), as_half2(v.w[1])),
+                                  __hmax2_nan(as_half2(v.w[2]), as_half2(v.w[3])));
+    tmax = __hmax2_nan(tmax, m);
+    if (by_vector) atomicAdd(&s.fine[order_key(__half_as_ushort(max_of(m))) >> 5], 1u);
+  }
+  const uint32_t tkey = order_key(__half_as_ushort(__hmax_nan(__low2half(tmax), __high2half(tmax))));
+  const uint32_t mkey = block_max<NT>(tkey == 0 ? 0xffffu : tkey, s.red);
   if (mkey == 0xffffu || mkey <= kKeyNegInf) {  // a NaN, or nothing to draw from
     if (tid == 0) {
       a.tokens[r] = -1;
@@ -456,25 +553,19 @@ __global__ void __launch_bounds__(NT, 1024 / NT) sample_kernel(const SampleParam
     }
     return;
   }
-  const __half mhalf = key_half(mkey);
-  const float m32 = __half2float(mhalf);
-  const bool greedy = !(T > 0.f);
-  const bool use_k = top_k > 0 && top_k < vocab;
-  const bool use_p = top_p < 1.f;
+  const float m32 = __half2float(key_half(mkey));
 
-  if (greedy || (use_k && top_k == 1) || min_p > 1.f) {  // the lowest index of the maximum
-    const __half2 limit = __half2half2(mhalf);
+  if (!(T > 0.f) || (use_k && top_k == 1) || min_p > 1.f) {  // the lowest index of the maximum
+    const __half2 limit = __half2half2(key_half(mkey));
     uint32_t best = 0;  // ~index, so that the largest is the lowest index
-    for (int c = 0; c < nchunk; ++c) {
-      if (nchunk > 1) load(c);
+#pragma unroll 1
+    for (int i = tid; i < nvec; i += NT) {
+      const uint32_t ge = vec_ge(vec(i), limit);
+      if (ge) {
 #pragma unroll
-      for (int i = 0; i < VPT; ++i) {
-        const uint32_t ge = vec_ge(v[i], limit);
-        if (ge) {
-#pragma unroll
-          for (int j = 7; j >= 0; --j)
-            if (ge & ge_bit(j)) best = max(best, ~(uint32_t)(8 * ((c * VPT + i) * NT + tid) + j));
-        }
+        for (int j = 0; j < 8; ++j)
+          if (ge & ge_bit(j)) best = max(best, ~(uint32_t)(8 * i + j));
+        break;
       }
     }
     best = block_max<NT>(best, s.red);
@@ -485,18 +576,16 @@ __global__ void __launch_bounds__(NT, 1024 / NT) sample_kernel(const SampleParam
     return;
   }
 
-  const Exp ex{(double)m32, 64.0 * 1.4426950408889634 / (double)T, s.tab};
-  // An infinite maximum leaves every finite logit without weight.
+  const Weights wt{{(double)m32, 64.0 * 1.4426950408889634 / (double)T, s.tab}, mkey};
   const bool minf = mkey == 0xfc00u;
-  auto units = [&](uint32_t bits, uint32_t key) -> u64 {
-    return key == mkey ? (u64)kUnit : minf ? 0ull : to_units(ex.value(bits));
-  };
 
   // Elements below `lkey` stay out of the list. First: weights that round to 0.
   auto key_below = [&](float x) {  // key of the largest half <= x, and never that of -inf
     return max(order_key(__half_as_ushort(__float2half_rd(x))), kKeyNegInf + 1);
   };
-  uint32_t lkey = minf ? mkey : min(mkey, key_below(m32 - 30.2f * T));
+  // (30.2 nats are 2^-43.57; the bound itself is rounded up, so that no exponent is below that.)
+  uint32_t lkey = mkey;
+  if (!minf) lkey = min(mkey, max(order_key(__half_as_ushort(__float2half_ru(m32 - 30.2f * T))), kKeyNegInf + 1));
 
   // min-p as a key: the smallest key whose weight reaches it (32 probes a step, every warp for itself).
   uint32_t mpkey = 0;
@@ -506,7 +595,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) sample_kernel(const SampleParam
     while (hi - lo > 1) {
       const uint32_t step = (hi - lo + 31) / 32;
       const uint32_t key = min(lo + (lane + 1) * step, hi);
-      const bool ok = key == mkey || (!minf && ex.value(key_bits(key)) >= want);
+      const bool ok = key == mkey || (!minf && wt.ex.value<true>(key_bits(key)) >= want);
       const uint32_t first = __ffs(__ballot_sync(0xffffffffu, ok)) - 1;
       hi = min(lo + (first + 1) * step, hi);
       lo += first * step;
@@ -516,174 +605,230 @@ __global__ void __launch_bounds__(NT, 1024 / NT) sample_kernel(const SampleParam
   }
 
   const bool tail = use_p && !use_k && !minf;  // what is below the limit is part of the sum
-  if (use_k && top_k * 4 <= min(nvec, NT)) {
-    for (int i = tid; i < kBins; i += NT) s.hist.count[i] = 0;
-    __syncthreads();
-    if (tkey) atomicAdd(&s.hist.count[tkey >> 5], 1u);
+  uint32_t safe = lkey;                        // of a tried limit: the one that is always low enough
+  const float c = (float)(1.4426950408889634 / (double)T);  // exponents are fma(x, c, c0)
+  const float c0 = (float)(-(double)m32 * (double)c);
+  if (by_thread || by_vector) {
+    if (by_thread) atomicAdd(&s.fine[tkey >> 5], 1u);
     __syncthreads();
     int* found = reinterpret_cast<int*>(&s.key);  // key, left
-    find_bin<NT>(s.hist.count, (uint32_t)top_k, s.red, found);
+    find_bin<NT>(s.fine, (uint32_t)top_k, s.red, found);
     if (found[0] >= 0) lkey = max(lkey, (uint32_t)found[0] << 5);
   } else if (tail) {
-    lkey = max(lkey, min(mkey, key_below(m32 + T * logf((1.f - fmaxf(top_p, 0.f)) * 0.999f / (float)vocab))));
+    safe = lkey = max(lkey, min(mkey, key_below(m32 + T * logf((1.f - fmaxf(top_p, 0.f)) * 0.999f / (float)vocab))));
+    // From the row's first part: the weight below 2^-2.5, 2^-5, ... of the maximum.
+    float below[kGuess + 1] = {};
+    const Vec v = vec(tid);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float2 f = __half22float2(as_half2(v.w[j]));
+      const float y0 = fmaf(f.x, c, c0), y1 = fmaf(f.y, c, c0);
+      const float e0 = ex2(y0), e1 = ex2(y1);
+      below[kGuess] += e0 + e1;
+#pragma unroll
+      for (int g = 0; g < kGuess; ++g) {
+        if (y0 < -2.5f * (g + 1)) below[g] += e0;
+        if (y1 < -2.5f * (g + 1)) below[g] += e1;
+      }
+    }
+#pragma unroll
+    for (int g = 0; g <= kGuess; ++g) {
+      below[g] = warp_sum(below[g]);
+      if (lane == 0) s.redf[warp][g] = below[g];
+    }
+    __syncthreads();
+    float sum = 0.f;
+    if (lane <= kGuess)
+      for (int w = 0; w < NW; ++w) sum += s.redf[w][lane];
+    // The whole row's weight: the light part scaled up, of the heavy one what was seen, or the maximum's.
+    const float share = (float)vocab / (float)min(vocab, NT * 8);
+    const float light = __shfl_sync(0xffffffffu, sum, 1);
+    const float all = fmaxf(__shfl_sync(0xffffffffu, sum, kGuess) - light, 1.f) + light * share;
+    // The first level that leaves three quarters of 1 - top_p below it, and a place between it and the one before.
+    const float want = 0.75f * (1.f - top_p) * all;
+    const uint32_t fits = __ballot_sync(0xffffffffu, lane < kGuess && sum * share <= want);
+    if (fits) {
+      const int g = __ffs(fits) - 1;
+      const float upper = __shfl_sync(0xffffffffu, sum, max(g - 1, 0)) * share, lower = __shfl_sync(0xffffffffu, sum, g) * share;
+      float at = (float)(g + 1);
+      if (g > 0) at = (float)g + log2f(upper / want) / fmaxf(log2f(upper / fmaxf(lower, 1e-30f)), 1e-3f);
+      lkey = max(lkey, min(mkey, key_below(m32 - 2.5f * fminf(at, (float)(g + 1)) / c)));
+    }
+    __syncthreads();
   }
 
-  // The list: entries per segment of 256 elements (one warp's vectors of one step), their places, the copy.
-  const __half2 limit = __half2half2(key_half(lkey));
-  const int nseg = (vocab + 255) / 256;
-  float rest = 0.f;
-  const float c_hi = (float)(1.4426950408889634 / (double)T);
-  const float c_lo = (float)(1.4426950408889634 / (double)T - (double)c_hi);
-  for (int c = 0; c < nchunk; ++c) {
-    if (nchunk > 1) load(c);
-#pragma unroll
-    for (int i = 0; i < VPT; ++i) {
-      const uint32_t ge = vec_ge(v[i], limit);
-      const uint32_t n = __reduce_add_sync(0xffffffffu, __popc(ge));
-      const int seg = (c * VPT + i) * NW + warp;
-      if (lane == 0 && seg < nseg) s.seg[seg] = n;
-      if (tail) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float2 f = __half22float2(as_half2(v[i].w[j]));
-          const float d0 = f.x - m32, d1 = f.y - m32;
-          const float e0 = exp2f(fmaf(d0, c_hi, d0 * c_lo)), e1 = exp2f(fmaf(d1, c_hi, d1 * c_lo));
-          // a position past the end is a NaN, for which e < 2 is false too
-          rest += (!(ge & ge_bit(2 * j)) && e0 < 2.f ? e0 : 0.f) + (!(ge & ge_bit(2 * j + 1)) && e1 < 2.f ? e1 : 0.f);
-        }
-      }
+  uint32_t tau, left;      // the lowest key kept; how many of the elements at it (0xffffffff: all)
+  bool lists;              // or the whole row
+  int ngroup;
+  __half2 limit;
+  // Group g: up to 256 entries that follow each other in the row.
+  auto group = [&](int g, int& count) -> const unsigned short* {
+    if (!lists) {
+      count = min(256, vocab - g * 256);
+      return reinterpret_cast<const unsigned short*>(row) + g * 256;
     }
-  }
-  u64 tail_mass = 0;
-  if (tail) {
-    rest = warp_sum(rest);
-    if (lane == 0) s.redf[warp] = rest;
-    __syncthreads();
-    tail_mass = to_units((double)warp_sum(lane < NW ? s.redf[lane] : 0.f) * kUnit);
-  }
-  __syncthreads();
-  uint32_t nlist;
-  {
-    constexpr int PER = kSegs / NT;
-    uint32_t n[PER], sum = 0;
-    const int per = (nseg + NT - 1) / NT;  // segments a thread
-#pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      n[i] = i < per && tid * per + i < nseg ? s.seg[tid * per + i] : 0u;
-      sum += n[i];
-    }
-    uint32_t at = block_scan<NT>(sum, s.red, &nlist);
-#pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      if (i < per && tid * per + i < nseg) s.seg[tid * per + i] = at;
-      at += n[i];
-    }
-  }
-  __syncthreads();
-  const bool listed = nlist <= kList;
-  if (listed) {
-    for (int c = 0; c < nchunk; ++c) {
-      if (nchunk > 1) load(c);
-#pragma unroll
-      for (int i = 0; i < VPT; ++i) {
-        const uint32_t ge = vec_ge(v[i], limit);
-        if (__any_sync(0xffffffffu, ge)) {
-          const int seg = (c * VPT + i) * NW + warp;
-          const uint32_t n = __popc(ge);
-          uint32_t at = s.seg[min(seg, nseg - 1)] + warp_scan(n) - n;
-#pragma unroll
-          for (int j = 0; j < 8; ++j)
-            if (ge & ge_bit(j)) s.list[at++] = (unsigned short)v[i].bits(j);
-        }
-      }
-    }
-  }
-  const uint32_t n = listed ? nlist : (uint32_t)vocab;  // places
-  const unsigned short* source = listed ? s.list : reinterpret_cast<const unsigned short*>(row);
-  auto entry = [&](uint32_t place, uint32_t& bits) -> uint32_t {  // key, or 0 where nothing is
-    bits = source[place];
+    constexpr int kPer = kOwn / 256;
+    count = min(256, (int)s.listed[g / kPer] - g % kPer * 256);
+    return s.list + g * 256;
+  };
+  auto key_of = [&](uint32_t bits) -> uint32_t {  // 0 below the limit (a whole row has such entries)
     const uint32_t key = order_key(bits);
     return key >= lkey ? key : 0u;
   };
-  __syncthreads();
-
-  // tau: the lowest key kept; left: how many of the elements at it (0xffffffff: all).
-  uint32_t tau = lkey, left = 0xffffffffu;
-  if (use_k || use_p) {
-    int shift = 0;
-    while (((mkey - lkey) >> shift) >= kBins) ++shift;
-    for (int i = tid; i < kBins; i += NT) {
-      s.hist.count[i] = 0;
-      s.hist.mass[i] = 0;
+  for (;;) {  // at most twice
+    // The lists, and the weight of what stays out of them.
+    limit = __half2half2(key_half(lkey));
+    const float limit32 = __half2float(key_half(lkey));
+    float rest = 0.f;
+    uint32_t mine = 0;
+#pragma unroll 2
+    for (int i = v0 + lane; i < v0 + (v1 - v0 + 31 & ~31); i += 32) {
+      Vec v;
+      v.w[0] = v.w[1] = v.w[2] = v.w[3] = kFillNegInf * 0x10001u;
+      if (i < v1) v = vec(i);
+      const uint32_t ge = vec_ge(v, limit);
+      if (__any_sync(0xffffffffu, ge)) {
+        const uint32_t cnt = __popc(ge);
+        const uint32_t upto = warp_scan(cnt);
+        uint32_t at = mine + upto - cnt;
+        mine += __shfl_sync(0xffffffffu, upto, 31);
+        if (mine <= kOwn) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            if (ge & ge_bit(j)) s.list[warp * kOwn + at++] = (unsigned short)v.bits(j);
+        }
+      }
+      if (tail) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float2 f = __half22float2(as_half2(v.w[j]));
+          const float e0 = ex2(fmaf(f.x, c, c0)), e1 = ex2(fmaf(f.y, c, c0));
+          if (f.x < limit32) rest += e0;
+          if (f.y < limit32) rest += e1;
+        }
+      }
+    }
+    if (lane == 0) s.listed[warp] = mine;
+    if (tail) {
+      rest = warp_sum(rest);
+      if (lane == 0) s.redf[warp][0] = rest;
     }
     __syncthreads();
-    for (uint32_t p = tid; p < n; p += NT) {
-      uint32_t bits;
-      const uint32_t key = entry(p, bits);
-      if (key) {
+    u64 tail_mass = 0;
+    if (tail) {
+      // What c and c0 lost to rounding, for the difference to the maximum that the weight below the limit has about: a
+      // nat under it.
+      const double lost = ((double)limit32 - (double)m32 - (double)T) * (1.4426950408889634 / (double)T - (double)c) +
+                          (-(double)m32 * (double)c - (double)c0);
+      tail_mass = to_units((double)warp_sum(lane < NW ? s.redf[lane][0] : 0.f) * (1.0 + 0.6931471805599453 * lost) * kUnit);
+    }
+    lists = __reduce_max_sync(0xffffffffu, lane < NW ? s.listed[lane] : 0u) <= kOwn;
+    ngroup = lists ? kList / 256 : (vocab + 255) / 256;
+
+    tau = lkey, left = 0xffffffffu;
+    if (!use_k && !use_p) break;
+    // Bins in descending order of the keys; more than one key to a bin only where the range is wide.
+    const uint32_t range = mkey - lkey;
+    int shift = 0;
+    if (range >= kFine)
+      for (shift = 1; (range >> shift) >= kCoarse;) ++shift;
+    const int bins = (int)(range >> shift) + 1;
+    for (int i = tid; i < bins; i += NT) s.fine[i] = 0;
+    if (shift)
+      for (int i = tid; i < bins; i += NT)
+        s.coarse.limb[0][i] = s.coarse.limb[1][i] = s.coarse.limb[2][i] = s.coarse.limb[3][i] = 0;
+    __syncthreads();
+#pragma unroll 1
+    for (int g = warp; g < ngroup; g += NW) {
+      int count;
+      const unsigned short* p = group(g, count);
+#pragma unroll 1
+      for (int i = lane; i < count; i += 32) {
+        const uint32_t bits = p[i], key = key_of(bits);
+        if (!key) continue;
         const uint32_t b = (mkey - key) >> shift;
-        atomicAdd(&s.hist.count[b], 1u);
-        if (use_p) atomicAdd(&s.hist.mass[b], units(bits, key));
+        atomicAdd(&s.fine[b], 1u);
+        if (shift && use_p) {
+          const u64 w = wt.of(bits, key);
+#pragma unroll
+          for (int l = 0; l < 4; ++l) atomicAdd(&s.coarse.limb[l][b], (uint32_t)(w >> (11 * l)) & 0x7ffu);
+        }
       }
     }
     __syncthreads();
-    constexpr int PER = kBins / NT;
-    uint32_t cnt[PER], csum = 0, ctotal;
-    u64 mass[PER], msum = 0, mtotal = 0, mabove = 0;
-#pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      cnt[i] = s.hist.count[tid * PER + i];
-      csum += cnt[i];
-      mass[i] = s.hist.mass[tid * PER + i];
-      msum += mass[i];
+    auto bin_mass = [&](int b) -> u64 {
+      if (shift)
+        return s.coarse.limb[0][b] + ((u64)s.coarse.limb[1][b] << 11) + ((u64)s.coarse.limb[2][b] << 22) +
+               ((u64)s.coarse.limb[3][b] << 33);
+      const uint32_t cnt = s.fine[b];
+      return cnt ? cnt * weight_of_key(wt, mkey - b) : 0ull;
+    };
+    const int per = (bins + NT - 1) / NT;
+    const int b0 = min(tid * per, bins), b1 = min(b0 + per, bins);
+    uint32_t csum = 0, ctotal;
+    u64 msum = 0, mtotal = 0, mabove = 0;
+#pragma unroll 1
+    for (int i = b0; i < b1; ++i) {
+      csum += s.fine[i];
+      if (use_p) {
+        if (shift)
+          msum += bin_mass(i);
+        else if (s.fine[i])
+          msum += s.fine[i] * wt.of(key_bits(mkey - i), mkey - i);
+      }
     }
     const uint32_t cabove = block_scan<NT>(csum, s.red, &ctotal);
     if (use_p) mabove = block_scan<NT>(msum, s.red64, &mtotal);
+    if (lkey > safe && (double)mtotal < (double)fmaxf(top_p, 0.f) * (double)(mtotal + tail_mass) * (1.0 + 1e-6)) {
+      lkey = safe;  // the cut lies below the limit after all
+      continue;
+    }
     mtotal += tail_mass;
 
-    // Counts of a bin's keys, in descending order of the keys.
+    // Counts of a bin's keys (up to 64), in descending order of the keys.
     auto fill_sub = [&](uint32_t bin) {
-      if (tid < 32) s.sub[tid] = 0;
+      if (tid < 64) s.sub[tid] = 0;
       __syncthreads();
-      for (uint32_t p = tid; p < n; p += NT) {
-        uint32_t bits;
-        const uint32_t key = entry(p, bits), d = mkey - key;
-        if (key && d >> shift == bin) atomicAdd(&s.sub[d & ((1u << shift) - 1u)], 1u);
+#pragma unroll 1
+      for (int g = warp; g < ngroup; g += NW) {
+        int count;
+        const unsigned short* p = group(g, count);
+#pragma unroll 1
+        for (int i = lane; i < count; i += 32) {
+          const uint32_t key = key_of(p[i]), d = mkey - key;
+          if (key && d >> shift == bin) atomicAdd(&s.sub[d & ((1u << shift) - 1u)], 1u);
+        }
       }
       __syncthreads();
     };
 
     if (use_k && (uint32_t)top_k < ctotal) {
-      uint32_t ab = cabove;
-      u64 mb = mabove;
-      if (ab < (uint32_t)top_k && ab + csum >= (uint32_t)top_k) {
-#pragma unroll
-        for (int i = 0; i < PER; ++i) {
-          if (ab < (uint32_t)top_k && ab + cnt[i] >= (uint32_t)top_k) {
-            s.bin = tid * PER + i;
-            s.left = (uint32_t)top_k - ab;
-            s.before = mb;
-          }
-          ab += cnt[i];
-          mb += mass[i];
+      if (cabove < (uint32_t)top_k && cabove + csum >= (uint32_t)top_k) {  // one thread
+        uint32_t ab = cabove;
+        u64 mb = mabove;
+        int i = b0;
+        while (ab + s.fine[i] < (uint32_t)top_k) {
+          ab += s.fine[i];
+          if (use_p) mb += bin_mass(i);
+          ++i;
         }
+        s.bin = i;
+        s.left = (uint32_t)top_k - ab;
+        s.before = mb;
       }
       __syncthreads();
       const uint32_t bin = s.bin;
       if (shift) fill_sub(bin);
-      if (tid < 32) {
-        const uint32_t key = mkey - ((bin << shift) + (shift ? lane : 0));
-        const uint32_t want = s.left;
-        const uint32_t c = shift ? s.sub[lane] : lane == 0 ? want : 0u;
-        const uint32_t inc = warp_scan(c);
-        const bool here = inc - c < want && inc >= want;
-        const uint32_t take = here ? want - (inc - c) : inc < want ? c : 0u;
-        const u64 w = warp_sum64(take ? (u64)take * units(key_bits(key), key) : 0ull);
-        if (here) {
-          s.key = key;
-          s.left = take;
-          s.before += w;  // the weight of the first top_k
-        }
+      if (tid == 0) {
+        uint32_t want = s.left, key = mkey - (bin << shift);
+        if (shift)
+          for (int i = 0; s.sub[i] < want; ++i, --key) {
+            want -= s.sub[i];
+            if (use_p && s.sub[i]) s.before += s.sub[i] * weight_of_key(wt, key);
+          }
+        if (use_p) s.before += want * weight_of_key(wt, key);  // the weight of the first top_k
+        s.key = key;
+        s.left = want;
       }
       __syncthreads();
       tau = s.key;
@@ -693,32 +838,38 @@ __global__ void __launch_bounds__(NT, 1024 / NT) sample_kernel(const SampleParam
     }
     if (use_p) {
       // Kept are the ranks with less than `target` before them, and the first.
-      const double target = (double)fmaxf(top_p, 0.f) * (double)mtotal;
-      u64 mb = mabove;
+      const double target = fmax((double)top_p * (double)mtotal, 1.0);  // in units: the first has 2^42
       if (tid == 0) s.bin = 0xffffffffu;
       __syncthreads();
-#pragma unroll
-      for (int i = 0; i < PER; ++i) {
-        // Of one bin at most: the weight before it is below the target (or it is the maximum's), that with it not.
-        if (mass[i] && (mb == 0 || (double)mb < target) && (double)(mb + mass[i]) >= target) {
-          s.bin = tid * PER + i;
-          s.before = mb;
+      if ((double)mabove < target && (double)(mabove + msum) >= target) {  // one thread, if the target is within
+        u64 mb = mabove;
+        int i = b0;
+        for (; i < b1 - 1; ++i) {
+          const u64 m = bin_mass(i);
+          if ((double)(mb + m) >= target) break;
+          mb += m;
         }
-        mb += mass[i];
+        s.bin = i;
+        s.before = mb;
       }
       __syncthreads();
       const uint32_t bin = s.bin;
       if (bin != 0xffffffffu) {
         if (shift) fill_sub(bin);
-        if (tid < 32) {
-          const uint32_t key = mkey - ((bin << shift) + (shift ? lane : 0));
-          const uint32_t c = shift ? s.sub[lane] : lane == 0 ? s.hist.count[bin] : 0u;
-          const u64 w = c ? units(key_bits(key), key) : 0ull;
-          const u64 inc = s.before + warp_scan((u64)c * w), exc = inc - (u64)c * w;
-          if (w && (exc == 0 || (double)exc < target) && (double)inc >= target) {
-            s.key = key;
-            s.left = (uint32_t)fmin(fmax(ceil((target - (double)exc) / (double)w), 1.0), (double)c);
+        if (tid == 0) {
+          uint32_t key = mkey - (bin << shift), cnt = shift ? s.sub[0] : s.fine[bin];
+          u64 mb = s.before, w = weight_of_key(wt, key);
+          if (shift) {
+            const int last = (1 << shift) - 1;
+            for (int i = 0; i < last && (double)(mb + cnt * w) < target;) {
+              mb += cnt * w;
+              cnt = s.sub[++i];
+              --key;
+              w = cnt ? weight_of_key(wt, key) : 0ull;
+            }
           }
+          s.key = key;
+          s.left = w ? (uint32_t)fmin(fmax(ceil((target - (double)mb) / (double)w), 1.0), (double)cnt) : cnt;
         }
         __syncthreads();
         // Never past the top-k threshold.
@@ -733,30 +884,32 @@ __global__ void __launch_bounds__(NT, 1024 / NT) sample_kernel(const SampleParam
       left = 0xffffffffu;
     }
     __syncthreads();  // the histogram's memory becomes the groups'
+    break;
   }
 
-  // Weights and ties at tau per group of 256 places, which lie in the order (step, lane).
+  // Weights and ties at tau per group.
   const bool ties = left != 0xffffffffu;
-  u64* gmass = listed ? s.group.mass : s.row.mass;
-  uint32_t* gties = listed ? s.group.ties : s.row.ties;
-  const int ngroup = (int)((n + 255) / 256);
+  u64* gmass = lists ? s.group.mass : s.row.mass;
+  uint32_t* gties = lists ? s.group.ties : s.row.ties;
+#pragma unroll 1
   for (int g = warp; g < ngroup; g += NW) {
+    int count;
+    const unsigned short* p = group(g, count);
     u64 w = 0;
     uint32_t tie = 0;
-#pragma unroll 2
-    for (int j = 0; j < 8; ++j) {
-      const uint32_t p = g * 256 + j * 32 + lane;
-      if (p < n) {
-        uint32_t bits;
-        const uint32_t key = entry(p, bits);
-        if (ties && key == tau)
-          ++tie;
-        else if (key >= tau)
-          w += units(bits, key);
-      }
+#pragma unroll 1
+    for (int i = lane; i < count; i += 32) {
+      const uint32_t bits = p[i], key = key_of(bits);
+      if (ties && key == tau)
+        ++tie;
+      else if (key >= tau)
+        w += wt.of(bits, key);
     }
-    w = warp_sum64(w);
-    tie = __reduce_add_sync(0xffffffffu, tie);
+    __syncwarp();
+    if (count > 0) {
+      w = warp_sum64(w);
+      tie = __reduce_add_sync(0xffffffffu, tie);
+    }
     if (lane == 0) {
       gmass[g] = w;
       gties[g] = tie;
@@ -766,15 +919,16 @@ __global__ void __launch_bounds__(NT, 1024 / NT) sample_kernel(const SampleParam
   if (warp != 0) return;
 
   // One warp: a run of groups per lane. Ties are kept while fewer than `left` stand before them.
-  const u64 wtie = ties ? units(key_bits(tau), tau) : 0ull;
+  const u64 wtie = ties ? weight_of_key(wt, tau) : 0ull;
   const int per = (ngroup + 31) / 32;
   const int g0 = min(lane * per, ngroup), g1 = min(g0 + per, ngroup);
   uint32_t tsum = 0;
-  for (int g = g0; g < g1; ++g) tsum += gties[g];
+  u64 wsum = 0;
+#pragma unroll 1
+  for (int g = g0; g < g1; ++g) tsum += gties[g], wsum += gmass[g];
   uint32_t tb = warp_scan(tsum) - tsum;
-  auto kept = [&](uint32_t before, uint32_t c) -> uint32_t { return before >= left ? 0u : min(c, left - before); };
-  u64 wsum = (u64)kept(tb, tsum) * wtie;
-  for (int g = g0; g < g1; ++g) wsum += gmass[g];
+  auto kept = [&](uint32_t before, uint32_t n) -> uint32_t { return before >= left ? 0u : min(n, left - before); };
+  wsum += (u64)kept(tb, tsum) * wtie;
   const u64 winc = warp_scan(wsum);
   const u64 total = __shfl_sync(0xffffffffu, winc, 31);
   // The first place whose running weight exceeds u * total.
@@ -785,6 +939,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) sample_kernel(const SampleParam
   int g = 0;
   const bool mine = wb <= target && target < winc;
   if (mine) {
+#pragma unroll 1
     for (g = g0; g < g1; ++g) {
       const u64 w = gmass[g] + (u64)kept(tb, gties[g]) * wtie;
       if (target < wb + w) break;
@@ -796,19 +951,22 @@ __global__ void __launch_bounds__(NT, 1024 / NT) sample_kernel(const SampleParam
   g = __shfl_sync(0xffffffffu, g, src);
   wb = __shfl_sync(0xffffffffu, wb, src);
   tb = __shfl_sync(0xffffffffu, tb, src);
+  // Within the group, 32 entries at a time.
+  int count;
+  const unsigned short* p = group(g, count);
   uint32_t place = 0, tkeyf = mkey;
-  for (int j = 0; j < 8; ++j) {
-    const uint32_t p = g * 256 + j * 32 + lane;
-    uint32_t bits = 0;
-    const uint32_t key = p < n ? entry(p, bits) : 0u;
+#pragma unroll 1
+  for (int j = 0; j < count; j += 32) {
+    const uint32_t bits = j + lane < count ? p[j + lane] : 0u;
+    const uint32_t key = j + lane < count ? key_of(bits) : 0u;
     const uint32_t tie = __ballot_sync(0xffffffffu, ties && key == tau);
     const uint32_t t_here = tb + __popc(tie & ((1u << lane) - 1u));
-    const u64 w = ties && key == tau ? (t_here < left ? wtie : 0ull) : key >= tau ? units(bits, key) : 0ull;
+    const u64 w = ties && key == tau ? (t_here < left ? wtie : 0ull) : key >= tau ? wt.of(bits, key) : 0ull;
     const u64 inc = wb + warp_scan(w);
     const uint32_t hit = __ballot_sync(0xffffffffu, target < inc);
     if (hit) {
       const int l = __ffs(hit) - 1;
-      place = g * 256 + j * 32 + l;
+      place = g * 256 + j + l;
       tkeyf = __shfl_sync(0xffffffffu, key, l);
       break;
     }
@@ -816,29 +974,31 @@ __global__ void __launch_bounds__(NT, 1024 / NT) sample_kernel(const SampleParam
     tb += __popc(tie);
   }
 
-  // The element at that place: its segment, then the entry's rank within it.
+  // The element of that place: in a list, the so-manieth above the limit of its warp's stretch.
   int64_t token = place;
-  if (listed) {
-    int lo = 0, hi = nseg;  // the last segment that begins at or before the place
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) / 2;
-      if (s.seg[mid] <= place)
-        lo = mid;
-      else
-        hi = mid;
-    }
-    const int64_t first = (int64_t)lo * 256 + lane * 8;
-    const uint32_t ge = vec_ge(load_vec(row, first, vocab), limit);
-    const uint32_t c = __popc(ge), want = place - s.seg[lo];
-    uint32_t before = warp_scan(c) - c;
-    uint32_t found = 0;  // index + 1
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-      if (ge & ge_bit(j)) {
-        if (before == want) found = (uint32_t)(first + j) + 1;
-        ++before;
+  if (lists) {
+    const int w = place / kOwn;
+    uint32_t want = place - w * kOwn;
+    const int e1 = min((w + 1) * stretch, nvec);
+#pragma unroll 1
+    for (int i = w * stretch + lane;; i += 32) {
+      const uint32_t ge = i < e1 ? vec_ge(vec(i), limit) : 0u;
+      const uint32_t cnt = __popc(ge), upto = warp_scan(cnt), here = __shfl_sync(0xffffffffu, upto, 31);
+      if (want >= here) {
+        if (i - lane + 32 >= e1) break;  // (never: the list has that many)
+        want -= here;
+        continue;
       }
-    token = (int64_t)__reduce_max_sync(0xffffffffu, found) - 1;
+      uint32_t before = upto - cnt, found = 0;  // index + 1
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (ge & ge_bit(j)) {
+          if (before == want) found = (uint32_t)(i * 8 + j) + 1;
+          ++before;
+        }
+      token = (int64_t)__reduce_max_sync(0xffffffffu, found) - 1;
+      break;
+    }
   }
   if (lane == 0) {
     a.tokens[r] = token;
@@ -849,17 +1009,16 @@ __global__ void __launch_bounds__(NT, 1024 / NT) sample_kernel(const SampleParam
   }
 }
 
-template <int NT, int VPT, bool kRegs>
+template <int NT>
 int launch_sample(const SampleParams& p, int64_t rows, cudaStream_t s) {
   static std::atomic<uint64_t> done{0};
   JX_CUDA_TRY(once_per_device(done,
                               [] {
-                                return cudaFuncSetAttribute(sample_kernel<NT, VPT, kRegs>,
-                                                            cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                return cudaFuncSetAttribute(sample_kernel<NT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                                             (int)sizeof(SampleShared));
                               }),
               "jx_sample: shared memory");
-  sample_kernel<NT, VPT, kRegs><<<(unsigned)rows, NT, sizeof(SampleShared), s>>>(p);
+  sample_kernel<NT><<<(unsigned)rows, NT, sizeof(SampleShared), s>>>(p);
   JX_CHECK_LAUNCH("jx_sample");
   return JX_OK;
 }
@@ -871,14 +1030,18 @@ using namespace jx;
 
 extern "C" int jx_top_logits(const void* logits16, int64_t rows, int vocab, int64_t ld, int k, void* values16,
                              int64_t* ids, jx_stream_t stream) {
-  JX_CHECK_ARG(rows > 0 && rows <= 0x7fffffff && vocab > 0 && ld >= vocab, "jx_top_logits: bad shape");
+  JX_CHECK_ARG(rows > 0 && rows <= 0x7fffffff && vocab > 0 && vocab <= 1 << 30 && ld >= vocab, "jx_top_logits: bad shape");
   JX_CHECK_ARG(k > 0 && k <= vocab && k <= sel::kMaxTop, "jx_top_logits: k must be in [1, min(vocab, %d)] (got %d)",
                sel::kMaxTop, k);
   JX_CHECK_ARG(logits16 && values16 && ids, "jx_top_logits: NULL argument");
   JX_CHECK_ARG(ld % 8 == 0 && aligned16(logits16), "jx_top_logits: ld%%8 and 16B alignment required");
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  sel::top_logits_kernel<512, 8><<<(unsigned)rows, 512, 0, s>>>(static_cast<const __half*>(logits16), ld, vocab, k,
-                                                               static_cast<__half*>(values16), ids);
+  const __half* x = static_cast<const __half*>(logits16);
+  __half* v = static_cast<__half*>(values16);
+  if (vocab <= 65536)
+    sel::top_logits_kernel<512, 8, uint32_t><<<(unsigned)rows, 512, 0, s>>>(x, ld, vocab, k, v, ids);
+  else
+    sel::top_logits_kernel<512, 8, sel::u64><<<(unsigned)rows, 512, 0, s>>>(x, ld, vocab, k, v, ids);
   JX_CHECK_LAUNCH("jx_top_logits");
   return JX_OK;
 }
@@ -888,13 +1051,12 @@ extern "C" int jx_sample(const void* logits16, int64_t rows, int vocab, int64_t 
                          const float* top_ps, float top_p, const float* min_ps, float min_p, int64_t* tokens,
                          float* logprobs, jx_stream_t stream) {
   JX_CHECK_ARG(logits16 && uniforms && tokens, "jx_sample: NULL argument");
-  JX_CHECK_ARG(rows > 0 && rows <= 0x7fffffff && vocab > 0 && vocab <= sel::kSegs * 256 && ld >= vocab,
-               "jx_sample: bad shape (rows %lld, vocab %d, at most %d)", (long long)rows, vocab, sel::kSegs * 256);
+  JX_CHECK_ARG(rows > 0 && rows <= 0x7fffffff && vocab > 0 && vocab <= sel::kGroups * 256 && ld >= vocab,
+               "jx_sample: bad shape (rows %lld, vocab %d, at most %d)", (long long)rows, vocab, sel::kGroups * 256);
   JX_CHECK_ARG(ld % 8 == 0 && aligned16(logits16), "jx_sample: ld%%8 and 16B alignment required");
   sel::SampleParams p{static_cast<const __half*>(logits16), ld, vocab, uniforms, temperatures, top_ks, top_ps, min_ps,
                       temperature, top_p, min_p, top_k, tokens, logprobs};
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  // Rows that a block's registers hold are read once, longer ones again by each step.
-  if (vocab <= 1024 * 8 * 4) return sel::launch_sample<1024, 4, true>(p, rows, s);
-  return sel::launch_sample<1024, 4, false>(p, rows, s);
+  // Two blocks of 512 threads share an SM where there are rows for them, else a row gets 1024.
+  return rows > num_sms() ? sel::launch_sample<512>(p, rows, s) : sel::launch_sample<1024>(p, rows, s);
 }

@@ -53,7 +53,8 @@ def _ptr(t: torch.Tensor | None) -> int | None:
 
 
 def _stream() -> int:
-    return torch.cuda.current_stream().cuda_stream
+    """The current device's current stream (the handle alone: building torch's Stream object costs about 5 us a call)."""
+    return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
 
 
 def _check(t: torch.Tensor, dtype: torch.dtype, name: str, contiguous: bool = True) -> None:
@@ -69,14 +70,24 @@ def _check(t: torch.Tensor, dtype: torch.dtype, name: str, contiguous: bool = Tr
 
 def _check_here(**tensors: torch.Tensor | None) -> None:
     """Every tensor must be on the current device: the launch goes to its current stream."""
-    here = torch.cuda.current_device()
+    here = torch._C._cuda_getDevice()
     for name, t in tensors.items():
-        if t is not None and t.device.index != here:
+        if t is not None and t.get_device() != here:
             raise ValueError(f"{name} is on {t.device}, the current device is cuda:{here}")
 
 
+def _plain(dtype: torch.dtype, *tensors) -> bool:
+    """Whether all are contiguous tensors of this type on the current device: the common case in one step; where
+    it fails the callers' own checks find out what is wrong."""
+    here = torch._C._cuda_getDevice() if torch.cuda.is_initialized() else -2
+    for t in tensors:
+        if not isinstance(t, torch.Tensor) or t.dtype is not dtype or t.get_device() != here or not t.is_contiguous():
+            return False
+    return True
+
+
 def _shape(t: torch.Tensor, shape: tuple, name: str) -> None:
-    if tuple(t.shape) != shape:
+    if t.shape != shape:
         raise ValueError(f"{name} must have shape {shape}, got {tuple(t.shape)}")
 
 
@@ -372,43 +383,50 @@ def attn_decode_prefix(qkv: torch.Tensor, kprefix: torch.Tensor, vprefix: torch.
     marks an idle sequence (zero output, nothing appended). `max_len` is their upper bound (default: the caches'
     rows). Returns [B, H*D]. Calls that may overlap need workspaces of their own."""
     kv = H if kv_heads is None else kv_heads
-    for name, t in (("qkv", qkv), ("kprefix", kprefix), ("vprefix", vprefix), ("kcache", kcache), ("vcache", vcache)):
-        _check(t, F16, name, contiguous=False)
-        if t.stride(-1) != 1:
-            raise ValueError(f"{name} must have unit column stride")
-    _check(lengths, I32, "lengths")
-    _check_here(qkv=qkv, kprefix=kprefix, vprefix=vprefix, kcache=kcache, vcache=vcache, lengths=lengths,
-                workspace=workspace, out=out)
-    B = qkv.shape[0]
-    max_len = kcache.shape[1] if max_len is None else max_len
+    if not (_plain(F16, qkv, kprefix, vprefix, kcache, vcache) and _plain(I32, lengths)):
+        for name, t in (("qkv", qkv), ("kprefix", kprefix), ("vprefix", vprefix), ("kcache", kcache), ("vcache", vcache)):
+            _check(t, F16, name, contiguous=False)
+            if t.stride(-1) != 1:
+                raise ValueError(f"{name} must have unit column stride")
+        _check(lengths, I32, "lengths")
+        _check_here(qkv=qkv, kprefix=kprefix, vprefix=vprefix, kcache=kcache, vcache=vcache, lengths=lengths)
+    w = kv * D
+    qs, ps, cs = qkv.stride(), kprefix.stride(), kcache.stride()
+    B, rows = kcache.shape[:2] if kcache.dim() == 3 else (0, 0)
+    if max_len is None:
+        max_len = rows
     _shape(qkv, (B, (H + 2 * kv) * D), "qkv")
     _shape(lengths, (B,), "lengths")
-    _shape(kcache, (B, kcache.shape[1], kv * D), "kcache")
-    if kprefix.dim() != 2 or kprefix.shape[1] != kv * D or not 0 <= prefix_len <= kprefix.shape[0]:
+    _shape(kcache, (B, rows, w), "kcache")
+    if kprefix.dim() != 2 or kprefix.shape[1] != w or not 0 <= prefix_len <= kprefix.shape[0]:
         raise ValueError("attn_decode_prefix: kprefix must be [>= prefix_len, kv_heads*D]")
-    if kprefix.shape != vprefix.shape or kcache.shape != vcache.shape or (
-            kprefix.stride() != vprefix.stride() or kcache.stride() != vcache.stride()):
+    if kprefix.shape != vprefix.shape or kcache.shape != vcache.shape or ps != vprefix.stride() or cs != vcache.stride():
         raise ValueError("attn_decode_prefix: keys and values must share a layout")
-    if not 0 < max_len <= kcache.shape[1]:
+    if not 0 < max_len <= rows:
         raise ValueError("attn_decode_prefix: the caches must hold `max_len` positions")
-    (s0, s1), w = kcache.stride()[:2], kv * D
-    if B > 1 and not (min(s0, s1) >= w and (s0 >= (kcache.shape[1] - 1) * s1 + w or s1 >= (B - 1) * s0 + w)):
+    s0, s1 = cs[:2]
+    if B > 1 and not (min(s0, s1) >= w and (s0 >= (rows - 1) * s1 + w or s1 >= (B - 1) * s0 + w)):
         raise ValueError("attn_decode_prefix: the sequences' caches overlap")
     need = attn_decode_prefix_workspace_bytes(B, H, kv, prefix_len, max_len)
     if workspace is None:
         workspace = torch.empty(need // 4 + 4, device=qkv.device, dtype=F32)
-    elif not workspace.is_contiguous() or workspace.numel() * workspace.element_size() < need:
-        raise ValueError(f"attn_decode_prefix: workspace needs {need} bytes")
+    else:
+        _check_here(workspace=workspace)
+        if not workspace.is_contiguous() or workspace.numel() * workspace.element_size() < need:
+            raise ValueError(f"attn_decode_prefix: workspace needs {need} bytes")
     if out is None:
         out = torch.empty(B, H * D, device=qkv.device, dtype=F16)
     else:
         _check(out, F16, "out", contiguous=False)
+        _check_here(out=out)
         _shape(out, (B, H * D), "out")
-    row = lambda t, i, w: t.stride(i) if t.shape[i] > 1 else w  # noqa: E731  (a single row's stride says nothing)
-    _lib.call("jx_attn_decode_prefix", qkv.data_ptr(), row(qkv, 0, qkv.shape[1]), kprefix.data_ptr(), vprefix.data_ptr(),
-              row(kprefix, 0, kv * D), prefix_len, kcache.data_ptr(), vcache.data_ptr(), row(kcache, 1, kv * D),
-              row(kcache, 0, 0), lengths.data_ptr(), max_len, B, H, kv, D, 1.0 / math.sqrt(D), workspace.data_ptr(),
-              out.data_ptr(), row(out, 0, H * D), _stream())
+        if out.stride(1) != 1:
+            raise ValueError("out must have unit column stride")
+    # A dimension of one row has no stride to speak of.
+    _lib.call("jx_attn_decode_prefix", qkv.data_ptr(), qs[0] if B > 1 else (H + 2 * kv) * D, kprefix.data_ptr(),
+              vprefix.data_ptr(), ps[0] if kprefix.shape[0] > 1 else w, prefix_len, kcache.data_ptr(), vcache.data_ptr(),
+              s1 if rows > 1 else w, s0 if B > 1 else 0, lengths.data_ptr(), max_len, B, H, kv, D, 1.0 / math.sqrt(D),
+              workspace.data_ptr(), out.data_ptr(), out.stride(0) if B > 1 else H * D, _stream())
     return out
 
 
@@ -422,31 +440,34 @@ def sample(logits16: torch.Tensor, uniforms: torch.Tensor, temperature: float | 
     0 is greedy; top_k 0, top_p 1 and min_p 0 are off. Each setting is a number, or a device tensor with one value
     per row (f32; top_k int32). A row with a NaN or without a finite logit gives token -1 and a NaN."""
     rows, vocab, ld = _logit_rows(logits16, "logits16")
+    here = [logits16, uniforms]
     _check(uniforms, F32, "uniforms")
     _shape(uniforms, (rows,), "uniforms")
-    per_row = []
+    args = []
     for name, v, dtype in (("temperature", temperature, F32), ("top_k", top_k, I32), ("top_p", top_p, F32),
                            ("min_p", min_p, F32)):
         if isinstance(v, torch.Tensor):
             _check(v, dtype, name)
             _shape(v, (rows,), name)
-            per_row += [v, 0]
+            here.append(v)
+            args += [v.data_ptr(), 0]
         else:
-            if v != v or (name == "temperature" and v < 0):
+            if v != v or (v < 0 and name == "temperature"):
                 raise ValueError(f"sample: bad {name} {v}")
-            per_row += [None, min(max(int(v), 0), 2**31 - 1) if dtype == I32 else float(v)]
+            args += [None, min(max(int(v), 0), 2**31 - 1) if dtype is I32 else float(v)]
+    for name, given, dtype in (("tokens", tokens, I64), ("logprobs", logprobs, F32)):
+        if given is not None:
+            _check(given, dtype, name)
+            _shape(given, (rows,), name)
+            here.append(given)
+    device = torch._C._cuda_getDevice()
+    if any(t.get_device() != device for t in here):
+        raise ValueError(f"sample: every tensor must be on the current device, cuda:{device}")
     tokens = torch.empty(rows, device=logits16.device, dtype=I64) if tokens is None else tokens
     logprobs = torch.empty(rows, device=logits16.device, dtype=F32) if logprobs is None else logprobs
-    _check(tokens, I64, "tokens")
-    _check(logprobs, F32, "logprobs")
-    _shape(tokens, (rows,), "tokens")
-    _shape(logprobs, (rows,), "logprobs")
-    t, t_s, k, k_s, p, p_s, m, m_s = per_row
-    _check_here(logits16=logits16, uniforms=uniforms, temperature=t, top_k=k, top_p=p, min_p=m, tokens=tokens,
-                logprobs=logprobs)
     if rows:
-        _lib.call("jx_sample", logits16.data_ptr(), rows, vocab, ld, uniforms.data_ptr(), _ptr(t), t_s, _ptr(k), k_s,
-                  _ptr(p), p_s, _ptr(m), m_s, tokens.data_ptr(), logprobs.data_ptr(), _stream())
+        _lib.call("jx_sample", logits16.data_ptr(), rows, vocab, ld, uniforms.data_ptr(), *args, tokens.data_ptr(),
+                  logprobs.data_ptr(), _stream())
     return tokens, logprobs
 
 
@@ -454,13 +475,17 @@ def top_logits(logits16: torch.Tensor, k: int, values: torch.Tensor | None = Non
     """The k largest fp16 logits of each row, largest first, the lower index first among equal ones (NaN last):
     (values f16 [rows, k], ids int64 [rows, k]); k at most min(vocab, 1024)."""
     rows, vocab, ld = _logit_rows(logits16, "logits16")
-    values = torch.empty(rows, k, device=logits16.device, dtype=F16) if values is None else values
-    ids = torch.empty(rows, k, device=logits16.device, dtype=I64) if ids is None else ids
-    _check(values, F16, "values")
-    _check(ids, I64, "ids")
-    _shape(values, (rows, k), "values")
-    _shape(ids, (rows, k), "ids")
     _check_here(logits16=logits16, values=values, ids=ids)
+    if values is None:
+        values = torch.empty(rows, k, device=logits16.device, dtype=F16)
+    else:
+        _check(values, F16, "values")
+        _shape(values, (rows, k), "values")
+    if ids is None:
+        ids = torch.empty(rows, k, device=logits16.device, dtype=I64)
+    else:
+        _check(ids, I64, "ids")
+        _shape(ids, (rows, k), "ids")
     if rows:
         _lib.call("jx_top_logits", logits16.data_ptr(), rows, vocab, ld, k, values.data_ptr(), ids.data_ptr(), _stream())
     return values, ids
@@ -520,7 +545,8 @@ def ce_fwd_parts(parts: torch.Tensor, logits16: torch.Tensor, targets: torch.Ten
 
 def ce_loss(row_loss: torch.Tensor, targets: torch.Tensor, ignore_index: int = -100,
             out: torch.Tensor | None = None, accumulate: bool = False) -> torch.Tensor:
-    out = out if out is not None else torch.zeros(3, device=row_loss.device, dtype=F32)
+    if out is None:  # the kernel writes all three unless it adds to them
+        out = (torch.zeros if accumulate else torch.empty)(3, device=row_loss.device, dtype=F32)
     _lib.call("jx_ce_loss", row_loss.data_ptr(), targets.data_ptr(), ignore_index, row_loss.numel(), out.data_ptr(),
               int(accumulate), _stream())
     return out
@@ -535,18 +561,20 @@ def ce_bwd(logits16, targets, lse, grad_loss: torch.Tensor, count: torch.Tensor,
 # ---------------------------------------------------------------- distillation
 def _teacher(logits16, teacher_ids, teacher_logits, targets):
     rows, vocab, ld = _logit_rows(logits16, "logits16")
-    _check(teacher_ids, I64, "teacher_ids")
     if not isinstance(teacher_logits, torch.Tensor) or teacher_logits.dtype not in (F16, F32):
         raise TypeError("teacher_logits must be a float16 or float32 tensor")
-    _check(teacher_logits, teacher_logits.dtype, "teacher_logits")
-    _check(targets, I64, "targets")
+    if not (_plain(I64, teacher_ids, targets) and _plain(teacher_logits.dtype, teacher_logits)):
+        _check(teacher_ids, I64, "teacher_ids")
+        _check(teacher_logits, teacher_logits.dtype, "teacher_logits")
+        _check(targets, I64, "targets")
+        _check_here(teacher_ids=teacher_ids, teacher_logits=teacher_logits, targets=targets)
     if teacher_ids.dim() != 2:
         raise ValueError("teacher_ids must be [rows, K]")
     K = teacher_ids.shape[1]
     _shape(teacher_ids, (rows, K), "teacher_ids")
     _shape(teacher_logits, (rows, K), "teacher_logits")
     _shape(targets, (rows,), "targets")
-    _check_here(logits16=logits16, teacher_ids=teacher_ids, teacher_logits=teacher_logits, targets=targets)
+    _check_here(logits16=logits16)
     return rows, vocab, ld, K
 
 
@@ -561,12 +589,16 @@ def distill_fwd(logits16: torch.Tensor, teacher_ids: torch.Tensor, teacher_logit
     gemm_f16_ce_parts for these logits saves the pass over them at temperature 1. Returns (stats f32 [3, rows],
     row_loss f32 [rows]); ce_loss(row_loss, targets, ignore_index) is the mean."""
     rows, vocab, ld, K = _teacher(logits16, teacher_ids, teacher_logits, targets)
-    stats = torch.empty(3, rows, device=logits16.device, dtype=F32) if stats is None else stats
-    row_loss = torch.empty(rows, device=logits16.device, dtype=F32) if row_loss is None else row_loss
-    _check(stats, F32, "stats")
-    _check(row_loss, F32, "row_loss")
-    _shape(stats, (3, rows), "stats")
-    _shape(row_loss, (rows,), "row_loss")
+    if stats is None:
+        stats = torch.empty(3, rows, device=logits16.device, dtype=F32)
+    else:
+        _check(stats, F32, "stats")
+        _shape(stats, (3, rows), "stats")
+    if row_loss is None:
+        row_loss = torch.empty(rows, device=logits16.device, dtype=F32)
+    else:
+        _check(row_loss, F32, "row_loss")
+        _shape(row_loss, (rows,), "row_loss")
     if parts is not None:
         _check(parts, F32, "parts")
         if parts.numel() < rows * ce_parts_blocks(vocab) * 2:
@@ -588,13 +620,15 @@ def distill_bwd(logits16: torch.Tensor, teacher_ids: torch.Tensor, teacher_logit
     orows, ovocab, ld_out = _logit_rows(out, "out")
     if (orows, ovocab) != (rows, vocab):
         raise ValueError(f"out must have shape {(rows, vocab)}, got {(orows, ovocab)}")
-    _check(stats, F32, "stats")
+    if not _plain(F32, stats, grad_loss, count):
+        _check(stats, F32, "stats")
+        _check(grad_loss, F32, "grad_loss")
+        _check(count, F32, "count")
+        _check_here(stats=stats, grad_loss=grad_loss, count=count)
     _shape(stats, (3, rows), "stats")
-    _check(grad_loss, F32, "grad_loss")
-    _check(count, F32, "count")
     if grad_loss.numel() != 1 or count.numel() != 1:
         raise ValueError("grad_loss and count must hold one value")
-    _check_here(stats=stats, grad_loss=grad_loss, count=count, out=out)
+    _check_here(out=out)
     _lib.call("jx_distill_bwd", logits16.data_ptr(), rows, vocab, ld, teacher_ids.data_ptr(), teacher_logits.data_ptr(),
               int(teacher_logits.dtype == F16), K, targets.data_ptr(), ignore_index, float(temperature), float(alpha),
               stats.data_ptr(), grad_loss.data_ptr(), count.data_ptr(), out.data_ptr(), ld_out, _stream())
