@@ -82,12 +82,12 @@ _SEQ_TILE = 256
 
 
 def _pad_rows(t: torch.Tensor, fill: int) -> torch.Tensor:
-    """[B, T] integer rows padded on the right to a multiple of the sequence tile with `fill`."""
-    T = t.shape[-1]
+    """[B, T] rows ([B, T, K] too) padded along T to a multiple of the sequence tile with `fill`."""
+    T = t.shape[1]
     Tp = -(-T // _SEQ_TILE) * _SEQ_TILE
     if Tp == T:
         return t
-    out = torch.full((t.shape[0], Tp), fill, dtype=t.dtype, device=t.device)
+    out = torch.full((t.shape[0], Tp, *t.shape[2:]), fill, dtype=t.dtype, device=t.device)
     out[:, :T] = t
     return out
 
@@ -500,6 +500,52 @@ class JishuiForCausalLM(nn.Module):
         ws = self._trunk_fwd(ids, train=False, ce=True)
         return self._ce_forward(ws, tg.reshape(-1), ignore_index)[2].clone()
 
+    def distill_loss(self, inputs: torch.Tensor, targets: torch.Tensor, teacher_ids: torch.Tensor,
+                     teacher_logits: torch.Tensor, temperature: float = 1.0, alpha: float = 1.0,
+                     ignore_index: int = -100) -> torch.Tensor:
+        """Mean over the counted positions of alpha temperature^2 KL(teacher || student) + (1 - alpha) CE(targets):
+        the teacher known by its top logits at every position (teacher_ids int64 [B, T, K], -1 for an unused slot;
+        teacher_logits fp16 or fp32 [B, T, K], as `top_logits` gives them), the student's softmax over the whole
+        vocabulary, both at `temperature`. Positions whose target is ignore_index count for nothing."""
+        if inputs.shape[-1] > self.config.max_position_embeddings:
+            raise ValueError("sequence exceeds configured context length")
+        if targets.shape != inputs.shape:
+            raise ValueError(f"targets {tuple(targets.shape)} and inputs {tuple(inputs.shape)} differ in shape")
+        if teacher_ids.shape != teacher_logits.shape or teacher_ids.dim() != 3 or teacher_ids.shape[:2] != inputs.shape:
+            raise ValueError(f"teacher_ids {tuple(teacher_ids.shape)} and teacher_logits {tuple(teacher_logits.shape)} must "
+                             f"be [{inputs.shape[0]}, {inputs.shape[1]}, K]")
+        ids = _pad_rows(inputs.to(torch.int64).contiguous(), 0)
+        tg = _pad_rows(targets.to(torch.int64).contiguous(), ignore_index).reshape(-1)
+        t_ids = _pad_rows(teacher_ids.to(torch.int64).contiguous(), -1).flatten(0, 1)
+        t_logits = _pad_rows(teacher_logits.detach().contiguous(), 0).flatten(0, 1)
+        args = (tg, t_ids, t_logits, float(temperature), float(alpha), ignore_index)
+        if torch.is_grad_enabled() and self.embed_tokens.weight.requires_grad:
+            return _DistillFn.apply(self, ids, *args, *self.parameters())
+        return self._distill_forward(ids, False, *args)[2][2].clone()
+
+    def _distill_forward(self, ids, train: bool, tg, t_ids, t_logits, temperature, alpha, ignore_index):
+        # The head's block statistics replace the pass over the logits at temperature 1, and the hard targets' part of it
+        # at any other.
+        parts = temperature == 1.0 or alpha < 1.0
+        ws = self._trunk_fwd(ids, train=train, ce=parts)
+        stats, rows = ops.distill_fwd(ws.logits, t_ids, t_logits, tg, temperature=temperature, alpha=alpha,
+                                      ignore_index=ignore_index, parts=ws.ce_parts if parts else None)
+        return ws, stats, ops.ce_loss(rows, tg, ignore_index)
+
+    @torch.no_grad()
+    def top_logits(self, input_ids: torch.Tensor, k: int) -> tuple[torch.Tensor, torch.Tensor]:
+        """The k largest logits at every position, largest first: (values fp16 [B, T, k], ids int64 [B, T, k]), what a
+        student's `distill_loss` takes from its teacher."""
+        T = input_ids.shape[-1]
+        if T > self.config.max_position_embeddings:
+            raise ValueError("sequence exceeds configured context length")
+        if not 1 <= k <= min(self.config.vocab_size, 1024):
+            raise ValueError(f"k must be in [1, min(vocab_size, 1024)], got {k}")
+        ids = _pad_rows(input_ids.to(torch.int64).contiguous(), 0)
+        ws = self._trunk_fwd(ids, train=False)
+        values, top = ops.top_logits(ws.logits, k)
+        return values.view(*ids.shape, k)[:, :T].contiguous(), top.view(*ids.shape, k)[:, :T].contiguous()
+
     def _ce_forward(self, ws: Workspace, tg: torch.Tensor, ignore_index: int) -> torch.Tensor:
         """Loss from the statistics the head left in ws.ce_parts (the trunk ran with ce=True)."""
         ops.ce_fwd_parts(ws.ce_parts, ws.logits, tg, ignore_index, lse=ws.ce_lse, row_loss=ws.row_loss)
@@ -590,6 +636,30 @@ class _LossFn(torch.autograd.Function):
         return (None, None, None, None) + (None,) * (len(ctx.needs_input_grad) - 4)
 
 
+class _DistillFn(torch.autograd.Function):
+    """_LossFn for distill_loss: the logits' gradient is written over them, then every parameter's."""
+
+    @staticmethod
+    def forward(ctx, model: JishuiForCausalLM, ids, tg, t_ids, t_logits, temperature, alpha, ignore_index, *params):
+        ws, stats, out = model._distill_forward(ids, True, tg, t_ids, t_logits, temperature, alpha, ignore_index)
+        model._gen += 1
+        ctx.model, ctx.gen, ctx.ws = model, model._gen, ws
+        ctx.settings = dict(temperature=temperature, alpha=alpha, ignore_index=ignore_index)
+        ctx.save_for_backward(ids, tg, t_ids, t_logits, stats, out)
+        return out[2].clone()
+
+    @staticmethod
+    def backward(ctx, grad_loss):
+        model, ws = ctx.model, ctx.ws
+        if model._gen != ctx.gen:
+            raise RuntimeError("another training forward ran before this backward; activations were overwritten")
+        ids, tg, t_ids, t_logits, stats, out = ctx.saved_tensors
+        g = grad_loss.detach().to(torch.float32).reshape(1).contiguous()
+        ops.distill_bwd(ws.logits, t_ids, t_logits, tg, stats, g, out[1:2], **ctx.settings)
+        model._backward_from_dlogits(ws, ids)
+        return (None,) * len(ctx.needs_input_grad)
+
+
 class _LogitsFn(torch.autograd.Function):
     """forward() under autograd: returns fp16 logits; backward takes dlogits."""
 
@@ -618,3 +688,9 @@ class _LogitsFn(torch.autograd.Function):
 def causal_lm_loss(model: JishuiForCausalLM, inputs: torch.Tensor, targets: torch.Tensor) -> torch.Tensor:
     """Mean next-token cross-entropy (model_torch.py:102-104) through the fused head + CE."""
     return model.loss(inputs, targets)
+
+
+def distillation_loss(model: JishuiForCausalLM, inputs: torch.Tensor, targets: torch.Tensor, teacher_ids: torch.Tensor,
+                      teacher_logits: torch.Tensor, temperature: float = 1.0, alpha: float = 1.0) -> torch.Tensor:
+    """causal_lm_loss's counterpart for a student that learns from a teacher's top logits (model.distill_loss)."""
+    return model.distill_loss(inputs, targets, teacher_ids, teacher_logits, temperature, alpha)

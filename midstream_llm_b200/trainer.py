@@ -24,15 +24,18 @@ from .data import tensor_batch
 from .model import JishuiForCausalLM, causal_lm_loss
 from .optim import AdamW, GradScaler, clip_grad_norm_
 
-Batch = tuple[torch.Tensor, torch.Tensor]
+Batch = tuple[torch.Tensor, ...]
 
 
 def train_update(model: JishuiForCausalLM, optimizer: AdamW, scaler: GradScaler,
                  micro_batches: Callable[[], Sequence[Batch]], grad_accum_steps: int, grad_clip: float, lr: float,
-                 max_attempts: int = 8, on_retry: Callable[[int, float], None] | None = None) -> dict:
+                 max_attempts: int = 8, on_retry: Callable[[int, float], None] | None = None,
+                 loss_fn: Callable[..., torch.Tensor] = causal_lm_loss) -> dict:
     """Runs one update. `micro_batches()` returns this update's micro-batches; it is
     called again on a retry and must replay the same samples (the reference
-    restores its sampler state for that, pretrain_torch.py:204-207)."""
+    restores its sampler state for that, pretrain_torch.py:204-207). `loss_fn(model, *micro_batch)` is
+    the loss of one: inputs and targets for the default, and the teacher's top ids and logits as well for
+    `distillation_loss` (with its settings bound by functools.partial)."""
     for attempt in range(max_attempts):
         optimizer.zero_grad(set_to_none=True)
         total = None
@@ -40,13 +43,13 @@ def train_update(model: JishuiForCausalLM, optimizer: AdamW, scaler: GradScaler,
         if len(batches) != grad_accum_steps:
             raise ValueError(f"expected {grad_accum_steps} micro-batches, got {len(batches)}")
         reducer = model.grad_reducer
-        for i, (x, y) in enumerate(batches):
+        for i, batch in enumerate(batches):
             # Data parallel: only the last micro-step's backward all-reduces the accumulated gradients
             # (the reference's no_sync rule, docs/torch-distributed.md:65); AVG is linear, so the sum of
             # the micro-steps' gradients is averaged across ranks once.
             if reducer is not None:
                 reducer.enabled = i == len(batches) - 1
-            loss = causal_lm_loss(model, x, y)
+            loss = loss_fn(model, *batch)
             total = loss.detach() if total is None else total + loss.detach()
             scaler.scale(loss / grad_accum_steps).backward()
         if reducer is not None:
