@@ -28,6 +28,12 @@ __device__ __forceinline__ uint32_t order_key(uint32_t h) {
   return (h & 0x8000u) ? (~h & 0xffffu) : (h | 0x8000u);
 }
 
+// The same of anything but a NaN.
+__device__ __forceinline__ uint32_t order_key_num(uint32_t h) {
+  h = h == 0x8000u ? 0u : h;
+  return (h ^ ((uint32_t)((int)(h << 16) >> 31) | 0x8000u)) & 0xffffu;
+}
+
 __device__ __forceinline__ uint32_t key_bits(uint32_t key) { return (key & 0x8000u) ? key ^ 0x8000u : ~key & 0xffffu; }
 
 __device__ __forceinline__ __half key_half(uint32_t key) { return __ushort_as_half((unsigned short)key_bits(key)); }
@@ -399,9 +405,9 @@ __global__ void __launch_bounds__(NT, 1024 / NT)
 //   - top-p without top-k: e < (1 - top_p) / V, since all such elements together weigh less than what top-p
 //     drops (the maximum alone weighs 1). That limit is low, so a higher one is tried first, which a part of the row
 //     says leaves three quarters of 1 - top_p below; whether it does is seen from the sums, and if not, the
-//     safe one is taken. What lies below the limit is summed in fp32; the error (about 1e-9 of the total, from
-//     arguments with an exact difference and a two-part 1 / T) only moves the place of the cut, by less than a
-//     thousandth of the tokens' weight there.
+//     safe one is taken. What lies below the limit is summed in fp32, which only moves the place of the cut; where
+//     the cut is nearer to a border between two ranks than that sum's error, the row is taken again with the
+//     safe limit (about one row in a thousand).
 // A histogram of the list's keys gives the threshold: counts alone where a bin is one key (its weight is the
 // count times one exponential), else counts and weights, the latter in four 11-bit limbs, since shared memory adds 32
 // bits at a time. Then the kept weights are summed per 256 list places, and the group where the running sum passes
@@ -410,9 +416,9 @@ __global__ void __launch_bounds__(NT, 1024 / NT)
 constexpr int kFine = 8192;      // bins of one key
 constexpr int kCoarse = 2048;    // bins of several
 constexpr int kGroups = 4096;    // groups of 256 elements of a whole row: vocabularies up to 2^20
-constexpr int kList = 24576;     // list places, over all warps
+constexpr int kList = 32768;     // list places, over all warps
 constexpr double kUnit = 4398046511104.0;  // 2^42: weights of a row of 2^20 elements sum to at most 2^62
-constexpr int kExpTab = 64;
+constexpr int kExpTab = 256;
 constexpr int kGuess = 8;        // limits tried, 2.5 octaves of weight apart
 
 struct SampleParams {
@@ -430,11 +436,11 @@ struct SampleParams {
   float* logp;
 };
 
-// e * 2^42 for x = M + d (see weight()): 2^(j/64) from the table, the rest of the exponent by the Taylor
-// series of 2^(r/64), |r| <= 1/2, to the fourth power (relative error below 4e-14).
+// e * 2^42: 2^(j/256) from the table, the rest of the exponent by the Taylor series of 2^(r/256), |r| <= 1/2, to the
+// third power (relative error below 2e-13). At the maximum the result is 2^42 exactly.
 struct Exp {
   double m;        // the row's maximum
-  double c;        // 64 log2(e) / T
+  double c;        // 256 log2(e) / T
   const double* tab;
 
   // kAny: also for values whose weight rounds to 0, down to -inf.
@@ -442,15 +448,15 @@ struct Exp {
   __device__ __forceinline__ double value(uint32_t h) const {
     // A half's bits moved to a double's places are the value times 2^-1008, subnormals too.
     const double x = __hiloint2double((int)((h & 0x8000u) << 16 | (h & 0x7fffu) << 10), 0);
-    const double y = fma(x, 0x1p1008, -m) * c;  // 64 log2(e_i), exact difference
-    if (kAny && !(y > -64.0 * 60.0)) return 0.0;
+    const double y = fma(x, 0x1p1008, -m) * c;  // 256 log2(e_i), exact difference
+    if (kAny && !(y > -256.0 * 60.0)) return 0.0;
     const double t = y + 0x1.8p52;  // rounds to an integer, which sits in the low word
     const int n = __double2loint(t);
     const double r = y - (t - 0x1.8p52);
-    constexpr double b = 0.010830424696249145;  // ln 2 / 64
-    const double p = fma(r, fma(r, fma(r, fma(r, b * b * b * b / 24.0, b * b * b / 6.0), b * b / 2.0), b), 1.0);
+    constexpr double b = 0.6931471805599453 / 256.0;
+    const double p = fma(r, fma(r, fma(r, b * b * b / 6.0, b * b / 2.0), b), 1.0);
     const double w = tab[n & (kExpTab - 1)];
-    return __hiloint2double(__double2hiint(w) + ((n >> 6) << 20), __double2loint(w)) * p;
+    return __hiloint2double(__double2hiint(w) + ((n >> 8) << 20), __double2loint(w)) * p;
   }
 };
 
@@ -478,7 +484,8 @@ struct SampleShared {
       uint32_t ties[kList / 256];
     } group;
   };
-  uint32_t listed[32];  // entries of each warp's list
+  uint32_t listed[32];            // entries of each warp's list
+  unsigned short upto[32][32];    // of those, how many stand before each 32nd part of the warp's stretch
   uint32_t sub[64];
   double tab[kExpTab];
   u64 red64[32];
@@ -493,9 +500,7 @@ static_assert(2 * (sizeof(SampleShared) + 1024) <= 233472, "two blocks an SM");
 struct Weights {
   Exp ex;
   uint32_t mkey;
-  __device__ __forceinline__ u64 of(uint32_t bits, uint32_t key) const {  // key >= the least lkey
-    return key == mkey ? (u64)kUnit : to_units(ex.value<false>(bits));
-  }
+  __device__ __forceinline__ u64 of(uint32_t bits) const { return to_units(ex.value<false>(bits)); }  // not below the least lkey
 };
 
 // The same as a call, for any key: an infinite maximum leaves every finite logit without weight.
@@ -514,7 +519,9 @@ __global__ void __launch_bounds__(NT, 1024 / NT) sample_kernel(const SampleParam
   const int vocab = a.vocab;
   const int nvec = (vocab + 7) / 8;
   constexpr int kOwn = kList / NW;               // places of a warp's list
+  constexpr int kPer = kOwn / 256;               // groups of it
   const int stretch = (nvec + NW - 1) / NW;      // vectors of a warp's part of the row
+  const int part = (stretch + 1023) / 1024 * 32;  // vectors of a 32nd of it, whole steps
   const int v0 = warp * stretch, v1 = min(v0 + stretch, nvec);
   auto vec = [&](int i) { return load_vec<kFillNegInf>(row, i, vocab); };
   const float Tr = a.temperature ? a.temperature[r] : a.temperature_s;
@@ -536,7 +543,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) sample_kernel(const SampleParam
 
   // The maximum, NaN if one stands in the row.
   __half2 tmax = __half2half2(__ushort_as_half((unsigned short)kFillNegInf));
-#pragma unroll 4
+#pragma unroll 8
   for (int i = tid; i < nvec; i += NT) {
     const Vec v = vec(i);
     const __half2 m = __hmax2_nan(__hmax2_nan(as_half2(v.w[0]), as_half2(v.w[1])),
@@ -576,8 +583,8 @@ __global__ void __launch_bounds__(NT, 1024 / NT) sample_kernel(const SampleParam
     return;
   }
 
-  const Weights wt{{(double)m32, 64.0 * 1.4426950408889634 / (double)T, s.tab}, mkey};
-  const bool minf = mkey == 0xfc00u;
+  const bool minf = mkey == 0xfc00u;  // (Exp sees the bits of an infinity as 65536)
+  const Weights wt{{minf ? 65536.0 : (double)m32, 256.0 * 1.4426950408889634 / (double)T, s.tab}, mkey};
 
   // Elements below `lkey` stay out of the list. First: weights that round to 0.
   auto key_below = [&](float x) {  // key of the largest half <= x, and never that of -inf
@@ -659,7 +666,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) sample_kernel(const SampleParam
 
   uint32_t tau, left;      // the lowest key kept; how many of the elements at it (0xffffffff: all)
   bool lists;              // or the whole row
-  int ngroup;
+  int ngroup, rounds;
   __half2 limit;
   // Group g: up to 256 entries that follow each other in the row.
   auto group = [&](int g, int& count) -> const unsigned short* {
@@ -667,12 +674,13 @@ __global__ void __launch_bounds__(NT, 1024 / NT) sample_kernel(const SampleParam
       count = min(256, vocab - g * 256);
       return reinterpret_cast<const unsigned short*>(row) + g * 256;
     }
-    constexpr int kPer = kOwn / 256;
     count = min(256, (int)s.listed[g / kPer] - g % kPer * 256);
     return s.list + g * 256;
   };
+  // The groups of a warp: with lists, the k-th group of another list for every k, since the last ones are empty.
+  auto group_of = [&](int k) -> int { return lists ? (warp + k) % NW * kPer + k : k * NW + warp; };
   auto key_of = [&](uint32_t bits) -> uint32_t {  // 0 below the limit (a whole row has such entries)
-    const uint32_t key = order_key(bits);
+    const uint32_t key = order_key_num(bits);
     return key >= lkey ? key : 0u;
   };
   for (;;) {  // at most twice
@@ -681,12 +689,23 @@ __global__ void __launch_bounds__(NT, 1024 / NT) sample_kernel(const SampleParam
     const float limit32 = __half2float(key_half(lkey));
     float rest = 0.f;
     uint32_t mine = 0;
-#pragma unroll 2
-    for (int i = v0 + lane; i < v0 + (v1 - v0 + 31 & ~31); i += 32) {
+    int parts = 0, mark = lane == 0 ? v0 : 0x7fffffff;
+    auto own_vec = [&](int i) {
       Vec v;
       v.w[0] = v.w[1] = v.w[2] = v.w[3] = kFillNegInf * 0x10001u;
       if (i < v1) v = vec(i);
+      return v;
+    };
+    // The next two steps' vectors are on their way while one is looked at.
+    Vec v = own_vec(v0 + lane), ahead = own_vec(v0 + lane + 32), after;
+#pragma unroll 1
+    for (int i = v0 + lane; i < v0 + (v1 - v0 + 31 & ~31); i += 32, v = ahead, ahead = after) {
+      after = own_vec(i + 64);
       const uint32_t ge = vec_ge(v, limit);
+      if (i >= mark) {  // lane 0, at the first vector of a part
+        s.upto[warp][parts++] = (unsigned short)min(mine, 0xffffu);
+        mark += part;
+      }
       if (__any_sync(0xffffffffu, ge)) {
         const uint32_t cnt = __popc(ge);
         const uint32_t upto = warp_scan(cnt);
@@ -724,6 +743,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) sample_kernel(const SampleParam
     }
     lists = __reduce_max_sync(0xffffffffu, lane < NW ? s.listed[lane] : 0u) <= kOwn;
     ngroup = lists ? kList / 256 : (vocab + 255) / 256;
+    rounds = (ngroup + NW - 1) / NW;
 
     tau = lkey, left = 0xffffffffu;
     if (!use_k && !use_p) break;
@@ -739,7 +759,9 @@ __global__ void __launch_bounds__(NT, 1024 / NT) sample_kernel(const SampleParam
         s.coarse.limb[0][i] = s.coarse.limb[1][i] = s.coarse.limb[2][i] = s.coarse.limb[3][i] = 0;
     __syncthreads();
 #pragma unroll 1
-    for (int g = warp; g < ngroup; g += NW) {
+    for (int k = 0; k < rounds; ++k) {
+      const int g = group_of(k);
+      if (g >= ngroup) break;
       int count;
       const unsigned short* p = group(g, count);
 #pragma unroll 1
@@ -749,7 +771,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) sample_kernel(const SampleParam
         const uint32_t b = (mkey - key) >> shift;
         atomicAdd(&s.fine[b], 1u);
         if (shift && use_p) {
-          const u64 w = wt.of(bits, key);
+          const u64 w = wt.of(bits);
 #pragma unroll
           for (int l = 0; l < 4; ++l) atomicAdd(&s.coarse.limb[l][b], (uint32_t)(w >> (11 * l)) & 0x7ffu);
         }
@@ -774,7 +796,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) sample_kernel(const SampleParam
         if (shift)
           msum += bin_mass(i);
         else if (s.fine[i])
-          msum += s.fine[i] * wt.of(key_bits(mkey - i), mkey - i);
+          msum += s.fine[i] * wt.of(key_bits(mkey - i));
       }
     }
     const uint32_t cabove = block_scan<NT>(csum, s.red, &ctotal);
@@ -790,7 +812,9 @@ __global__ void __launch_bounds__(NT, 1024 / NT) sample_kernel(const SampleParam
       if (tid < 64) s.sub[tid] = 0;
       __syncthreads();
 #pragma unroll 1
-      for (int g = warp; g < ngroup; g += NW) {
+      for (int k = 0; k < rounds; ++k) {
+      const int g = group_of(k);
+      if (g >= ngroup) break;
         int count;
         const unsigned short* p = group(g, count);
 #pragma unroll 1
@@ -868,10 +892,19 @@ __global__ void __launch_bounds__(NT, 1024 / NT) sample_kernel(const SampleParam
               w = cnt ? weight_of_key(wt, key) : 0ull;
             }
           }
+          const double q = w ? (target - (double)mb) / (double)w : 0.0;
           s.key = key;
-          s.left = w ? (uint32_t)fmin(fmax(ceil((target - (double)mb) / (double)w), 1.0), (double)cnt) : cnt;
+          s.left = w ? (uint32_t)fmin(fmax(ceil(q), 1.0), (double)cnt) : cnt;
+          // Too near to a border for the fp32 sum's error (about 3e-7 of it): once more with the safe limit, below
+          // which lies a few hundredths of that weight.
+          s.bin = lkey > safe && fabs(q - rint(q)) * (double)w <= 3e-7 * (double)tail_mass ? 1u : 0u;
         }
         __syncthreads();
+        if (s.bin) {
+          lkey = safe;
+          __syncthreads();
+          continue;
+        }
         // Never past the top-k threshold.
         if (s.key > tau || (s.key == tau && s.left < left)) {
           tau = s.key;
@@ -892,7 +925,9 @@ __global__ void __launch_bounds__(NT, 1024 / NT) sample_kernel(const SampleParam
   u64* gmass = lists ? s.group.mass : s.row.mass;
   uint32_t* gties = lists ? s.group.ties : s.row.ties;
 #pragma unroll 1
-  for (int g = warp; g < ngroup; g += NW) {
+  for (int k = 0; k < rounds; ++k) {
+      const int g = group_of(k);
+      if (g >= ngroup) break;
     int count;
     const unsigned short* p = group(g, count);
     u64 w = 0;
@@ -903,7 +938,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) sample_kernel(const SampleParam
       if (ties && key == tau)
         ++tie;
       else if (key >= tau)
-        w += wt.of(bits, key);
+        w += wt.of(bits);
     }
     __syncwarp();
     if (count > 0) {
@@ -951,45 +986,65 @@ __global__ void __launch_bounds__(NT, 1024 / NT) sample_kernel(const SampleParam
   g = __shfl_sync(0xffffffffu, g, src);
   wb = __shfl_sync(0xffffffffu, wb, src);
   tb = __shfl_sync(0xffffffffu, tb, src);
-  // Within the group, 32 entries at a time.
+  // Within the group, eight entries a lane.
   int count;
   const unsigned short* p = group(g, count);
-  uint32_t place = 0, tkeyf = mkey;
-#pragma unroll 1
-  for (int j = 0; j < count; j += 32) {
-    const uint32_t bits = j + lane < count ? p[j + lane] : 0u;
-    const uint32_t key = j + lane < count ? key_of(bits) : 0u;
-    const uint32_t tie = __ballot_sync(0xffffffffu, ties && key == tau);
-    const uint32_t t_here = tb + __popc(tie & ((1u << lane) - 1u));
-    const u64 w = ties && key == tau ? (t_here < left ? wtie : 0ull) : key >= tau ? wt.of(bits, key) : 0ull;
-    const u64 inc = wb + warp_scan(w);
-    const uint32_t hit = __ballot_sync(0xffffffffu, target < inc);
-    if (hit) {
-      const int l = __ffs(hit) - 1;
-      place = g * 256 + j + l;
-      tkeyf = __shfl_sync(0xffffffffu, key, l);
-      break;
-    }
-    wb = __shfl_sync(0xffffffffu, inc, 31);
-    tb += __popc(tie);
+  u64 w8[8];
+  uint32_t tie8 = 0, bits8[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const bool in = lane * 8 + j < count;
+    bits8[j] = in ? p[lane * 8 + j] : 0u;
+    const uint32_t key = in ? key_of(bits8[j]) : 0u;
+    const bool tie = ties && key == tau;
+    tie8 |= tie ? 1u << j : 0u;
+    w8[j] = !tie && key >= tau ? wt.of(bits8[j]) : 0ull;
   }
+  tb += warp_scan((uint32_t)__popc(tie8)) - __popc(tie8);
+  wsum = 0;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    if (tie8 >> j & 1) {
+      w8[j] = tb < left ? wtie : 0ull;
+      ++tb;
+    }
+    wsum += w8[j];
+  }
+  wb += warp_scan(wsum) - wsum;
+  uint32_t place = 0, bitsf = 0;  // (of the lane that has it)
+  if (wb <= target && target < wb + wsum) {
+    bool open = true;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      wb += w8[j];
+      if (open && target < wb) {
+        open = false;
+        place = g * 256 + lane * 8 + j + 1;
+        bitsf = bits8[j];
+      }
+    }
+  }
+  place = __reduce_max_sync(0xffffffffu, place) - 1;
+  const uint32_t tkeyf = order_key_num(__reduce_max_sync(0xffffffffu, bitsf));
 
   // The element of that place: in a list, the so-manieth above the limit of its warp's stretch.
   int64_t token = place;
   if (lists) {
     const int w = place / kOwn;
     uint32_t want = place - w * kOwn;
-    const int e1 = min((w + 1) * stretch, nvec);
+    const int e0 = w * stretch, e1 = min(e0 + stretch, nvec);
+    const uint32_t here = e0 + lane * part < e1 ? s.upto[w][lane] : 0xffffffffu;
+    const int at = __popc(__ballot_sync(0xffffffffu, here <= want)) - 1;  // the part that holds it
+    want -= __shfl_sync(0xffffffffu, here, at);
 #pragma unroll 1
-    for (int i = w * stretch + lane;; i += 32) {
+    for (int i = e0 + at * part + lane; i - lane < e1; i += 32) {
       const uint32_t ge = i < e1 ? vec_ge(vec(i), limit) : 0u;
-      const uint32_t cnt = __popc(ge), upto = warp_scan(cnt), here = __shfl_sync(0xffffffffu, upto, 31);
-      if (want >= here) {
-        if (i - lane + 32 >= e1) break;  // (never: the list has that many)
-        want -= here;
+      const uint32_t cnt = __popc(ge), sum = __reduce_add_sync(0xffffffffu, cnt);
+      if (want >= sum) {
+        want -= sum;
         continue;
       }
-      uint32_t before = upto - cnt, found = 0;  // index + 1
+      uint32_t before = warp_scan(cnt) - cnt, found = 0;  // index + 1
 #pragma unroll
       for (int j = 0; j < 8; ++j)
         if (ge & ge_bit(j)) {
