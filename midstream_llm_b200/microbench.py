@@ -1,6 +1,6 @@
 """Operator microbenchmarks of the bandwidth-bound path and the dense kernels.
 
-    python -m midstream_llm_b200.microbench [--op all|rmsnorm|ce|adamw|gemm|attn] [--iters N]
+    python -m midstream_llm_b200.microbench [--op all|rmsnorm|ce|adamw|gemm|attn|eval|decode|generate|distill] [--iters N]
 
 Shapes (the operator workload of the Jishui-200M step):
   rmsnorm  fwd with residual add and bwd with residual gradient on fp16 [16384, 1024];
@@ -16,6 +16,8 @@ Shapes (the operator workload of the Jishui-200M step):
   attn     causal flash attention fwd / bwd at (B 16, T 1024) and (B 4, T 4096), 16 heads x 64
   eval     validation forward (no autograd, fused head + CE) of the 200M model at 16 x 1024
   decode   next-token logits with the KV cache vs re-running the whole context (200M, context ~1000)
+  generate one decode step's attention of sequences on a shared prefix, sampling, and whole completions of one prompt
+  distill  a teacher's top logits, the distillation loss and its logit gradient over 16384 rows of 32000
 Each line is JSON with the time per call (CUDA events, after warm-up, inputs
 larger than L2 unless noted), the achieved rate against the measured peaks and
 the SM clock read just before the timed calls (`sm_mhz`). The B200 is power-capped:
@@ -362,15 +364,76 @@ def bench_decode(iters: int) -> None:
                       "tokens_per_s": 1.0 / tf}), flush=True)
 
 
+def bench_generate(iters: int) -> None:
+    """Attention over a shared prefix against the bytes of prefix and own caches, sampling against the logits' read,
+    and completions per second of the 200M model (16 of a 1024-token prompt)."""
+    from .config import jishui_200m
+    from .decode import PromptSampler
+    from .model import JishuiForCausalLM
+    pk = _peaks()
+    g = torch.Generator(device="cuda").manual_seed(0)
+    r = lambda *s: torch.randn(*s, device="cuda", generator=g).half()  # noqa: E731
+    for B, H, P, S in ((16, 16, 1791, 257), (64, 16, 32749, 1000)):
+        qkv, kp, vp, kc, vc = r(B, 3 * H * 64), r(P, H * 64), r(P, H * 64), r(B, S, H * 64), r(B, S, H * 64)
+        lens = torch.randint(1, S + 1, (B,), device="cuda", generator=g, dtype=torch.int32)
+        ws = torch.empty(ops.attn_decode_prefix_workspace_bytes(B, H, H, P, S) // 4 + 4, device="cuda")
+        out = torch.empty(B, H * 64, device="cuda", dtype=torch.float16)
+        t = _time(lambda: ops.attn_decode_prefix(qkv, kp, vp, P, kc, vc, lens, H, 64, workspace=ws, out=out), iters)
+        _emit(f"attn_decode_prefix {B} sequences, prefix {P}, own 1-{S}, {H} heads", t,
+              256.0 * H * (P + int(lens.sum())), "GB/s", pk["hbm_gbs"])
+    for R, V, kw in ((64, 32000, dict(temperature=0.8, top_k=50, top_p=0.95)), (1024, 32000, dict(top_p=0.95)),
+                     (1024, 32000, {})):
+        x, u = r(R, V) * 2.5, torch.rand(R, device="cuda", generator=g)
+        tok, lp = torch.empty(R, device="cuda", dtype=torch.int64), torch.empty(R, device="cuda")
+        t = _time(lambda: ops.sample(x, u, **kw, tokens=tok, logprobs=lp), iters)
+        _emit(f"sample [{R},{V}] {kw}", t, 2.0 * R * V, "GB/s", pk["hbm_gbs"])
+    cfg = jishui_200m(2048)
+    torch.manual_seed(0)
+    model = JishuiForCausalLM(cfg).cuda()
+    with torch.no_grad():
+        for p in model.parameters():
+            if p.dim() == 2:
+                p.normal_(0.0, 0.02)
+    prompt = torch.randint(3, cfg.vocab_size, (1024,)).tolist()
+    for n in (1, 16, 64):
+        s = PromptSampler(model, n, 128)
+        s.generate(prompt, top_p=0.95)
+        t = _time(lambda: s.generate(prompt, top_p=0.95), 2, warmup=1)
+        print(json.dumps({"op": f"{n} completions of 128 tokens, 1024-token prompt, 200M", "us": t * 1e6,
+                          "tokens_per_s": n * 128 / t}), flush=True)
+
+
+def bench_distill(iters: int) -> None:
+    pk = _peaks()
+    M, V, K = 16384, 32000, 64
+    g = torch.Generator(device="cuda").manual_seed(1)
+    x = torch.randn(M, V, device="cuda", generator=g).half() * 2
+    teacher = torch.randn(M, V, device="cuda", generator=g).half() * 2
+    y = torch.randint(0, V, (M,), device="cuda", generator=g)
+    v, ids = torch.empty(M, K, device="cuda", dtype=torch.float16), torch.empty(M, K, device="cuda", dtype=torch.int64)
+    t = _time(lambda: ops.top_logits(teacher, K, values=v, ids=ids), iters)
+    _emit(f"top_logits [{M},{V}] k {K}", t, 2.0 * M * V + 10.0 * M * K, "GB/s", pk["hbm_gbs"])
+    stats, rows = torch.empty(3, M, device="cuda"), torch.empty(M, device="cuda")
+    grad, count = torch.full((1,), 65536.0, device="cuda"), torch.full((1,), float(M), device="cuda")
+    out = torch.empty_like(x)
+    for tau, alpha in ((1.0, 1.0), (2.0, 0.7), (1.5, 0.7)):
+        kw = dict(temperature=tau, alpha=alpha)
+        t = _time(lambda: ops.distill_fwd(x, ids, v, y, stats=stats, row_loss=rows, **kw), iters)
+        _emit(f"distill_fwd [{M},{V}] K {K} tau {tau} alpha {alpha}", t, 2.0 * M * V + 10.0 * M * K, "GB/s", pk["hbm_gbs"])
+        t = _time(lambda: ops.distill_bwd(x, ids, v, y, stats, grad, count, out=out, **kw), iters)
+        _emit(f"distill_bwd [{M},{V}] K {K} tau {tau} alpha {alpha}", t, 4.0 * M * V + 10.0 * M * K, "GB/s", pk["hbm_gbs"])
+
+
 def main() -> None:
     ap = argparse.ArgumentParser(description=__doc__, formatter_class=argparse.RawDescriptionHelpFormatter)
-    ap.add_argument("--op", default="all", choices=("all", "rmsnorm", "ce", "adamw", "gemm", "attn", "eval", "decode"))
+    ap.add_argument("--op", default="all", choices=("all", "rmsnorm", "ce", "adamw", "gemm", "attn", "eval", "decode", "generate",
+                                                            "distill"))
     ap.add_argument("--iters", type=int, default=10)
     a = ap.parse_args()
     torch.cuda.set_device(0)
     for name, fn in (("rmsnorm", bench_rmsnorm), ("ce", bench_ce), ("adamw", bench_adamw), ("gemm", bench_gemm),
                      ("attn", bench_attn), ("eval", bench_eval),
-                     ("decode", bench_decode)):
+                     ("decode", bench_decode), ("generate", bench_generate), ("distill", bench_distill)):
         if a.op in ("all", name):
             if a.op == "all":
                 torch.cuda.synchronize()
