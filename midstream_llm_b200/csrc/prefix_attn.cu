@@ -19,7 +19,8 @@
 // keys still pays the whole chain from TMA to the output (about 3 us). With up to four heads a key head they are
 // therefore scored by the second kernel, which joins the parts anyway, in plain fp32 arithmetic (one block per
 // sequence and key / value head, many blocks an SM; 64 sequences of 16 heads with a prefix of 128 and one token of their
-// own: 21.5 -> 14.3 us; with 500 own tokens and no prefix 48.6 -> 28.8 us). Larger groups, and few sequences with long own parts, which have to be split, take the matrix way.
+// own: 21.5 -> 14.3 us when this came in). Larger groups, and few sequences with long own parts, which have to be
+// split, take the matrix way.
 //
 // Work of the first kernel: the prefix tiles of all (row tile, key / value head) units stand in one line that is cut
 // into equal runs, one a block, so that each unit is split over a few blocks; the (sequence, head, chunk) items of
@@ -37,6 +38,7 @@
 // the chain scores - exponents - exponentials - product of a tile (about 3300 cycles with two blocks an SM), not by memory.
 #include <algorithm>
 #include <atomic>
+#include <type_traits>
 
 #include "jx_common.cuh"
 #include "jx_host.h"
@@ -54,6 +56,9 @@ constexpr uint32_t kOnes = 2048;          // 16 keys x 64 ones
 constexpr int kKSlots = 2, kVSlots = 3;
 constexpr int kLens = 512;  // lengths kept in shared memory
 constexpr uint32_t kTmemCols = 256;  // S^T [0,64) and [64,128), [O^T; l] [128,192)
+
+constexpr float kNoKey = -1e30f;  // the running maximum before the first key: below every product of fp16 numbers, and
+                                 // a score of -infinity less it is no NaN
 
 enum Status : int { kProducer = 601, kMma = 602, kSoftmax = 603 };
 
@@ -416,7 +421,7 @@ __global__ void __launch_bounds__(kThreads, 2)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   if (threadIdx.x == 32) {
-    tma_prefetch_desc(&tm_qp), tma_prefetch_desc(&tm_kp), tma_prefetch_desc(&tm_vp);
+    if (s.T > 0) tma_prefetch_desc(&tm_qp), tma_prefetch_desc(&tm_kp), tma_prefetch_desc(&tm_vp);
     if (s.chunks > 0) tma_prefetch_desc(&tm_qo), tma_prefetch_desc(&tm_kc), tma_prefetch_desc(&tm_vc);
   }
   if (threadIdx.x == 0) {
@@ -648,15 +653,21 @@ __global__ void __launch_bounds__(128) attn_prefix_join_kernel(const Params p, i
   dst[lane] = __floats2half2_rn(acc.x / L, acc.y / L);
 }
 
-// The same with the own keys: a block per (sequence, key / value head), NT threads. A warp takes 4 U keys at a time, eight
+// The same with the own keys: a block per (sequence, key / value head), NT threads. A warp takes 16 keys at a time, eight
 // lanes to a key (16 bytes each), four keys side by side, and every lane group keeps its own running (m, l, o) of the
-// keys it has seen; the prefix's parts are then added by warps (a lane two columns), and all partial results meet in
-// shared memory. Only the parts wait for the first kernel, so a block begins while that still runs.
-template <int G, int NT, int U>
-__global__ void __launch_bounds__(NT) attn_prefix_own_kernel(const Params p, int* status) {
-  constexpr int NW = NT / 32;
-  __shared__ float so[2 * NW][G][D];
-  __shared__ float sm[2 * NW][G], sl[2 * NW][G];
+// keys it has seen for each of the G heads. The prefix's parts are then added by warps (a head each, a lane two
+// columns), and all partial results meet in shared memory. Only the parts wait for the first kernel, so a block begins
+// while that still runs. Products go two columns at a time (packed fp32), and only a row's last step looks at the
+// length. 64 sequences of up to 1000 own tokens, 16 heads each: 25.5 us, 5.2 TB/s; 96 of 32 query heads on 8 key heads, up to
+// 500 tokens: 17.4 us, bound by the instructions of four heads for each key. (Two heads a warp, which halves the
+// registers, reads and converts every key twice: 20.5 us.)
+template <int G, int NT>
+__global__ void __launch_bounds__(NT, 512 / NT) attn_prefix_own_kernel(const Params p, int* status) {
+  constexpr int U = 4, KW = NT / 32;  // warps that share the keys
+  constexpr int JW = KW / G;          // warps that share a head's parts
+  static_assert(JW >= 1, "");
+  __shared__ float so[KW + JW][G][D];
+  __shared__ float sm[KW + JW][G], sl[KW + JW][G];
   const Sched& s = p.s;
   const int b = blockIdx.x / s.Hkv, h = blockIdx.x - b * s.Hkv;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -674,55 +685,56 @@ __global__ void __launch_bounds__(NT) attn_prefix_own_kernel(const Params p, int
   const __half* nk = row + (s.H + h) * D;
   const __half* nv = nk + s.Hkv * D;
   const int part = (lane & 7) * 8;
-  float q[G][8], m[G], l[G], o[G][8];
+  float2 q[G][4], o[G][4];
+  float m[G], l[G];
 #pragma unroll
   for (int g = 0; g < G; ++g) {
     const uint4 u = *reinterpret_cast<const uint4*>(row + (h * G + g) * D + part);
     const __half2* hq = reinterpret_cast<const __half2*>(&u);
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const float2 f = __half22float2(hq[j]);
-      q[g][2 * j] = f.x * p.scale_log2, q[g][2 * j + 1] = f.y * p.scale_log2;
+      q[g][j] = __fmul2_rn(__half22float2(hq[j]), make_float2(p.scale_log2, p.scale_log2));
+      o[g][j] = make_float2(0.f, 0.f);
     }
-    m[g] = -INFINITY, l[g] = 0.f;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) o[g][j] = 0.f;
+    m[g] = kNoKey, l[g] = 0.f;
   }
-  // The new key and value: appended, and read from their row of qkv below.
+  // The new key and value are appended first and read from there like the others.
   if (threadIdx.x < 16) {
     const int ch = (threadIdx.x & 7) * 8;
     const bool is_v = threadIdx.x >= 8;
     *reinterpret_cast<uint4*>((is_v ? vc : kc) + (int64_t)(len - 1) * p.ld_cache + ch) =
         *reinterpret_cast<const uint4*>((is_v ? nv : nk) + ch);
   }
-  for (int k0 = warp * 4 * U; k0 < len; k0 += NW * 4 * U) {
+  __syncthreads();
+  // The warp's keys: k0 + 4 i + lane / 8.
+  int k0 = warp * 4 * U;
+  const int64_t row4 = 4 * p.ld_cache;
+  const __half* kp = kc + (int64_t)(k0 + (lane >> 3)) * p.ld_cache + part;
+  const __half* vp = vc + (int64_t)(k0 + (lane >> 3)) * p.ld_cache + part;
+  auto step = [&](auto full) {
     uint4 ku[U], vu[U];
 #pragma unroll
     for (int i = 0; i < U; ++i) {
-      const int k = k0 + i * 4 + (lane >> 3);
-      ku[i] = vu[i] = make_uint4(0, 0, 0, 0);
-      if (k < len) {
-        const bool fresh = k == len - 1;
-        ku[i] = *reinterpret_cast<const uint4*>((fresh ? nk : kc + (int64_t)k * p.ld_cache) + part);
-        vu[i] = *reinterpret_cast<const uint4*>((fresh ? nv : vc + (int64_t)k * p.ld_cache) + part);
+      if (full.value || k0 + 4 * i + (lane >> 3) < len) {
+        ku[i] = *reinterpret_cast<const uint4*>(kp + i * row4);
+        vu[i] = *reinterpret_cast<const uint4*>(vp + i * row4);
+      } else {
+        ku[i] = vu[i] = make_uint4(0, 0, 0, 0);
       }
     }
     float sc[G][U];
 #pragma unroll
     for (int i = 0; i < U; ++i) {
       const __half2* hk = reinterpret_cast<const __half2*>(&ku[i]);
-      float f[8];
+      float2 f[4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float2 x = __half22float2(hk[j]);
-        f[2 * j] = x.x, f[2 * j + 1] = x.y;
-      }
+      for (int j = 0; j < 4; ++j) f[j] = __half22float2(hk[j]);
 #pragma unroll
       for (int g = 0; g < G; ++g) {
-        float a = 0.f, c = 0.f;
+        float2 a = __fmul2_rn(q[g][0], f[0]);
 #pragma unroll
-        for (int j = 0; j < 8; j += 2) a = fmaf(q[g][j], f[j], a), c = fmaf(q[g][j + 1], f[j + 1], c);
-        sc[g][i] = a + c;
+        for (int j = 1; j < 4; ++j) a = __ffma2_rn(q[g][j], f[j], a);
+        sc[g][i] = a.x + a.y;
       }
     }
 #pragma unroll
@@ -736,17 +748,19 @@ __global__ void __launch_bounds__(NT) attn_prefix_own_kernel(const Params p, int
       float nm = m[g];
 #pragma unroll
       for (int i = 0; i < U; ++i) {
-        if (k0 + i * 4 + (lane >> 3) >= len) sc[g][i] = -INFINITY;
+        if (!full.value && k0 + i * 4 + (lane >> 3) >= len) sc[g][i] = -INFINITY;
         nm = fmaxf(nm, sc[g][i]);
       }
-      const float a = nm == -INFINITY ? 1.f : ex2(m[g] - nm);  // no key of this lane group yet
-      l[g] *= a;
+      if (__any_sync(0xffffffffu, nm > m[g])) {  // (a step in which no maximum grows rescales nothing)
+        const float a = ex2(m[g] - nm);
+        l[g] *= a;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) o[g][j] *= a;
-      m[g] = nm;
+        for (int j = 0; j < 4; ++j) o[g][j] = __fmul2_rn(o[g][j], make_float2(a, a));
+        m[g] = nm;
+      }
 #pragma unroll
       for (int i = 0; i < U; ++i) {
-        sc[g][i] = nm == -INFINITY ? 0.f : ex2(sc[g][i] - nm);
+        sc[g][i] = ex2(sc[g][i] - m[g]);
         l[g] += sc[g][i];
       }
     }
@@ -757,31 +771,30 @@ __global__ void __launch_bounds__(NT) attn_prefix_own_kernel(const Params p, int
       for (int j = 0; j < 4; ++j) {
         const float2 x = __half22float2(hv[j]);
 #pragma unroll
-        for (int g = 0; g < G; ++g) {
-          o[g][2 * j] = fmaf(sc[g][i], x.x, o[g][2 * j]);
-          o[g][2 * j + 1] = fmaf(sc[g][i], x.y, o[g][2 * j + 1]);
-        }
+        for (int g = 0; g < G; ++g) o[g][j] = __ffma2_rn(make_float2(sc[g][i], sc[g][i]), x, o[g][j]);
       }
     }
-  }
+  };
+  constexpr int kStep = KW * 4 * U;
+  for (; k0 + 4 * U <= len; k0 += kStep, kp += kStep * p.ld_cache, vp += kStep * p.ld_cache) step(std::true_type{});
+  if (k0 < len) step(std::false_type{});
   // The four lane groups of the warp, then the warp's result to shared memory.
 #pragma unroll
   for (int g = 0; g < G; ++g) {
     float wm = fmaxf(m[g], __shfl_xor_sync(0xffffffffu, m[g], 8));
     wm = fmaxf(wm, __shfl_xor_sync(0xffffffffu, wm, 16));
-    const float a = m[g] == -INFINITY ? 0.f : ex2(m[g] - wm);
+    const float a = ex2(m[g] - wm);
     l[g] *= a;
     l[g] += __shfl_xor_sync(0xffffffffu, l[g], 8);
     l[g] += __shfl_xor_sync(0xffffffffu, l[g], 16);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      o[g][j] *= a;
-      o[g][j] += __shfl_xor_sync(0xffffffffu, o[g][j], 8);
-      o[g][j] += __shfl_xor_sync(0xffffffffu, o[g][j], 16);
-    }
-    if (lane < 8) {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) so[warp][g][part + j] = o[g][j];
+    for (int j = 0; j < 4; ++j) {
+      float2 v = __fmul2_rn(o[g][j], make_float2(a, a));
+      v.x += __shfl_xor_sync(0xffffffffu, v.x, 8);
+      v.y += __shfl_xor_sync(0xffffffffu, v.y, 8);
+      v.x += __shfl_xor_sync(0xffffffffu, v.x, 16);
+      v.y += __shfl_xor_sync(0xffffffffu, v.y, 16);
+      if (lane < 8) *reinterpret_cast<float2*>(&so[warp][g][part + 2 * j]) = v;
     }
     if (lane == 0) sm[warp][g] = wm, sl[warp][g] = l[g];
   }
@@ -791,13 +804,13 @@ __global__ void __launch_bounds__(NT) attn_prefix_own_kernel(const Params p, int
     const int unit = b / s.nb * s.Hkv + h;
     npre = s.block_of(unit * s.NT + s.NT - 1) - s.block_of(unit * s.NT) + 1;
   }
-#pragma unroll
-  for (int g = 0; g < G; ++g) {
+  if (warp < JW * G) {
+    const int g = warp % G, j = warp / G;
     const int64_t at = ((int64_t)b * s.H + h * G + g) * s.nparts;
     float M = -INFINITY, L = 0.f;
     float2 acc = make_float2(0.f, 0.f);
 #pragma unroll 4
-    for (int i = warp; i < npre; i += NW) {
+    for (int i = j; i < npre; i += JW) {
       const float2 ml = p.ml[at + i];
       const float2 v = *reinterpret_cast<const float2*>(p.o + (at + i) * D + 2 * lane);
       const float nm = fmaxf(M, ml.x);
@@ -807,18 +820,18 @@ __global__ void __launch_bounds__(NT) attn_prefix_own_kernel(const Params p, int
       acc.y = acc.y * a + v.y * w;
       M = nm;
     }
-    *reinterpret_cast<float2*>(&so[NW + warp][g][2 * lane]) = acc;
-    if (lane == 0) sm[NW + warp][g] = M, sl[NW + warp][g] = L;
+    *reinterpret_cast<float2*>(&so[KW + j][g][2 * lane]) = acc;
+    if (lane == 0) sm[KW + j][g] = M, sl[KW + j][g] = L;
   }
   __syncthreads();
   for (int i = threadIdx.x; i < G * D; i += NT) {
     const int g = i / D, d = i % D;
     float M = -INFINITY;
 #pragma unroll
-    for (int w = 0; w < 2 * NW; ++w) M = fmaxf(M, sm[w][g]);
+    for (int w = 0; w < KW + JW; ++w) M = fmaxf(M, sm[w][g]);
     float L = 0.f, a = 0.f;
 #pragma unroll
-    for (int w = 0; w < 2 * NW; ++w) {
+    for (int w = 0; w < KW + JW; ++w) {
       const float e = sm[w][g] == -INFINITY ? 0.f : ex2(sm[w][g] - M);
       L = fmaf(sl[w][g], e, L);
       a = fmaf(so[w][g][d], e, a);
@@ -899,17 +912,19 @@ extern "C" int jx_attn_decode_prefix(const void* qkv, int64_t ld_qkv, const void
                    (prefix_len == 0 || (ld_prefix % 8 == 0 && ld_prefix >= Hkv * 64)),
                "%s: row strides must be multiples of 8 and hold a row", name);
   // Queries as [sequence][head][64]: one box holds G heads of one sequence, or of a row tile's sequences.
-  CUtensorMap qp, qo, kp, vp, kc, vc;
+  CUtensorMap qp{}, qo{}, kp{}, vp{}, kc{}, vc{};  // those of what there is
   const uint64_t qdims[3] = {64, (uint64_t)H, (uint64_t)B}, qstr[2] = {128, (uint64_t)ld_qkv * 2};
   const uint32_t qob[3] = {64, (uint32_t)G, 1}, qpb[3] = {64, (uint32_t)G, (uint32_t)p.s.nb};
   const uint64_t cdims[3] = {(uint64_t)Hkv * 64, (uint64_t)max_len, (uint64_t)B};
   const uint64_t cstr[2] = {(uint64_t)ld_cache * 2, (uint64_t)(B > 1 ? cache_batch_stride : ld_cache) * 2};
   const uint32_t cbox[3] = {64, 128, 1};
-  bool ok = make_tmap_f16_3d(&qo, qkv, qdims, qstr, qob) && make_tmap_f16_3d(&qp, qkv, qdims, qstr, qpb) &&
-            make_tmap_f16_3d(&kc, kcache, cdims, cstr, cbox) && make_tmap_f16_3d(&vc, vcache, cdims, cstr, cbox);
-  kp = kc, vp = vc;
-  if (ok && prefix_len > 0)
-    ok = make_tmap_f16(&kp, kprefix, (uint64_t)Hkv * 64, prefix_len, ld_prefix, 64, 128) &&
+  bool ok = true;
+  if (p.s.chunks > 0)
+    ok = make_tmap_f16_3d(&qo, qkv, qdims, qstr, qob) && make_tmap_f16_3d(&kc, kcache, cdims, cstr, cbox) &&
+         make_tmap_f16_3d(&vc, vcache, cdims, cstr, cbox);
+  if (ok && p.s.T > 0)
+    ok = make_tmap_f16_3d(&qp, qkv, qdims, qstr, qpb) &&
+         make_tmap_f16(&kp, kprefix, (uint64_t)Hkv * 64, prefix_len, ld_prefix, 64, 128) &&
          make_tmap_f16(&vp, vprefix, (uint64_t)Hkv * 64, prefix_len, ld_prefix, 64, 128);
   JX_CHECK_ARG(ok, "%s: cannot encode a TMA descriptor", name);
   p.qkv = static_cast<const __half*>(qkv);
@@ -959,15 +974,19 @@ extern "C" int jx_attn_decode_prefix(const void* qkv, int64_t ld_qkv, const void
   }
   cfg.dynamicSmemBytes = 0;
   if (p.s.plain) {
-    // Eight warps where one head's sequences may have more than 128 keys of their own, else four; two steps' keys in
-    // flight with several heads, whose state takes the registers.
-    const int NT = G == 1 && max_len > 128 ? 256 : 128;
-    void (*own[4])(const pfx::Params, int*) = {
-        NT == 256 ? pfx::attn_prefix_own_kernel<1, 256, 4> : pfx::attn_prefix_own_kernel<1, 128, 4>,
-        pfx::attn_prefix_own_kernel<2, 128, 2>, pfx::attn_prefix_own_kernel<3, 128, 2>, pfx::attn_prefix_own_kernel<4, 128, 2>};
+    // Eight warps share the keys of a pair where four would make its longest row the end of the kernel: with more than
+    // 512 own keys up to eight pairs an SM (1024 pairs of up to 1000 keys behind a long prefix 77.7 -> 72.1 us; of up
+    // to 200 keys 43.5 -> 46.4), with more than 128 up to two (256 pairs of up to 257 keys 5.1 -> 4.2 us, 768 of up to 500 8.4 -> 9.5).
+    const int wide = max_len > 512 ? 8 : max_len > 128 ? 2 : 0;
+    const int NT = B * Hkv < wide * num_sms() ? 256 : 128;
+    void (*own[2][4])(const pfx::Params, int*) = {
+        {pfx::attn_prefix_own_kernel<1, 128>, pfx::attn_prefix_own_kernel<2, 128>, pfx::attn_prefix_own_kernel<3, 128>,
+         pfx::attn_prefix_own_kernel<4, 128>},
+        {pfx::attn_prefix_own_kernel<1, 256>, pfx::attn_prefix_own_kernel<2, 256>, pfx::attn_prefix_own_kernel<3, 256>,
+         pfx::attn_prefix_own_kernel<4, 256>}};
     cfg.gridDim = dim3(B * Hkv);
     cfg.blockDim = dim3(NT);
-    JX_CUDA_TRY(cudaLaunchKernelEx(&cfg, own[G - 1], p, status), name);
+    JX_CUDA_TRY(cudaLaunchKernelEx(&cfg, own[NT == 256][G - 1], p, status), name);
   } else {
     cfg.gridDim = dim3(B * H);
     cfg.blockDim = dim3(128);
