@@ -34,7 +34,7 @@
 //   warps 2-5 softmax, one key per thread, and the parts' output,
 //   warp 6    issues the second products (with one warp for both, its twelve products a tile, their waits and
 //             commits follow each other: 36.4 against 35.4 us at 64 rows of 32749 keys, 29.4 against 27.6 at one).
-// 64 sequences of 16 heads on a prefix of 32749, 1 to 1000 own tokens: 72 us, 3.7 TB/s; the prefix's tiles are bound by
+// 64 sequences of 16 heads on a prefix of 32749, 1 to 1000 own tokens: 59 us, 4.5 TB/s; the prefix's tiles are bound by
 // the chain scores - exponents - exponentials - product of a tile (about 3300 cycles with two blocks an SM), not by memory.
 #include <algorithm>
 #include <atomic>
@@ -220,6 +220,16 @@ __device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, u
 
 // Until the kernel before this one is done and what it wrote is visible.
 __device__ __forceinline__ void prior_kernel_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
+// 16 bytes to shared memory, of which the first `bytes` are read and the others zero.
+__device__ __forceinline__ void cp_async_16(void* dst, const void* src, uint32_t bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
 
 __device__ __forceinline__ float ex2(float x) {
   float y;
@@ -658,15 +668,21 @@ __global__ void __launch_bounds__(128) attn_prefix_join_kernel(const Params p, i
 // keys it has seen for each of the G heads. The prefix's parts are then added by warps (a head each, a lane two
 // columns), and all partial results meet in shared memory. Only the parts wait for the first kernel, so a block begins
 // while that still runs. Products go two columns at a time (packed fp32), and only a row's last step looks at the
-// length. 64 sequences of up to 1000 own tokens, 16 heads each: 25.5 us, 5.2 TB/s; 96 of 32 query heads on 8 key heads, up to
-// 500 tokens: 17.4 us, bound by the instructions of four heads for each key. (Two heads a warp, which halves the
-// registers, reads and converts every key twice: 20.5 us.)
+// length.
+//
+// What bounds it is how many bytes are on their way: copies go to a ring of two 16-key steps a warp in shared memory
+// (loads straight to registers, a step at a time: 72.2 us for 64 sequences of 16 heads, up to 1000 own keys behind 32749;
+// rings of two, three and four steps 59.0, 59.8 and 73.8, since four leave too few blocks an SM). The own keys' share of
+// that is about 21 us, 6.3 TB/s. With four heads a key head it is bound by their instructions: 96 sequences of 32 heads,
+// up to 500 keys, 18.9 us.
+constexpr int kOwnStages = 2, kOwnStage = 4096;  // bytes of 16 keys and values
+
 template <int G, int NT>
-__global__ void __launch_bounds__(NT, 512 / NT) attn_prefix_own_kernel(const Params p, int* status) {
+__global__ void __launch_bounds__(NT, (G <= 2 ? 640 : G == 3 ? 512 : 384) / NT) attn_prefix_own_kernel(const Params p, int* status) {
   constexpr int U = 4, KW = NT / 32;  // warps that share the keys
   constexpr int JW = KW / G;          // warps that share a head's parts
   static_assert(JW >= 1, "");
-  __shared__ float so[KW + JW][G][D];
+  extern __shared__ __align__(16) uint8_t own_smem[];  // a ring a warp; in the end the partial results
   __shared__ float sm[KW + JW][G], sl[KW + JW][G];
   const Sched& s = p.s;
   const int b = blockIdx.x / s.Hkv, h = blockIdx.x - b * s.Hkv;
@@ -685,6 +701,37 @@ __global__ void __launch_bounds__(NT, 512 / NT) attn_prefix_own_kernel(const Par
   const __half* nk = row + (s.H + h) * D;
   const __half* nv = nk + s.Hkv * D;
   const int part = (lane & 7) * 8;
+  // Steps of the warp: keys k0 + 4 i + lane / 8, fetched kOwnStages ahead. Every lane copies what it reads itself, so nobody
+  // waits for another lane; the new token's row comes from qkv.
+  constexpr int kStep = KW * 4 * U;
+  static_assert(kOwnStage == 2 * U * 512, "");
+  uint8_t* region = own_smem + warp * (kOwnStages * kOwnStage);
+  uint8_t* ring = region + lane * 16;
+  int k0 = warp * 4 * U, kf = k0;
+  const int64_t row4 = 4 * p.ld_cache;
+  const __half* kp = kc + (int64_t)(k0 + (lane >> 3)) * p.ld_cache + part;
+  const __half* vp = vc + (int64_t)(k0 + (lane >> 3)) * p.ld_cache + part;
+  auto fetch = [&](uint8_t* slot) {
+    if (kf + 4 * U < len) {
+#pragma unroll
+      for (int i = 0; i < U; ++i) {
+        cp_async_16(slot + i * 512, kp + i * row4, 16);
+        cp_async_16(slot + (U + i) * 512, vp + i * row4, 16);
+      }
+    } else if (kf < len) {
+#pragma unroll
+      for (int i = 0; i < U; ++i) {
+        const int key = kf + 4 * i + (lane >> 3);
+        const uint32_t bytes = key < len ? 16 : 0;  // zeros behind the end
+        cp_async_16(slot + i * 512, key < len - 1 ? kp + i * row4 : nk + part, bytes);
+        cp_async_16(slot + (U + i) * 512, key < len - 1 ? vp + i * row4 : nv + part, bytes);
+      }
+    }
+    cp_async_commit();
+    kf += kStep, kp += kStep * p.ld_cache, vp += kStep * p.ld_cache;
+  };
+#pragma unroll
+  for (int i = 0; i < kOwnStages; ++i) fetch(ring + i * kOwnStage);
   float2 q[G][4], o[G][4];
   float m[G], l[G];
 #pragma unroll
@@ -698,29 +745,18 @@ __global__ void __launch_bounds__(NT, 512 / NT) attn_prefix_own_kernel(const Par
     }
     m[g] = kNoKey, l[g] = 0.f;
   }
-  // The new key and value are appended first and read from there like the others.
-  if (threadIdx.x < 16) {
+  if (threadIdx.x < 16) {  // the new key and value are appended
     const int ch = (threadIdx.x & 7) * 8;
     const bool is_v = threadIdx.x >= 8;
     *reinterpret_cast<uint4*>((is_v ? vc : kc) + (int64_t)(len - 1) * p.ld_cache + ch) =
         *reinterpret_cast<const uint4*>((is_v ? nv : nk) + ch);
   }
-  __syncthreads();
-  // The warp's keys: k0 + 4 i + lane / 8.
-  int k0 = warp * 4 * U;
-  const int64_t row4 = 4 * p.ld_cache;
-  const __half* kp = kc + (int64_t)(k0 + (lane >> 3)) * p.ld_cache + part;
-  const __half* vp = vc + (int64_t)(k0 + (lane >> 3)) * p.ld_cache + part;
-  auto step = [&](auto full) {
+  auto step = [&](auto full, const uint8_t* slot) {
     uint4 ku[U], vu[U];
 #pragma unroll
     for (int i = 0; i < U; ++i) {
-      if (full.value || k0 + 4 * i + (lane >> 3) < len) {
-        ku[i] = *reinterpret_cast<const uint4*>(kp + i * row4);
-        vu[i] = *reinterpret_cast<const uint4*>(vp + i * row4);
-      } else {
-        ku[i] = vu[i] = make_uint4(0, 0, 0, 0);
-      }
+      ku[i] = *reinterpret_cast<const uint4*>(slot + i * 512);
+      vu[i] = *reinterpret_cast<const uint4*>(slot + (U + i) * 512);
     }
     float sc[G][U];
 #pragma unroll
@@ -775,10 +811,40 @@ __global__ void __launch_bounds__(NT, 512 / NT) attn_prefix_own_kernel(const Par
       }
     }
   };
-  constexpr int kStep = KW * 4 * U;
-  for (; k0 + 4 * U <= len; k0 += kStep, kp += kStep * p.ld_cache, vp += kStep * p.ld_cache) step(std::true_type{});
-  if (k0 < len) step(std::false_type{});
-  // The four lane groups of the warp, then the warp's result to shared memory.
+  uint32_t at_slot = 0;
+  while (k0 < len) {
+    cp_async_wait<kOwnStages - 1>();
+    const uint8_t* slot = ring + at_slot;
+    if (k0 + 4 * U <= len)
+      step(std::true_type{}, slot);
+    else
+      step(std::false_type{}, slot);
+    fetch(ring + at_slot);  // every lane has used what it overwrites
+    at_slot = at_slot == (kOwnStages - 1) * kOwnStage ? 0 : at_slot + kOwnStage;
+    k0 += kStep;
+  }
+  // The prefix's parts: warp j G + g takes parts j, j + JW, .. of head g. The first four are under way while the own keys'
+  // results are brought together.
+  prior_kernel_wait();
+  int npre = 0;
+  if (s.T > 0) {
+    const int unit = b / s.nb * s.Hkv + h;
+    npre = s.block_of(unit * s.NT + s.NT - 1) - s.block_of(unit * s.NT) + 1;
+  }
+  const int part0 = warp < JW * G ? warp / G : npre;
+  const int64_t at = ((int64_t)b * s.H + h * G + warp % G) * s.nparts;
+  float2 ml[4], po[4];
+  auto read_parts = [&](int i0) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const bool is = i0 + i * JW < npre;
+      ml[i] = is ? p.ml[at + i0 + i * JW] : make_float2(-INFINITY, 0.f);
+      po[i] = is ? *reinterpret_cast<const float2*>(p.o + (at + i0 + i * JW) * D + 2 * lane) : make_float2(0.f, 0.f);
+    }
+  };
+  read_parts(part0);
+  // The four lane groups of the warp, then the warp's result to its ring, which nothing is on its way to any more.
+  __syncwarp();
 #pragma unroll
   for (int g = 0; g < G; ++g) {
     float wm = fmaxf(m[g], __shfl_xor_sync(0xffffffffu, m[g], 8));
@@ -794,33 +860,31 @@ __global__ void __launch_bounds__(NT, 512 / NT) attn_prefix_own_kernel(const Par
       v.y += __shfl_xor_sync(0xffffffffu, v.y, 8);
       v.x += __shfl_xor_sync(0xffffffffu, v.x, 16);
       v.y += __shfl_xor_sync(0xffffffffu, v.y, 16);
-      if (lane < 8) *reinterpret_cast<float2*>(&so[warp][g][part + 2 * j]) = v;
+      if (lane < 8) *reinterpret_cast<float2*>(region + (g * D + part + 2 * j) * 4) = v;
     }
     if (lane == 0) sm[warp][g] = wm, sl[warp][g] = l[g];
   }
-  prior_kernel_wait();
-  int npre = 0;
-  if (s.T > 0) {
-    const int unit = b / s.nb * s.Hkv + h;
-    npre = s.block_of(unit * s.NT + s.NT - 1) - s.block_of(unit * s.NT) + 1;
-  }
   if (warp < JW * G) {
     const int g = warp % G, j = warp / G;
-    const int64_t at = ((int64_t)b * s.H + h * G + g) * s.nparts;
-    float M = -INFINITY, L = 0.f;
+    float M = kNoKey, L = 0.f;
     float2 acc = make_float2(0.f, 0.f);
-#pragma unroll 4
-    for (int i = j; i < npre; i += JW) {
-      const float2 ml = p.ml[at + i];
-      const float2 v = *reinterpret_cast<const float2*>(p.o + (at + i) * D + 2 * lane);
-      const float nm = fmaxf(M, ml.x);
-      const float a = M == -INFINITY ? 0.f : ex2(M - nm), w = ex2(ml.x - nm);
-      L = L * a + ml.y * w;
-      acc.x = acc.x * a + v.x * w;
-      acc.y = acc.y * a + v.y * w;
+    for (int i0 = part0;;) {
+      float nm = M;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) nm = fmaxf(nm, ml[i].x);
+      const float a = ex2(M - nm);
+      L *= a, acc = __fmul2_rn(acc, make_float2(a, a));
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float w = ex2(ml[i].x - nm);
+        L = fmaf(ml[i].y, w, L);
+        acc = __ffma2_rn(make_float2(w, w), po[i], acc);
+      }
       M = nm;
+      if ((i0 += 4 * JW) >= npre) break;
+      read_parts(i0);
     }
-    *reinterpret_cast<float2*>(&so[KW + j][g][2 * lane]) = acc;
+    *reinterpret_cast<float2*>(region + (G * D + 2 * lane) * 4) = acc;
     if (lane == 0) sm[KW + j][g] = M, sl[KW + j][g] = L;
   }
   __syncthreads();
@@ -834,7 +898,8 @@ __global__ void __launch_bounds__(NT, 512 / NT) attn_prefix_own_kernel(const Par
     for (int w = 0; w < KW + JW; ++w) {
       const float e = sm[w][g] == -INFINITY ? 0.f : ex2(sm[w][g] - M);
       L = fmaf(sl[w][g], e, L);
-      a = fmaf(so[w][g][d], e, a);
+      const int from = w < KW ? w : (w - KW) * G + g, at = w < KW ? i : G * D + d;
+      a = fmaf(reinterpret_cast<const float*>(own_smem + from * (kOwnStages * kOwnStage))[at], e, a);
     }
     dst[i] = __float2half_rn(a / L);
   }
@@ -946,13 +1011,20 @@ extern "C" int jx_attn_decode_prefix(const void* qkv, int64_t ld_qkv, const void
   static_assert(kFixed + 2 * 1024 + 1024 <= 233472 / 2, "two blocks an SM with up to eight heads a key / value head");
   const size_t smem = kFixed + 2 * p.q_own_stride;
   static std::atomic<uint64_t> done{0};
-  JX_CUDA_TRY(once_per_device(done,
-                              [] {
-                                return cudaFuncSetAttribute(pfx::attn_prefix_part_kernel,
-                                                            cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                                            (int)(kFixed + 2 * pfx::kQTile));
-                              }),
-              name);
+  static void (*const own[2][4])(const pfx::Params, int*) = {
+      {pfx::attn_prefix_own_kernel<1, 128>, pfx::attn_prefix_own_kernel<2, 128>, pfx::attn_prefix_own_kernel<3, 128>,
+       pfx::attn_prefix_own_kernel<4, 128>},
+      {pfx::attn_prefix_own_kernel<1, 256>, pfx::attn_prefix_own_kernel<2, 256>, pfx::attn_prefix_own_kernel<3, 256>,
+       pfx::attn_prefix_own_kernel<4, 256>}};
+  auto set_up = [] {
+    cudaError_t e = cudaFuncSetAttribute(pfx::attn_prefix_part_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                         (int)(kFixed + 2 * pfx::kQTile));
+    for (int i = 0; e == cudaSuccess && i < 8; ++i)
+      e = cudaFuncSetAttribute(own[i / 4][i % 4], cudaFuncAttributeMaxDynamicSharedMemorySize,
+                               (i < 4 ? 4 : 8) * pfx::kOwnStages * pfx::kOwnStage);
+    return e;
+  };
+  JX_CUDA_TRY(once_per_device(done, set_up), name);
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   int* status = status_ptr();
   // Both kernels may be set up while the one before them finishes; they wait before they read what it wrote.
@@ -974,18 +1046,12 @@ extern "C" int jx_attn_decode_prefix(const void* qkv, int64_t ld_qkv, const void
   }
   cfg.dynamicSmemBytes = 0;
   if (p.s.plain) {
-    // Eight warps share the keys of a pair where four would make its longest row the end of the kernel: with more than
-    // 512 own keys up to eight pairs an SM (1024 pairs of up to 1000 keys behind a long prefix 77.7 -> 72.1 us; of up
-    // to 200 keys 43.5 -> 46.4), with more than 128 up to two (256 pairs of up to 257 keys 5.1 -> 4.2 us, 768 of up to 500 8.4 -> 9.5).
-    const int wide = max_len > 512 ? 8 : max_len > 128 ? 2 : 0;
-    const int NT = B * Hkv < wide * num_sms() ? 256 : 128;
-    void (*own[2][4])(const pfx::Params, int*) = {
-        {pfx::attn_prefix_own_kernel<1, 128>, pfx::attn_prefix_own_kernel<2, 128>, pfx::attn_prefix_own_kernel<3, 128>,
-         pfx::attn_prefix_own_kernel<4, 128>},
-        {pfx::attn_prefix_own_kernel<1, 256>, pfx::attn_prefix_own_kernel<2, 256>, pfx::attn_prefix_own_kernel<3, 256>,
-         pfx::attn_prefix_own_kernel<4, 256>}};
+    // Eight warps share the keys of a pair where four would leave SMs empty (256 pairs of up to 257 keys behind 1791:
+    // 12.1 -> 11.1 us; 1024 pairs of up to 1000 58.8 -> 59.8).
+    const int NT = max_len > 128 && B * Hkv < 2 * num_sms() ? 256 : 128;
     cfg.gridDim = dim3(B * Hkv);
     cfg.blockDim = dim3(NT);
+    cfg.dynamicSmemBytes = NT / 32 * pfx::kOwnStages * pfx::kOwnStage;
     JX_CUDA_TRY(cudaLaunchKernelEx(&cfg, own[NT == 256][G - 1], p, status), name);
   } else {
     cfg.gridDim = dim3(B * H);
