@@ -86,6 +86,36 @@ def test_prefix_attention(ops, B, H, kv, P, lens):
         assert torch.equal(t.view(torch.int16), u.view(torch.int16))
 
 
+@pytest.mark.parametrize("kv,P,S", [(8, 0, 512), (8, 40, 130), (1, 0, 512), (1, 300, 257)])
+@pytest.mark.parametrize("G", [1, 2, 3, 4])
+def test_prefix_attention_own_keys(ops, G, kv, P, S):
+    """Own keys up to every border of the steps they are read in, with few and with many (sequence, head) pairs."""
+    lens = [0, 1, 15, 16, 17, 31, 33, 48, 63, 64, 65, 80, 96, 112, 127, 128, 129, 130]
+    lens += [n for n in (143, 144, 145, 192, 255, 256, 257, 384, 500, 511, 512) if n <= S]
+    lens = lens * (2 if kv > 1 else 1)
+    st = _prefix_state(len(lens), G * kv, kv, P, S, lens, seed=G + P)
+    out = ops.attn_decode_prefix(*st[:3], P, *st[3:], G * kv, 64, kv_heads=kv, max_len=S)
+    _prefix_check(out, *st[:5], P, lens, G * kv, kv)
+
+
+@pytest.mark.parametrize("H,kv", [(2, 2), (8, 1)])
+def test_prefix_attention_scores_of_minus_infinity(ops, H, kv):
+    """Keys with an infinite score below weigh nothing, a whole tile of them included; with such keys alone the result is
+    NaN, as the formula's."""
+    P, S, lens = 300, 200, [1, 40, 200, 3]
+    qkv, kp, vp, kc, vc, n = _prefix_state(4, H, kv, P, S, lens, seed=9)
+    q = qkv[:, :H * 64].view(4, H, 64)
+    q[:, :, 0] = q[:, :, 0].abs() + 0.5
+    kp.view(-1, kv, 64)[:256, :, 0] = -INF
+    kc[1:, :2].view(3, 2, kv, 64)[:, :, :, 0] = -INF  # (the first sequence has no keys before its new one)
+    out = ops.attn_decode_prefix(qkv, kp, vp, P, kc, vc, n, H, 64, kv_heads=kv, max_len=S)
+    _prefix_check(out, qkv, kp, vp, kc, vc, P, lens, H, kv)
+    kp.view(-1, kv, 64)[:, :, 0] = -INF
+    qkv[:, H * 64:(H + kv) * 64].view(4, kv, 64)[:, :, 0] = -INF
+    out = ops.attn_decode_prefix(qkv, kp, vp, P, kc, vc, n, H, 64, kv_heads=kv, max_len=S)
+    assert bool(out[0].isnan().all())
+
+
 def test_prefix_attention_views_and_repeats(ops):
     """Keys and values as columns of one fused buffer, padded rows of the queries and the output, the caches'
     sequences in another order than their rows; the same call twice gives the same bits."""
