@@ -469,7 +469,7 @@ __global__ void __launch_bounds__(kThreads, 2)
       // K and V take turns as their slots come free: V's are held longer, and K must not wait behind them.
       bool more_k = c.advance(s, lens), more_v = more_k;
       Cursor v = c;
-      uint32_t nk = 0, nv = 0;
+      uint32_t nk = 0, nv = 0, filled = 0;  // filled: bit q, Q slot q was; bit 8 + q, an odd number of times
       long long since = clock64();
       while (more_k || more_v) {
         bool idle = true;
@@ -479,6 +479,7 @@ __global__ void __launch_bounds__(kThreads, 2)
           const uint32_t use = c.is_own ? (uint32_t)(c.iown >> 1) : (uint32_t)c.ipre;
           if (c.j > 0 || mbar_test_wait(&bars->q_empty[q], (use & 1) ^ 1)) {
             if (c.j == 0) {
+              filled = (filled | 1u << q) ^ 256u << q;
               mbar_expect_tx(&bars->q_full[q], c.is_own ? p.q_own_bytes : p.q_pre_bytes);
               tma_load_3d(q == 2 ? sQp : sQ + q * p.q_own_stride, c.is_own ? &tm_qo : &tm_qp, &bars->q_full[q], 0, c.h * s.G,
                           c.b);
@@ -512,6 +513,15 @@ __global__ void __launch_bounds__(kThreads, 2)
           if (status) atomicExch(status, kProducer);
           break;
         }
+      }
+      if (*abort_flag) {  // a wait somewhere ran out: the copies under way come in before the block ends
+        auto drain = [&](uint64_t* bar, uint32_t fills) {
+          for (int i = 0; fills > 0 && i < (1 << 16) && !mbar_test_wait(bar, (fills - 1) & 1); ++i) __nanosleep(100);
+        };
+        for (int i = 0; i < 3; ++i) drain(&bars->q_full[i], filled >> i & 1 ? 2 - (filled >> (8 + i) & 1) : 0);
+        for (uint32_t i = 0; i < kKSlots; ++i) drain(&bars->k_full[i], (nk + kKSlots - 1 - i) / kKSlots);
+        for (uint32_t i = 0; i < kVSlots; ++i) drain(&bars->v_full[i], (nv + kVSlots - 1 - i) / kVSlots);
+        __nanosleep(1 << 19);  // and the products
       }
     }
     __syncwarp();

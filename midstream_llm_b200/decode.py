@@ -253,7 +253,10 @@ class PromptSampler:
         else:
             self.uniforms.uniform_(generator=generator)
         for (name, buf), v in zip(self.settings.items(), (temperature, top_k, top_p, min_p)):
-            buf.copy_(torch.as_tensor(v, dtype=buf.dtype).expand(self.n))
+            given = torch.as_tensor(v, dtype=buf.dtype)
+            if bool((given != given).any()) or (name == "temperature" and bool((given < 0).any())):
+                raise ValueError(f"bad {name} {v}")
+            buf.copy_(given.expand(self.n))
         self._start(ctx, -1 if eos_token_id is None else int(eos_token_id))
         self._draw()
         taken = 1

@@ -199,3 +199,11 @@ def test_distill_loss_refusals():
         mine.top_logits(x, 0)
     with pytest.raises(ValueError, match="context"):
         mine.top_logits(torch.zeros(1, 2000, device="cuda", dtype=torch.long), 4)
+
+
+def test_generate_refuses_settings_without_a_meaning():
+    from midstream_llm_b200 import generate
+    _, mine = _pairs()
+    for bad in (dict(temperature=-1.0), dict(temperature=[1.0, -0.5]), dict(top_p=float("nan")), dict(min_p=[0.0, float("nan")])):
+        with pytest.raises(ValueError, match="bad"):
+            generate(mine, [1, 2, 3], n=2, max_new_tokens=4, **bad)
