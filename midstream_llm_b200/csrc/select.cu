@@ -10,6 +10,7 @@
 // every value above one threshold key and the first few (by index) of the values at it.
 #include <cuda_fp16.h>
 
+#include <algorithm>
 #include <atomic>
 
 #include "jx_common.cuh"
@@ -148,15 +149,17 @@ __device__ __forceinline__ T block_scan(T v, T* red, T* total) {
 // Top logits: the k largest of a row in rank order.
 //
 // One block per row with the row in registers (rows longer than NT * 8 * VPT elements are read again for the
-// second pass). The k-th largest of the threads' maxima is a limit that at least k elements pass, and in general few
-// more: a histogram of the maxima, in bins of 16 keys down from the largest, gives it to within a bin. The few vectors that
+// later passes). The k-th largest of the threads' maxima is a limit that at least k elements pass, and in general few
+// more: a histogram of the maxima, in bins of 16 keys down from the largest, gives it to within a bin. Where k is large
+// against the threads the maxima of the 8-element vectors take their place. The few vectors that
 // hold such elements go to shared memory, their elements above the limit are collected, ranked among themselves by
-// counting and written. A row where too many pass (many equal values) or k is large against the threads takes
+// counting and written. A row where too many pass (many equal values) or k is large against the vectors takes
 // the exact way: two histograms of all keys find the threshold, values at it are taken in index order.
+// 16384 rows of 32000, top 64: 235 us, 4.5 TB/s; what follows the loads costs with k (4096 rows, top 16 51.7 us, 64 63.6,
+// 256 143), since the ranking's compares grow with its square.
 // ---------------------------------------------------------------------------------------------------------
 constexpr int kBins = 2048;     // upper 11 bits of a key
 constexpr int kCand = 2048;     // candidates a block can hold
-constexpr int kVecs = 512;      // vectors with candidates
 constexpr int kMaxTop = 1024;
 
 // With hist[bin] counting keys, finds the bin (from the top) in which the k-th key falls and how many keys lie
@@ -235,24 +238,34 @@ __device__ __noinline__ void exact_candidates(const unsigned short* row, int voc
   __syncthreads();
 }
 
-template <int NT, int VPT, typename C>
+template <int NT, typename C, bool kLarge>
+struct TopShared {
+  static constexpr int kOwn = kLarge ? 128 : 32;  // vectors with candidates that a warp can hold
+  union {
+    struct {
+      uint4 v[NT / 32 * kOwn];
+      int index[NT / 32 * kOwn];
+    } vec;
+    uint32_t hist[kBins];
+  };
+  __align__(16) C cand[kCand];
+  uint32_t red[32];
+  int found[2];
+  uint32_t ncand;
+};
+
+template <int NT, int VPT, typename C, bool kLarge>
 __global__ void __launch_bounds__(NT, 1024 / NT)
     top_logits_kernel(const __half* __restrict__ logits, int64_t ld, int vocab, int k, __half* __restrict__ values,
                       int64_t* __restrict__ ids) {
-  constexpr int NW = NT / 32;
   typedef CandidateOf<C> Cand;
-  constexpr int kOwn = kVecs / NW;  // vectors a warp can hold
-  __shared__ union {
-    struct {
-      uint4 v[kVecs];
-      int index[kVecs];
-    } vec;
-    uint32_t hist[kBins];
-  } s;
-  __shared__ __align__(16) C cand[kCand];
-  __shared__ uint32_t red[32];
-  __shared__ int found[2];
-  __shared__ uint32_t ncand;
+  constexpr int kOwn = TopShared<NT, C, kLarge>::kOwn;
+  extern __shared__ __align__(16) uint8_t smem_raw[];
+  TopShared<NT, C, kLarge>& s = *reinterpret_cast<TopShared<NT, C, kLarge>*>(smem_raw);
+  C* cand = s.cand;
+  uint32_t* red = s.red;
+  int* found = s.found;
+  uint32_t& ncand = s.ncand;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const __half* row = logits + (int64_t)blockIdx.x * ld;
   const int nvec = (vocab + 7) / 8;
@@ -260,20 +273,34 @@ __global__ void __launch_bounds__(NT, 1024 / NT)
 
   Vec v[VPT];
   __half2 tmax = __half2half2(__ushort_as_half(0xffffu));
-  for (int c = 0; c < nchunk; ++c) {
+  auto load = [&](int c) {
 #pragma unroll
     for (int i = 0; i < VPT; ++i) v[i] = load_vec<kFillNan>(row, (c * VPT + i) * NT + tid, vocab);
+  };
+  for (int c = 0; c < nchunk; ++c) {
+    load(c);
 #pragma unroll
     for (int i = 0; i < VPT; ++i) tmax = __hmax2(tmax, vec_max2(v[i]));
   }
   // The limit.
   constexpr int kTopBins = 1024;
-  const uint32_t tkey = order_key(__half_as_ushort(max_of(tmax)));
-  for (int i = tid; i < kTopBins; i += NT) s.hist[i] = 0;
+  const bool by_vector = kLarge && k <= nvec / 2;
+  for (int i = tid; i < (by_vector ? kBins : kTopBins); i += NT) s.hist[i] = 0;
   if (tid == 0) ncand = 0;
+  const uint32_t tkey = order_key(__half_as_ushort(max_of(tmax)));
   const uint32_t mkey = block_max<NT>(tkey, red);
   uint32_t lkey = 0;
-  if (k <= min(nvec, NT)) {
+  if (by_vector) {
+    for (int c = 0; c < nchunk; ++c) {
+      if (nchunk > 1) load(c);
+#pragma unroll
+      for (int i = 0; i < VPT; ++i)
+        if ((c * VPT + i) * NT + tid < nvec) atomicAdd(&s.hist[order_key(__half_as_ushort(max_of(vec_max2(v[i])))) >> 5], 1u);
+    }
+    __syncthreads();
+    find_bin<NT>(s.hist, (uint32_t)k, red, found);
+    if (found[0] > 0) lkey = (uint32_t)found[0] << 5;
+  } else if (k <= min(nvec, NT)) {
     const uint32_t d = (mkey - tkey) >> 4;
     if (tkey && d < kTopBins) atomicAdd(&s.hist[kTopBins - 1 - d], 1u);
     __syncthreads();
@@ -292,10 +319,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT)
     const uint32_t below = (1u << lane) - 1u;
     uint32_t nv = 0;
     for (int c = 0; c < nchunk; ++c) {
-      if (nchunk > 1) {
-#pragma unroll
-        for (int i = 0; i < VPT; ++i) v[i] = load_vec<kFillNan>(row, (c * VPT + i) * NT + tid, vocab);
-      }
+      if (nchunk > 1) load(c);
 #pragma unroll
       for (int i = 0; i < VPT; ++i) {
         const int at = (c * VPT + i) * NT + tid;
@@ -345,16 +369,18 @@ __global__ void __launch_bounds__(NT, 1024 / NT)
     iout[rank] = (int64_t)Cand::index(c);
   };
   // Padded with zeros (which no candidate is), to the vectors of the count or the power of two of the sort.
+  constexpr uint32_t kCount = 1024;
   uint32_t size = (n + 3) & ~3u;
-  if (n > 256)
-    for (size = 512; size < n;) size <<= 1;
+  if (n > kCount)
+    for (size = 2 * kCount; size < n;) size <<= 1;
   if (n + tid < size) cand[n + tid] = 0;
   for (uint32_t i = n + tid + NT; i < size; i += NT) cand[i] = 0;
   __syncthreads();
-  if (n <= 256) {
-    // Few: the rank of each is the number of larger ones (no two are equal: the index is part of them).
-    if (tid < (int)n) {
-      const C mine = cand[tid];
+  if (n <= kCount) {
+    // The rank of each is the number of larger ones (no two are equal: the index is part of them).
+#pragma unroll 1
+    for (uint32_t i = tid; i < n; i += NT) {
+      const C mine = cand[i];
       uint32_t rank = 0;
       constexpr int kPer = 16 / sizeof(C);
       for (uint32_t j = 0; j < size; j += kPer) {
@@ -1064,6 +1090,29 @@ __global__ void __launch_bounds__(NT, 1024 / NT) sample_kernel(const SampleParam
   }
 }
 
+template <int NT, typename C, bool kLarge>
+int launch_top_as(const __half* x, int64_t rows, int64_t ld, int vocab, int k, __half* values, int64_t* ids, cudaStream_t s) {
+  static std::atomic<uint64_t> done{0};
+  JX_CUDA_TRY(once_per_device(done,
+                              [] {
+                                return cudaFuncSetAttribute(top_logits_kernel<NT, 8, C, kLarge>,
+                                                            cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                            (int)sizeof(TopShared<NT, C, kLarge>));
+                              }),
+              "jx_top_logits: shared memory");
+  top_logits_kernel<NT, 8, C, kLarge><<<(unsigned)rows, NT, sizeof(TopShared<NT, C, kLarge>), s>>>(x, ld, vocab, k, values, ids);
+  JX_CHECK_LAUNCH("jx_top_logits");
+  return JX_OK;
+}
+
+// A limit from the threads' maxima lets few elements more than k pass while k is small against the threads; from there
+// on the vectors' maxima give it (4096 rows of 32000: top 160 95 us by threads, 105 by vectors; top 256 330 and 138).
+template <int NT, typename C>
+int launch_top(const __half* x, int64_t rows, int64_t ld, int vocab, int k, __half* values, int64_t* ids, cudaStream_t s) {
+  return k > std::min((vocab + 7) / 8, NT) * 3 / 8 ? launch_top_as<NT, C, true>(x, rows, ld, vocab, k, values, ids, s)
+                                                   : launch_top_as<NT, C, false>(x, rows, ld, vocab, k, values, ids, s);
+}
+
 template <int NT>
 int launch_sample(const SampleParams& p, int64_t rows, cudaStream_t s) {
   static std::atomic<uint64_t> done{0};
@@ -1093,12 +1142,12 @@ extern "C" int jx_top_logits(const void* logits16, int64_t rows, int vocab, int6
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   const __half* x = static_cast<const __half*>(logits16);
   __half* v = static_cast<__half*>(values16);
-  if (vocab <= 65536)
-    sel::top_logits_kernel<512, 8, uint32_t><<<(unsigned)rows, 512, 0, s>>>(x, ld, vocab, k, v, ids);
-  else
-    sel::top_logits_kernel<512, 8, sel::u64><<<(unsigned)rows, 512, 0, s>>>(x, ld, vocab, k, v, ids);
-  JX_CHECK_LAUNCH("jx_top_logits");
-  return JX_OK;
+  // Threads by the row's length, so that their registers hold it and short rows do not leave most of them idle (4096
+  // rows of 8000 with 512 threads each 60.8 us for the top 100, with 128 35.5 us).
+  if (vocab <= 128 * 64) return sel::launch_top<128, uint32_t>(x, rows, ld, vocab, k, v, ids, s);
+  if (vocab <= 256 * 64) return sel::launch_top<256, uint32_t>(x, rows, ld, vocab, k, v, ids, s);
+  if (vocab <= 65536) return sel::launch_top<512, uint32_t>(x, rows, ld, vocab, k, v, ids, s);
+  return sel::launch_top<512, sel::u64>(x, rows, ld, vocab, k, v, ids, s);
 }
 
 extern "C" int jx_sample(const void* logits16, int64_t rows, int vocab, int64_t ld, const float* uniforms,

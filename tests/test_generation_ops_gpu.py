@@ -372,6 +372,19 @@ def _top(x, k):
                                  (32000, 64), (32000, 128), (32000, 129), (32000, 1000), (40001, 64), (100_000, 700)])
 @pytest.mark.parametrize("kind", ["model", "ties", "equal", "nan", "rising"])
 def test_top_logits(ops, V, k, kind):
+    _top_logits_case(ops, V, k, kind)
+
+
+# A limit by threads and by vectors (above 3/8 of the threads), blocks of 128, 256 and 512 threads, rows that need a second
+# reading, and k past half of the vectors.
+@pytest.mark.parametrize("V,k", [(8000, 48), (8000, 49), (8192, 500), (8192, 513), (8193, 96), (16384, 97), (16377, 1024),
+                                 (16385, 192), (32768, 193), (32000, 256), (32776, 400), (65536, 1024), (65537, 193)])
+@pytest.mark.parametrize("kind", ["model", "ties", "equal", "nan", "rising"])
+def test_top_logits_limits(ops, V, k, kind):
+    _top_logits_case(ops, V, k, kind)
+
+
+def _top_logits_case(ops, V, k, kind):
     R = 3
     x = torch.randn(R, (V + 7) // 8 * 8, device="cuda", generator=_gen(V + k)) * 3
     if kind == "ties":
