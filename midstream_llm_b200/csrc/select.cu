@@ -439,10 +439,8 @@ __global__ void __launch_bounds__(NT, 1024 / NT)
 // bits at a time. Then the kept weights are summed per 256 list places, and the group where the running sum passes
 // its target is walked by one warp. Lists that do not fit are replaced by the whole row. All of this runs
 // once a row, mostly as cold code, so it is written in loops rather than unrolled.
-constexpr int kFine = 8192;      // bins of one key
-constexpr int kCoarse = 2048;    // bins of several
 constexpr int kGroups = 4096;    // groups of 256 elements of a whole row: vocabularies up to 2^20
-constexpr int kList = 32768;     // list places, over all warps
+constexpr int kShort = 8192;     // rows up to here get small blocks, whose lists always hold them
 constexpr double kUnit = 4398046511104.0;  // 2^42: weights of a row of 2^20 elements sum to at most 2^62
 constexpr int kExpTab = 256;
 constexpr int kGuess = 8;        // limits tried, 2.5 octaves of weight apart
@@ -491,7 +489,12 @@ __device__ __forceinline__ u64 to_units(double v) {
   return (u64)__double_as_longlong(v + 0x1p52) & 0xfffffffffffffull;
 }
 
+template <int NT>
 struct SampleShared {
+  static constexpr int kList = NT == 128 ? kShort : 32768;  // list places, over all warps
+  static constexpr int kFine = NT == 128 ? 4096 : 8192;     // bins of one key
+  static constexpr int kCoarse = NT == 128 ? 1024 : 2048;   // bins of several
+  static constexpr int kGroups = NT == 128 ? kShort / 256 : sel::kGroups;
   union {
     unsigned short list[kList];
     struct {
@@ -520,7 +523,8 @@ struct SampleShared {
   uint32_t key, left, bin;
   u64 before;
 };
-static_assert(2 * (sizeof(SampleShared) + 1024) <= 233472, "two blocks an SM");
+static_assert(2 * (sizeof(SampleShared<512>) + 1024) <= 233472, "two blocks an SM");
+static_assert(5 * (sizeof(SampleShared<128>) + 1024) <= 233472, "five blocks an SM");
 
 // Weight of a logit in units of 2^-42, as an integer.
 struct Weights {
@@ -537,14 +541,15 @@ __device__ __noinline__ u64 weight_of_key(const Weights& w, uint32_t key) {
 template <int NT>
 __global__ void __launch_bounds__(NT, 1024 / NT) sample_kernel(const SampleParams a) {
   extern __shared__ __align__(16) uint8_t smem_raw[];
-  SampleShared& s = *reinterpret_cast<SampleShared*>(smem_raw);
+  typedef SampleShared<NT> Shared;
+  Shared& s = *reinterpret_cast<Shared*>(smem_raw);
   constexpr int NW = NT / 32;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int64_t r = blockIdx.x;
   const __half* row = a.logits + r * a.ld;
   const int vocab = a.vocab;
   const int nvec = (vocab + 7) / 8;
-  constexpr int kOwn = kList / NW;               // places of a warp's list
+  constexpr int kOwn = Shared::kList / NW;       // places of a warp's list
   constexpr int kPer = kOwn / 256;               // groups of it
   const int stretch = (nvec + NW - 1) / NW;      // vectors of a warp's part of the row
   const int part = (stretch + 1023) / 1024 * 32;  // vectors of a 32nd of it, whole steps
@@ -556,7 +561,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) sample_kernel(const SampleParam
   const int top_k = a.top_k ? a.top_k[r] : a.top_k_s;
   const float top_p = a.top_p ? a.top_p[r] : a.top_p_s;
   const float min_p = a.min_p ? a.min_p[r] : a.min_p_s;
-  if (tid < kExpTab) s.tab[tid] = exp2((double)tid / kExpTab) * kUnit;
+  for (int i = tid; i < kExpTab; i += NT) s.tab[i] = exp2((double)i / kExpTab) * kUnit;
 
   const bool use_k = top_k > 0 && top_k < vocab;
   const bool use_p = top_p < 1.f;
@@ -768,7 +773,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) sample_kernel(const SampleParam
       tail_mass = to_units((double)warp_sum(lane < NW ? s.redf[lane][0] : 0.f) * (1.0 + 0.6931471805599453 * lost) * kUnit);
     }
     lists = __reduce_max_sync(0xffffffffu, lane < NW ? s.listed[lane] : 0u) <= kOwn;
-    ngroup = lists ? kList / 256 : (vocab + 255) / 256;
+    ngroup = lists ? Shared::kList / 256 : (vocab + 255) / 256;
     rounds = (ngroup + NW - 1) / NW;
 
     tau = lkey, left = 0xffffffffu;
@@ -776,8 +781,8 @@ __global__ void __launch_bounds__(NT, 1024 / NT) sample_kernel(const SampleParam
     // Bins in descending order of the keys; more than one key to a bin only where the range is wide.
     const uint32_t range = mkey - lkey;
     int shift = 0;
-    if (range >= kFine)
-      for (shift = 1; (range >> shift) >= kCoarse;) ++shift;
+    if (range >= Shared::kFine)
+      for (shift = 1; (range >> shift) >= Shared::kCoarse;) ++shift;
     const int bins = (int)(range >> shift) + 1;
     for (int i = tid; i < bins; i += NT) s.fine[i] = 0;
     if (shift)
@@ -1119,10 +1124,10 @@ int launch_sample(const SampleParams& p, int64_t rows, cudaStream_t s) {
   JX_CUDA_TRY(once_per_device(done,
                               [] {
                                 return cudaFuncSetAttribute(sample_kernel<NT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                                            (int)sizeof(SampleShared));
+                                                            (int)sizeof(SampleShared<NT>));
                               }),
               "jx_sample: shared memory");
-  sample_kernel<NT><<<(unsigned)rows, NT, sizeof(SampleShared), s>>>(p);
+  sample_kernel<NT><<<(unsigned)rows, NT, sizeof(SampleShared<NT>), s>>>(p);
   JX_CHECK_LAUNCH("jx_sample");
   return JX_OK;
 }
@@ -1162,6 +1167,8 @@ extern "C" int jx_sample(const void* logits16, int64_t rows, int vocab, int64_t 
                       temperature, top_p, min_p, top_k, tokens, logprobs};
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   // Two blocks of 512 threads share an SM where there are rows for them, else a row gets 1024 (one row of 32000 with top-k
-  // and top-p: 15 us, 1024 rows with top-k 62 us, of 50257 with top-p 198 us).
+  // and top-p: 15 us, 1024 rows with top-k 62 us, of 50257 with top-p 198 us). Five small blocks where rows are short and
+  // many waves of them come (20000 rows of 2000 with top-p 1026 -> 530 us; 400 rows of 4000 31 -> 43).
+  if (rows > 8 * num_sms() && vocab <= sel::kShort) return sel::launch_sample<128>(p, rows, s);
   return rows > num_sms() ? sel::launch_sample<512>(p, rows, s) : sel::launch_sample<1024>(p, rows, s);
 }

@@ -272,6 +272,28 @@ def test_sample_matches_the_definition(ops, V, kind):
     _check_draws(ops, x, u, FILTERS)
 
 
+@pytest.mark.parametrize("V,R", [(1, 1300), (257, 1300), (2049, 1400), (8192, 1300), (8193, 1200), (24000, 300)])
+@pytest.mark.parametrize("kind", ["model", "ties", "flat"])
+def test_sample_many_rows(ops, V, R, kind):
+    """Rows drawn many at a time, where they get smaller blocks: the definition for some, and for all the bits of the same
+    rows in small calls."""
+    x = torch.randn(R, (V + 7) // 8 * 8, device="cuda", generator=_gen(V + 1)) * {"model": 3.0, "ties": 3.0, "flat": 0.05}[kind]
+    if kind == "ties":
+        x = (x * 2).round() / 2
+    x = x.half()[:, :V]
+    u = torch.rand(R, device="cuda", generator=_gen(R))
+    rows = [FILTERS[r % len(FILTERS)] for r in range(R)]
+    kw = {n: torch.tensor([s.get(a, d) for s in rows], device="cuda", dtype=t)
+          for n, a, d, t in (("temperature", "T", 1.0, torch.float32), ("top_k", "k", 0, torch.int32),
+                             ("top_p", "p", 1.0, torch.float32), ("min_p", "m", 0.0, torch.float32))}
+    tok, lp = ops.sample(x, u, **kw)
+    host = x[:63].cpu().numpy()
+    assert tok[:63].tolist() == [_draw(host[r], float(u[r]), **rows[r])[0] for r in range(63)]
+    for i in range(0, R, 100):
+        t, l = ops.sample(x[i:i + 100], u[i:i + 100], **{n: v[i:i + 100] for n, v in kw.items()})
+        assert torch.equal(t, tok[i:i + 100]) and torch.equal(l.view(torch.int32), lp[i:i + 100].view(torch.int32))
+
+
 def test_sample_a_large_vocabulary(ops):
     V = 200_001
     x = (torch.randn(6, 200_008, device="cuda", generator=_gen(1)) * 2).half()[:, :V]
