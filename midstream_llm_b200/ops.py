@@ -7,6 +7,7 @@ missing library raises.
 """
 from __future__ import annotations
 
+import functools
 import math
 
 import torch
@@ -364,8 +365,14 @@ def attn_decode(qkv: torch.Tensor, kcache: torch.Tensor, vcache: torch.Tensor, l
     return o
 
 
+@functools.lru_cache(maxsize=256)
+def _prefix_workspace_bytes(device: int, *sizes: int) -> int:
+    return _lib.query("jx_attn_decode_prefix_workspace_bytes", *sizes)
+
+
 def attn_decode_prefix_workspace_bytes(B: int, H: int, kv_heads: int, prefix_len: int, max_len: int) -> int:
-    n = _lib.query("jx_attn_decode_prefix_workspace_bytes", B, H, kv_heads, prefix_len, max_len)
+    device = torch._C._cuda_getDevice() if torch.cuda.is_initialized() else -1
+    n = _prefix_workspace_bytes(device, B, H, kv_heads, prefix_len, max_len)
     if n < 0:
         raise ValueError(f"attn_decode_prefix: unsupported shape B {B}, H {H}, kv_heads {kv_heads}, prefix {prefix_len}, "
                          f"max_len {max_len}")
