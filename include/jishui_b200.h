@@ -280,7 +280,8 @@ int jx_ce_bwd(void* logits16, int64_t rows, int vocab, int64_t ld, const int64_t
  * t / temperature over the used slots (id >= 0), q = softmax(z / temperature), q1 = softmax(z):
  *   row_loss = alpha temperature^2 sum_k p_k (log p_k - log q[id_k]) + (1 - alpha) (-log q1[y]).
  * Slots naming the same id count as separate entries of that sum. A slot with t = -inf has no weight; a row
- * without a weighted slot has no first term. Rows with y == ignore_index give loss 0. A target outside
+ * without a weighted slot has no first term. Rows with y == ignore_index give loss 0 and statistics 0, and nothing
+ * else of them is read. A target outside
  * [0, vocab) that is not ignore_index gives a NaN loss and status 202, an id >= vocab a NaN loss and status 203.
  * teacher_logits: [rows, K], f16 or f32 (teacher_is_f16). stats: f32 [3, rows], the log-sum-exp of z / temperature,
  * of z (where alpha < 1) and of the used t / temperature, for the backward. parts (may be NULL): the block

@@ -124,9 +124,7 @@ __device__ __forceinline__ void finish_row(const Params& p, int64_t row, double 
   if (used) kl = d / s / p.tau + lse - lse_t;
   const int64_t y = p.targets[row];
   float loss;
-  if (y == p.ignore_index) {
-    loss = 0.f;
-  } else if (y < 0 || y >= p.vocab) {
+  if (y < 0 || y >= p.vocab) {
     if (status) atomicExch(status, kStatusCeBadTarget);
     loss = __int_as_float(0x7fc00000);
   } else {
@@ -160,6 +158,12 @@ __device__ __forceinline__ bool load_slots(const Params& p, int64_t row, const _
   return bad;
 }
 
+// A row that counts for nothing: nothing else of it is read. One thread.
+__device__ __forceinline__ void skip_row(const Params& p, int64_t row, float* row_loss) {
+  row_loss[row] = 0.f;
+  p.stats[row] = p.stats[p.rows + row] = p.stats[2 * p.rows + row] = 0.f;
+}
+
 // Merges a row's block statistics (max, sum) by one warp; every lane gets log sum exp(z).
 __device__ __forceinline__ double parts_lse(const float2* parts, int nblk, float* gmax) {
   float m = -INFINITY, s = 0.f;
@@ -186,10 +190,14 @@ __global__ void __launch_bounds__(kPartWarps * 32) distill_parts_kernel(const Pa
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int64_t row = (int64_t)blockIdx.x * kPartWarps + warp;
   if (row >= p.rows) return;
+  const int64_t y = p.targets[row];
+  if (y == p.ignore_index) {
+    if (lane == 0) skip_row(p, row, row_loss);
+    return;
+  }
   float* st = slots + warp * 2 * p.K;
   const __half* z = p.logits + row * p.ld;
   const bool bad = load_slots<32>(p, row, z, st, st + p.K, nullptr, lane, status);
-  const int64_t y = p.targets[row];
   const float zy = y >= 0 && y < p.vocab ? __half2float(z[y]) : 0.f;
   float gm;
   const double lse = parts_lse(p.parts + row * p.nblk, p.nblk, &gm);
@@ -213,6 +221,11 @@ __global__ void __launch_bounds__(NT, 1024 / NT) distill_fwd_kernel(const Params
   const __half* z = p.logits + row * p.ld;
   const int nvec = (p.vocab + 7) / 8;
   const float c = kLog2e / p.tau;
+  const int64_t y = p.targets[row];
+  if (y == p.ignore_index) {
+    if (tid == 0) skip_row(p, row, row_loss);
+    return;
+  }
   if (tid == 0) rbad = 0;
   float m = -INFINITY, s = 0.f, s1 = 0.f;
   for (int base = 0; base < nvec; base += NT * VPT) {
@@ -298,7 +311,6 @@ __global__ void __launch_bounds__(NT, 1024 / NT) distill_fwd_kernel(const Params
   s1 = warp_sum(s1);
   const double lse = (double)gm / p.tau + log_wide(s);
   const double lse1 = kTwo ? (double)gm + log_wide(s1) : p.parts ? rlse1 : lse;
-  const int64_t y = p.targets[row];
   const float zy = y >= 0 && y < p.vocab ? __half2float(z[y]) : 0.f;
   finish_row(p, row, lse, lse1, slots, slots + p.K, rbad != 0, zy, row_loss, status);
 }

@@ -592,7 +592,7 @@ def distill_fwd(logits16: torch.Tensor, teacher_ids: torch.Tensor, teacher_logit
     """Per-row distillation loss from a teacher's K top logits, mixed with the cross-entropy of the targets:
     alpha temperature^2 KL(p || q) + (1 - alpha) CE, p the teacher's softmax over its used slots (id >= 0), q the
     student's over the vocabulary, both at `temperature`. logits16 [rows, vocab] fp16, teacher_ids int64 [rows, K],
-    teacher_logits fp16 or fp32 [rows, K], targets int64 [rows] (ignore_index rows give 0). `parts` from
+    teacher_logits fp16 or fp32 [rows, K], targets int64 [rows] (of ignore_index rows nothing is read; they give 0). `parts` from
     gemm_f16_ce_parts for these logits saves the pass over them at temperature 1. Returns (stats f32 [3, rows],
     row_loss f32 [rows]); ce_loss(row_loss, targets, ignore_index) is the mean."""
     rows, vocab, ld, K = _teacher(logits16, teacher_ids, teacher_logits, targets)

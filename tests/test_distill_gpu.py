@@ -113,6 +113,26 @@ def test_unused_slots_repeated_ids_and_ignored_rows(ops, tau, alpha):
     _check(ops, torch.nn.functional.pad(x, (0, 4))[:, :500], ids, t, y, tau, alpha, in_place=True)
 
 
+@pytest.mark.parametrize("tau,alpha", [(1.0, 1.0), (1.0, 0.5), (2.0, 0.7)])
+def test_what_ignored_rows_hold_does_not_matter(ops, tau, alpha):
+    """Ids past the vocabulary, NaN logits on either side: no loss, no gradient, no status; the other rows as without them."""
+    from midstream_llm_b200 import _lib
+    x, ids, t, y = _inputs(9, 704, 12, seed=4)
+    keep = torch.tensor([0, 2, 3, 5, 8], device="cuda")
+    skip = torch.tensor([1, 4, 6, 7], device="cuda")
+    stats0, rows0 = ops.distill_fwd(x[keep], ids[keep], t[keep], y[keep], temperature=tau, alpha=alpha, ignore_index=IGNORE)
+    y[skip], ids[skip], t[skip] = IGNORE, 10 ** 12, NAN
+    x[skip] = NAN
+    _lib.device_status()
+    stats, rows = ops.distill_fwd(x, ids, t, y, temperature=tau, alpha=alpha, ignore_index=IGNORE)
+    one = torch.ones(1, device="cuda")
+    dx = ops.distill_bwd(x, ids, t, y, stats, one, one, temperature=tau, alpha=alpha, ignore_index=IGNORE,
+                         out=torch.full_like(x, 2.0))
+    assert _lib.device_status() == 0
+    assert bool((rows[skip] == 0).all()) and bool((dx[skip] == 0).all()) and bool((stats[:, skip] == 0).all())
+    assert torch.equal(rows[keep], rows0) and torch.equal(stats[:, keep], stats0) and bool(dx[keep].isfinite().all())
+
+
 def test_a_batch_of_ignored_rows_and_a_repeat(ops):
     x, ids, t, y = _inputs(4, 256, 8, seed=2)
     y[:] = IGNORE
