@@ -24,20 +24,21 @@ __device__ __forceinline__ float ex2(float x) {
 }
 
 // What a row's softmax at temperature 1 costs the forward next to the one at tau: nothing (kOne: tau = 1, alpha = 1 or given block
-// statistics), multiplications (tau = 2, 3, 4: exp(z) is a power of exp(z / tau)) or a second exponential (kBoth). The
-// exponential unit takes 2000 cycles of an SM for 32000 logits where memory takes 2700, so a second one would set the
-// time (loss of 16384 x 32000: kBoth 271 us, kPow2 191 us, kOne 178 us; the logits' read alone is 160 us at the copy rate).
-enum Mode : int { kOne = 0, kBoth = 1, kPow2 = 2, kPow3 = 3, kPow4 = 4 };
+// statistics), multiplications (tau = 2, 3, 4: exp(z) is a power of exp(z / tau); tau = 1.5: both are powers of exp(z / 3)) or
+// a second exponential (kBoth). The exponential unit takes 2000 cycles of an SM for 32000 logits where memory takes 2700,
+// so a second one would set the time (loss of 16384 x 32000: kBoth 271 us, kPow2 190 us, kPow1h 196 us, kOne 178 us; the
+// logits' read alone is 160 us at the copy rate).
+enum Mode : int { kOne = 0, kBoth = 1, kPow2 = 2, kPow3 = 3, kPow4 = 4, kPow1h = 5 };
 
 inline Mode mode_of(float tau, bool two) {
   if (!two) return kOne;
-  return tau == 2.f ? kPow2 : tau == 3.f ? kPow3 : tau == 4.f ? kPow4 : kBoth;
+  return tau == 2.f ? kPow2 : tau == 3.f ? kPow3 : tau == 4.f ? kPow4 : tau == 1.5f ? kPow1h : kBoth;
 }
 
 template <int MODE>
 __device__ __forceinline__ float power(float w) {
   const float w2 = w * w;
-  return MODE == kPow2 ? w2 : MODE == kPow3 ? w2 * w : w2 * w2;
+  return MODE == kPow2 ? w2 : MODE == kPow3 || MODE == kPow1h ? w2 * w : w2 * w2;
 }
 
 struct Params {
@@ -258,7 +259,8 @@ __global__ void __launch_bounds__(NT, 1024 / NT) distill_fwd_kernel(const Params
       }
       m = nm;
     }
-    const float mc = -m * c, mc1 = -m * kLog2e;
+    const float ce = MODE == kPow1h ? kLog2e / 3.f : c;  // of the exponential that is taken
+    const float mc = -m * ce, mc1 = -m * kLog2e;
     float a[4] = {0.f, 0.f, 0.f, 0.f}, b[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
@@ -266,8 +268,8 @@ __global__ void __launch_bounds__(NT, 1024 / NT) distill_fwd_kernel(const Params
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const float2 f = __half22float2(h[j]);
-        const float w0 = ex2(fmaf(f.x, c, mc)), w1 = ex2(fmaf(f.y, c, mc));
-        a[j] += w0 + w1;
+        const float w0 = ex2(fmaf(f.x, ce, mc)), w1 = ex2(fmaf(f.y, ce, mc));
+        a[j] += MODE == kPow1h ? fmaf(w0, w0, w1 * w1) : w0 + w1;
         if constexpr (MODE == kBoth)
           b[j] += ex2(fmaf(f.x, kLog2e, mc1)) + ex2(fmaf(f.y, kLog2e, mc1));
         else if constexpr (kTwo)
@@ -453,6 +455,7 @@ void launch_fwd(const kd::Params& p, kd::Mode mode, float* row_loss, cudaStream_
     case kd::kPow2: kd::distill_fwd_kernel<NT, 8, kd::kPow2><<<grid, NT, smem, s>>>(p, row_loss, status); break;
     case kd::kPow3: kd::distill_fwd_kernel<NT, 8, kd::kPow3><<<grid, NT, smem, s>>>(p, row_loss, status); break;
     case kd::kPow4: kd::distill_fwd_kernel<NT, 8, kd::kPow4><<<grid, NT, smem, s>>>(p, row_loss, status); break;
+    case kd::kPow1h: kd::distill_fwd_kernel<NT, 8, kd::kPow1h><<<grid, NT, smem, s>>>(p, row_loss, status); break;
   }
 }
 

@@ -94,6 +94,15 @@ def test_loss_and_gradient(ops, R, V, K, tau, alpha):
     _check(ops, x, ids, t, y, tau, alpha)
 
 
+@pytest.mark.parametrize("R,V,K", [(3, 7, 3), (6, 1000, 64), (3, 8193, 5), (400, 9000, 16), (2, 50257, 1024)])
+@pytest.mark.parametrize("alpha", [1.0, 0.7, 0.0])
+def test_loss_and_gradient_at_one_and_a_half(ops, R, V, K, alpha):
+    """Where both softmaxes are powers of one exponential."""
+    x, ids, t, y = _inputs(R, V, K, seed=V + 2 * K, t_dtype=torch.float32)
+    x[0] = (x[0].float() * 40).half()  # logits far apart, whose powers underflow
+    _check(ops, x, ids, t, y, 1.5, alpha)
+
+
 @pytest.mark.parametrize("tau,alpha", [(1.0, 1.0), (3.0, 0.6)])
 def test_unused_slots_repeated_ids_and_ignored_rows(ops, tau, alpha):
     x, ids, t, y = _inputs(12, 500, 40, seed=1, distinct=False)  # ids drawn with repeats
