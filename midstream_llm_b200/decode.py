@@ -191,7 +191,7 @@ class Completions:
 class PromptSampler:
     """Draws `n` completions of one prompt. Buffers for `max_len` positions (prompt and completion together) are kept
     across calls; the captured step is reused while the prompt's length, the sampling settings' buffers and the model's
-    weight storage stay the same (their values may change)."""
+    weight storage stay the same (their values may change). One call at a time: the buffers are the sampler's."""
 
     _CHECK = 16  # steps between looks at whether every completion has ended
 

@@ -116,6 +116,21 @@ def test_prefix_attention_scores_of_minus_infinity(ops, H, kv):
     assert bool(out[0].isnan().all())
 
 
+@pytest.mark.parametrize("B", [1, 3])
+def test_prefix_attention_single_rows(ops, B):
+    """A prefix of no rows or one, caches of one row: dimensions whose stride says nothing."""
+    H, kv = 4, 2
+    qkv, kp, vp, kc, vc, n = _prefix_state(B, H, kv, 1, 1, [1] * B, seed=B)
+    for P in (0, 1):
+        k, v = kp[:P], vp[:P]
+        kb, vb = kc[:, :1].clone(), vc[:, :1].clone()
+        out = ops.attn_decode_prefix(qkv, k, v, P, kb, vb, n, H, 64, kv_heads=kv)
+        _prefix_check(out, qkv, k, v, kb, vb, P, [1] * B, H, kv)
+    empty = torch.empty(0, kv * 64, device="cuda", dtype=torch.float16)
+    assert torch.equal(ops.attn_decode_prefix(qkv, empty, empty, 0, kb, vb, n, H, 64, kv_heads=kv),
+                       ops.attn_decode_prefix(qkv, kp, vp, 0, kb, vb, n, H, 64, kv_heads=kv))
+
+
 def test_prefix_attention_views_and_repeats(ops):
     """Keys and values as columns of one fused buffer, padded rows of the queries and the output, the caches'
     sequences in another order than their rows; the same call twice gives the same bits."""
