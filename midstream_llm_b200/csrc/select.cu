@@ -434,7 +434,8 @@ __global__ void __launch_bounds__(NT, 1024 / NT)
 //     safe one is taken. What lies below the limit is summed in fp32, which only moves the place of the cut; where
 //     the cut is nearer to a border between two ranks than that sum's error, the row is taken again with the
 //     safe limit (about one row in a thousand).
-// A histogram of the list's keys gives the threshold: counts alone where a bin is one key (its weight is the
+// Lists of up to 256 entries together are ranked by counting, and the cuts are running sums over the ranks. Else a histogram
+// of the list's keys gives the threshold: counts alone where a bin is one key (its weight is the
 // count times one exponential), else counts and weights, the latter in four 11-bit limbs, since shared memory adds 32
 // bits at a time. Then the kept weights are summed per 256 list places, and the group where the running sum passes
 // its target is walked by one warp. Lists that do not fit are replaced by the whole row. All of this runs
@@ -538,7 +539,103 @@ __device__ __noinline__ u64 weight_of_key(const Weights& w, uint32_t key) {
   return key == w.mkey ? (u64)kUnit : w.mkey == 0xfc00u ? 0ull : to_units(w.ex.value<true>(key_bits(key)));
 }
 
+// The first place whose running weight exceeds this has the token.
+__device__ __forceinline__ u64 draw_at(float u, u64 total) {
+  const double ut = (double)u * (double)total;
+  const u64 target = ut > 0.0 ? (u64)ut : 0ull;
+  return target >= total ? total - 1 : target;
+}
+
+constexpr int kFew = 256;
+
+// The draw from lists of at most 256 entries together: ranked by counting, then every cut is a running sum over that many
+// places. Leaves the list place, its key and the kept weight in s.bin, s.key and s.before.
 template <int NT>
+__device__ __noinline__ void draw_of_few(SampleShared<NT>& s, Weights wt, uint32_t top_k, float top_p, uint32_t mpkey,
+                                         float u) {
+  constexpr int NW = NT / 32, kOwn = SampleShared<NT>::kList / NW;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const uint32_t listed = lane < NW ? s.listed[lane] : 0u, listed_to = warp_scan(listed);
+  const uint32_t n = __shfl_sync(0xffffffffu, listed_to, 31);
+  const uint32_t before = __shfl_sync(0xffffffffu, listed_to - listed, warp);
+  uint32_t* ck = s.fine;       // key, and the complement of the position in index order
+  uint32_t* cp = s.fine + 256;  // list place
+  u64* rw = reinterpret_cast<u64*>(s.fine + 512);   // weights in rank order
+  u64* kw = reinterpret_cast<u64*>(s.fine + 1024);  // kept weights in index order
+#pragma unroll 1
+  for (uint32_t i = lane; i < s.listed[warp]; i += 32) {
+    ck[before + i] = order_key_num(s.list[warp * kOwn + i]) << 16 | (0xffffu - (before + i));
+    cp[before + i] = warp * kOwn + i;
+  }
+  if (tid < 4 && n + tid < kFew) ck[n + tid] = 0;
+  __syncthreads();
+  u64 w = 0;
+  uint32_t rank = 0, key = 0;
+  if (tid < n) {
+    const uint32_t mine = ck[tid];
+    for (uint32_t j = 0; j < n; j += 4) {
+      const uint4 o = *reinterpret_cast<const uint4*>(&ck[j]);
+      rank += (o.x > mine) + (o.y > mine) + (o.z > mine) + (o.w > mine);
+    }
+    key = mine >> 16;
+    w = wt.of(key_bits(key));
+    rw[rank] = w;
+  }
+  __syncthreads();
+  const int c8 = lane * 8;
+  u64 w8[8], sum = 0;
+  if (warp == 0) {
+    const uint32_t kk = min(top_k, n);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      w8[j] = c8 + j < kk ? rw[c8 + j] : 0ull;
+      sum += w8[j];
+    }
+    const u64 inc = warp_scan(sum);
+    uint32_t keep = kk;
+    if (top_p < 1.f) {  // the ranks with less than the target before them
+      const double target = fmax((double)top_p * (double)__shfl_sync(0xffffffffu, inc, 31), 1.0);
+      u64 b = inc - sum;
+      uint32_t cnt = 0;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        cnt += c8 + j < kk && (double)b < target;
+        b += w8[j];
+      }
+      keep = __reduce_add_sync(0xffffffffu, cnt);
+    }
+    if (lane == 0) s.left = keep;
+  }
+  __syncthreads();
+  if (tid < n) kw[tid] = rank < s.left && key >= mpkey ? w : 0ull;
+  __syncthreads();
+  if (warp != 0) return;
+  sum = 0;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    w8[j] = c8 + j < n ? kw[c8 + j] : 0ull;
+    sum += w8[j];
+  }
+  const u64 inc = warp_scan(sum);
+  const u64 total = __shfl_sync(0xffffffffu, inc, 31);
+  const u64 target = draw_at(u, total);
+  u64 b = inc - sum;
+  uint32_t found = 0;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    if (b <= target && target < b + w8[j]) found = c8 + j + 1;
+    b += w8[j];
+  }
+  found = __reduce_max_sync(0xffffffffu, found) - 1;
+  if (lane == 0) {
+    s.bin = cp[found];
+    s.key = ck[found] >> 16;
+    s.before = total;
+  }
+  __syncwarp();
+}
+
+template <int NT, bool kTryFew>
 __global__ void __launch_bounds__(NT, 1024 / NT) sample_kernel(const SampleParams a) {
   extern __shared__ __align__(16) uint8_t smem_raw[];
   typedef SampleShared<NT> Shared;
@@ -696,6 +793,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) sample_kernel(const SampleParam
   }
 
   uint32_t tau, left;      // the lowest key kept; how many of the elements at it (0xffffffff: all)
+  bool few = false;            // all lists together are short
   bool lists;              // or the whole row
   int ngroup, rounds;
   __half2 limit;
@@ -773,6 +871,10 @@ __global__ void __launch_bounds__(NT, 1024 / NT) sample_kernel(const SampleParam
       tail_mass = to_units((double)warp_sum(lane < NW ? s.redf[lane][0] : 0.f) * (1.0 + 0.6931471805599453 * lost) * kUnit);
     }
     lists = __reduce_max_sync(0xffffffffu, lane < NW ? s.listed[lane] : 0u) <= kOwn;
+    if (kTryFew && !tail) {
+      few = __reduce_add_sync(0xffffffffu, lane < NW ? s.listed[lane] : 0u) <= min(NT, kFew);
+      if (few) break;
+    }
     ngroup = lists ? Shared::kList / 256 : (vocab + 255) / 256;
     rounds = (ngroup + NW - 1) / NW;
 
@@ -951,6 +1053,13 @@ __global__ void __launch_bounds__(NT, 1024 / NT) sample_kernel(const SampleParam
     break;
   }
 
+  uint32_t place = 0, tkeyf = 0;  // of the token, and the sum of all that is kept
+  u64 total = 0;
+  if (kTryFew && few) {
+    draw_of_few<NT>(s, wt, use_k ? (uint32_t)top_k : 0xffffffffu, use_p ? top_p : 1.f, mpkey, a.u[r]);
+    if (warp != 0) return;
+    place = s.bin, tkeyf = s.key, total = s.before;
+  } else {
   // Weights and ties at tau per group.
   const bool ties = left != 0xffffffffu;
   u64* gmass = lists ? s.group.mass : s.row.mass;
@@ -996,11 +1105,8 @@ __global__ void __launch_bounds__(NT, 1024 / NT) sample_kernel(const SampleParam
   auto kept = [&](uint32_t before, uint32_t n) -> uint32_t { return before >= left ? 0u : min(n, left - before); };
   wsum += (u64)kept(tb, tsum) * wtie;
   const u64 winc = warp_scan(wsum);
-  const u64 total = __shfl_sync(0xffffffffu, winc, 31);
-  // The first place whose running weight exceeds u * total.
-  const double ut = (double)a.u[r] * (double)total;
-  u64 target = ut > 0.0 ? (u64)ut : 0ull;
-  if (target >= total) target = total - 1;
+  total = __shfl_sync(0xffffffffu, winc, 31);
+  const u64 target = draw_at(a.u[r], total);
   u64 wb = winc - wsum;
   int g = 0;
   const bool mine = wb <= target && target < winc;
@@ -1042,7 +1148,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) sample_kernel(const SampleParam
     wsum += w8[j];
   }
   wb += warp_scan(wsum) - wsum;
-  uint32_t place = 0, bitsf = 0;  // (of the lane that has it)
+  uint32_t bitsf = 0;  // (place and bitsf: of the lane that has it)
   if (wb <= target && target < wb + wsum) {
     bool open = true;
 #pragma unroll
@@ -1056,7 +1162,9 @@ __global__ void __launch_bounds__(NT, 1024 / NT) sample_kernel(const SampleParam
     }
   }
   place = __reduce_max_sync(0xffffffffu, place) - 1;
-  const uint32_t tkeyf = order_key_num(__reduce_max_sync(0xffffffffu, bitsf));
+  tkeyf = order_key_num(__reduce_max_sync(0xffffffffu, bitsf));
+
+  }
 
   // The element of that place: in a list, the so-manieth above the limit of its warp's stretch.
   int64_t token = place;
@@ -1118,18 +1226,27 @@ int launch_top(const __half* x, int64_t rows, int64_t ld, int vocab, int k, __ha
                                                    : launch_top_as<NT, C, false>(x, rows, ld, vocab, k, values, ids, s);
 }
 
-template <int NT>
-int launch_sample(const SampleParams& p, int64_t rows, cudaStream_t s) {
+template <int NT, bool kTryFew>
+int launch_sample_as(const SampleParams& p, int64_t rows, cudaStream_t s) {
   static std::atomic<uint64_t> done{0};
   JX_CUDA_TRY(once_per_device(done,
                               [] {
-                                return cudaFuncSetAttribute(sample_kernel<NT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                return cudaFuncSetAttribute(sample_kernel<NT, kTryFew>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                                             (int)sizeof(SampleShared<NT>));
                               }),
               "jx_sample: shared memory");
-  sample_kernel<NT><<<(unsigned)rows, NT, sizeof(SampleShared<NT>), s>>>(p);
+  sample_kernel<NT, kTryFew><<<(unsigned)rows, NT, sizeof(SampleShared<NT>), s>>>(p);
   JX_CHECK_LAUNCH("jx_sample");
   return JX_OK;
+}
+
+// Short lists are worth the look where top-k or min-p may make them (one row of 32000 with all filters 15.7 -> 10.6 us, 20000
+// rows of 2000 483 -> 246). Where neither can, the code for them would only cost the long lists' loops registers (1024
+// rows of 50257 with top-p 199 -> 217 us).
+template <int NT>
+int launch_sample(const SampleParams& p, int64_t rows, cudaStream_t s) {
+  return p.top_k || p.top_k_s > 0 || p.min_p || p.min_p_s > 0.f ? launch_sample_as<NT, true>(p, rows, s)
+                                                                : launch_sample_as<NT, false>(p, rows, s);
 }
 
 }  // namespace sel
@@ -1167,7 +1284,7 @@ extern "C" int jx_sample(const void* logits16, int64_t rows, int vocab, int64_t 
                       temperature, top_p, min_p, top_k, tokens, logprobs};
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   // Two blocks of 512 threads share an SM where there are rows for them, else a row gets 1024 (one row of 32000 with top-k
-  // and top-p: 15 us, 1024 rows with top-k 62 us, of 50257 with top-p 198 us). Five small blocks where rows are short and
+  // and top-p: 10.6 us, 1024 rows of 50257 with top-p 198 us). Five small blocks where rows are short and
   // many waves of them come (20000 rows of 2000 with top-p 1026 -> 530 us; 400 rows of 4000 31 -> 43).
   if (rows > 8 * num_sms() && vocab <= sel::kShort) return sel::launch_sample<128>(p, rows, s);
   return rows > num_sms() ? sel::launch_sample<512>(p, rows, s) : sel::launch_sample<1024>(p, rows, s);

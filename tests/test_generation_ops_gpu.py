@@ -309,6 +309,20 @@ def test_sample_many_rows(ops, V, R, kind):
         assert torch.equal(t, tok[i:i + 100]) and torch.equal(l.view(torch.int32), lp[i:i + 100].view(torch.int32))
 
 
+@pytest.mark.parametrize("V,kind", [(40, "model"), (300, "ties"), (4000, "model"), (4000, "ties"), (24000, "model"), (24000, "flat")])
+def test_sample_short_lists(ops, V, kind):
+    """Every number of kept elements up to and past what the way for short lists takes, with the other filters on top."""
+    ks = [2, 3, 4, 5, 8, 31, 32, 33, 63, 64, 100, 127, 128, 129, 200, 251, 252, 253, 254, 255, 256, 257, 300]
+    rows = [dict(k=k, **more) for k in ks for more in (dict(), dict(p=0.8), dict(m=0.2, T=0.9), dict(p=0.6, m=0.05, T=3.0))]
+    rows += [dict(m=m, T=T) for m in (1e-6, 1e-3, 0.05, 0.5) for T in (0.3, 1.0, 4.0)]
+    x = torch.randn(len(rows), (V + 7) // 8 * 8, device="cuda", generator=_gen(V)) * (0.05 if kind == "flat" else 3.0)
+    if kind == "ties":
+        x = (x * 4).round() / 4
+    u = torch.rand(len(rows), device="cuda", generator=_gen(3))
+    u[::9], u[1::9] = 0.0, 1.0 - 2 ** -24
+    _check_draws(ops, x.half()[:, :V], u, rows)
+
+
 def test_sample_a_large_vocabulary(ops):
     V = 200_001
     x = (torch.randn(6, 200_008, device="cuda", generator=_gen(1)) * 2).half()[:, :V]
