@@ -91,7 +91,8 @@ __device__ __forceinline__ double warp_sum_d(double v) {
   return v;
 }
 
-// The row's loss from the log-sum-exp of z / tau and of z, by one warp: slot_t / slot_z hold the teacher's and the student's logits of the slots, t = -inf for an unused one.
+// The row's loss from the log-sum-exp of z / tau and of z, by one warp: slot_t / slot_z hold the teacher's and the
+// student's logits of the slots, t = -inf for an unused one.
 // The few terms of a row are put together in 64 bits, since the two logarithms of sums nearly cancel where
 // student and teacher agree.
 __device__ __forceinline__ void finish_row(const Params& p, int64_t row, double lse, double lse1,

@@ -1060,109 +1060,109 @@ __global__ void __launch_bounds__(NT, 1024 / NT) sample_kernel(const SampleParam
     if (warp != 0) return;
     place = s.bin, tkeyf = s.key, total = s.before;
   } else {
-  // Weights and ties at tau per group.
-  const bool ties = left != 0xffffffffu;
-  u64* gmass = lists ? s.group.mass : s.row.mass;
-  uint32_t* gties = lists ? s.group.ties : s.row.ties;
+    // Weights and ties at tau per group.
+    const bool ties = left != 0xffffffffu;
+    u64* gmass = lists ? s.group.mass : s.row.mass;
+    uint32_t* gties = lists ? s.group.ties : s.row.ties;
 #pragma unroll 1
-  for (int k = 0; k < rounds; ++k) {
+    for (int k = 0; k < rounds; ++k) {
       const int g = group_of(k);
       if (g >= ngroup) break;
-    int count;
-    const unsigned short* p = group(g, count);
-    u64 w = 0;
-    uint32_t tie = 0;
+      int count;
+      const unsigned short* p = group(g, count);
+      u64 w = 0;
+      uint32_t tie = 0;
 #pragma unroll 1
-    for (int i = lane; i < count; i += 32) {
-      const uint32_t bits = p[i], key = key_of(bits);
-      if (ties && key == tau)
-        ++tie;
-      else if (key >= tau)
-        w += wt.of(bits);
-    }
-    __syncwarp();
-    if (count > 0) {
-      w = warp_sum64(w);
-      tie = __reduce_add_sync(0xffffffffu, tie);
-    }
-    if (lane == 0) {
-      gmass[g] = w;
-      gties[g] = tie;
-    }
-  }
-  __syncthreads();
-  if (warp != 0) return;
-
-  // One warp: a run of groups per lane. Ties are kept while fewer than `left` stand before them.
-  const u64 wtie = ties ? weight_of_key(wt, tau) : 0ull;
-  const int per = (ngroup + 31) / 32;
-  const int g0 = min(lane * per, ngroup), g1 = min(g0 + per, ngroup);
-  uint32_t tsum = 0;
-  u64 wsum = 0;
-#pragma unroll 1
-  for (int g = g0; g < g1; ++g) tsum += gties[g], wsum += gmass[g];
-  uint32_t tb = warp_scan(tsum) - tsum;
-  auto kept = [&](uint32_t before, uint32_t n) -> uint32_t { return before >= left ? 0u : min(n, left - before); };
-  wsum += (u64)kept(tb, tsum) * wtie;
-  const u64 winc = warp_scan(wsum);
-  total = __shfl_sync(0xffffffffu, winc, 31);
-  const u64 target = draw_at(a.u[r], total);
-  u64 wb = winc - wsum;
-  int g = 0;
-  const bool mine = wb <= target && target < winc;
-  if (mine) {
-#pragma unroll 1
-    for (g = g0; g < g1; ++g) {
-      const u64 w = gmass[g] + (u64)kept(tb, gties[g]) * wtie;
-      if (target < wb + w) break;
-      wb += w;
-      tb += gties[g];
-    }
-  }
-  const int src = __ffs(__ballot_sync(0xffffffffu, mine)) - 1;
-  g = __shfl_sync(0xffffffffu, g, src);
-  wb = __shfl_sync(0xffffffffu, wb, src);
-  tb = __shfl_sync(0xffffffffu, tb, src);
-  // Within the group, eight entries a lane.
-  int count;
-  const unsigned short* p = group(g, count);
-  u64 w8[8];
-  uint32_t tie8 = 0, bits8[8];
-#pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    const bool in = lane * 8 + j < count;
-    bits8[j] = in ? p[lane * 8 + j] : 0u;
-    const uint32_t key = in ? key_of(bits8[j]) : 0u;
-    const bool tie = ties && key == tau;
-    tie8 |= tie ? 1u << j : 0u;
-    w8[j] = !tie && key >= tau ? wt.of(bits8[j]) : 0ull;
-  }
-  tb += warp_scan((uint32_t)__popc(tie8)) - __popc(tie8);
-  wsum = 0;
-#pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    if (tie8 >> j & 1) {
-      w8[j] = tb < left ? wtie : 0ull;
-      ++tb;
-    }
-    wsum += w8[j];
-  }
-  wb += warp_scan(wsum) - wsum;
-  uint32_t bitsf = 0;  // (place and bitsf: of the lane that has it)
-  if (wb <= target && target < wb + wsum) {
-    bool open = true;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      wb += w8[j];
-      if (open && target < wb) {
-        open = false;
-        place = g * 256 + lane * 8 + j + 1;
-        bitsf = bits8[j];
+      for (int i = lane; i < count; i += 32) {
+        const uint32_t bits = p[i], key = key_of(bits);
+        if (ties && key == tau)
+          ++tie;
+        else if (key >= tau)
+          w += wt.of(bits);
+      }
+      __syncwarp();
+      if (count > 0) {
+        w = warp_sum64(w);
+        tie = __reduce_add_sync(0xffffffffu, tie);
+      }
+      if (lane == 0) {
+        gmass[g] = w;
+        gties[g] = tie;
       }
     }
-  }
-  place = __reduce_max_sync(0xffffffffu, place) - 1;
-  tkeyf = order_key_num(__reduce_max_sync(0xffffffffu, bitsf));
+    __syncthreads();
+    if (warp != 0) return;
+
+    // One warp: a run of groups per lane. Ties are kept while fewer than `left` stand before them.
+    const u64 wtie = ties ? weight_of_key(wt, tau) : 0ull;
+    const int per = (ngroup + 31) / 32;
+    const int g0 = min(lane * per, ngroup), g1 = min(g0 + per, ngroup);
+    uint32_t tsum = 0;
+    u64 wsum = 0;
+#pragma unroll 1
+    for (int g = g0; g < g1; ++g) tsum += gties[g], wsum += gmass[g];
+    uint32_t tb = warp_scan(tsum) - tsum;
+    auto kept = [&](uint32_t before, uint32_t n) -> uint32_t { return before >= left ? 0u : min(n, left - before); };
+    wsum += (u64)kept(tb, tsum) * wtie;
+    const u64 winc = warp_scan(wsum);
+    total = __shfl_sync(0xffffffffu, winc, 31);
+    const u64 target = draw_at(a.u[r], total);
+    u64 wb = winc - wsum;
+    int g = 0;
+    const bool mine = wb <= target && target < winc;
+    if (mine) {
+#pragma unroll 1
+      for (g = g0; g < g1; ++g) {
+        const u64 w = gmass[g] + (u64)kept(tb, gties[g]) * wtie;
+        if (target < wb + w) break;
+        wb += w;
+        tb += gties[g];
+      }
+    }
+    const int src = __ffs(__ballot_sync(0xffffffffu, mine)) - 1;
+    g = __shfl_sync(0xffffffffu, g, src);
+    wb = __shfl_sync(0xffffffffu, wb, src);
+    tb = __shfl_sync(0xffffffffu, tb, src);
+    // Within the group, eight entries a lane.
+    int count;
+    const unsigned short* p = group(g, count);
+    u64 w8[8];
+    uint32_t tie8 = 0, bits8[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const bool in = lane * 8 + j < count;
+      bits8[j] = in ? p[lane * 8 + j] : 0u;
+      const uint32_t key = in ? key_of(bits8[j]) : 0u;
+      const bool tie = ties && key == tau;
+      tie8 |= tie ? 1u << j : 0u;
+      w8[j] = !tie && key >= tau ? wt.of(bits8[j]) : 0ull;
+    }
+    tb += warp_scan((uint32_t)__popc(tie8)) - __popc(tie8);
+    wsum = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      if (tie8 >> j & 1) {
+        w8[j] = tb < left ? wtie : 0ull;
+        ++tb;
+      }
+      wsum += w8[j];
+    }
+    wb += warp_scan(wsum) - wsum;
+    uint32_t bitsf = 0;  // (place and bitsf: of the lane that has it)
+    if (wb <= target && target < wb + wsum) {
+      bool open = true;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        wb += w8[j];
+        if (open && target < wb) {
+          open = false;
+          place = g * 256 + lane * 8 + j + 1;
+          bitsf = bits8[j];
+        }
+      }
+    }
+    place = __reduce_max_sync(0xffffffffu, place) - 1;
+    tkeyf = order_key_num(__reduce_max_sync(0xffffffffu, bitsf));
 
   }
 
