@@ -485,7 +485,7 @@ struct Exp {
   }
 };
 
-// round(v) of 0 <= v < 2^51 as an integer.
+// round(v) of 0 <= v < 2^51 as an integer: one weight (at most 2^42), not a sum of them.
 __device__ __forceinline__ u64 to_units(double v) {
   return (u64)__double_as_longlong(v + 0x1p52) & 0xfffffffffffffull;
 }
@@ -868,7 +868,9 @@ __global__ void __launch_bounds__(NT, 1024 / NT) sample_kernel(const SampleParam
       // nat under it.
       const double lost = ((double)limit32 - (double)m32 - (double)T) * (1.4426950408889634 / (double)T - (double)c) +
                           (-(double)m32 * (double)c - (double)c0);
-      tail_mass = to_units((double)warp_sum(lane < NW ? s.redf[lane][0] : 0.f) * (1.0 + 0.6931471805599453 * lost) * kUnit);
+      // (Up to 2^62: below a tried limit may lie most of a smooth row's weight, many times the maximum's.)
+      tail_mass = __double2ull_rn((double)warp_sum(lane < NW ? s.redf[lane][0] : 0.f) * (1.0 + 0.6931471805599453 * lost) *
+                                  kUnit);
     }
     lists = __reduce_max_sync(0xffffffffu, lane < NW ? s.listed[lane] : 0u) <= kOwn;
     if (kTryFew && !tail) {

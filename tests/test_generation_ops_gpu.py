@@ -468,3 +468,46 @@ def test_top_logits_refusals(ops):
         ops.top_logits(torch.zeros(1, 4096, device="cuda", dtype=torch.float16), 1025)
     v, i = ops.top_logits(x[:0], 4)
     assert v.shape == (0, 4) and i.shape == (0, 4)
+
+
+# ---------------------------------------------------------------- top-p alone
+# Smooth rows: most of the weight lies below the limit that a row's list of tokens starts at. (spread, temperature)
+SMOOTH = [(0.36, 1.0), (0.4, 1.0), (0.45, 1.0), (0.5, 1.0), (0.55, 1.0), (1.0, 3.0)]
+
+
+def _check_alike(ops, x, u, tokens, logprobs, times, **kw):
+    """The rows again, `times` over in one call: the same draws (more rows get smaller blocks)."""
+    tok, lp = ops.sample(x.repeat(times, 1), u.repeat(times), **kw)
+    assert torch.equal(tok, tokens.repeat(times)) and torch.equal(lp.view(torch.int32), logprobs.view(torch.int32).repeat(times))
+
+
+@pytest.mark.parametrize("V", [8192, 24000, 32000, 32768, 50256])
+@pytest.mark.parametrize("p", [0.3, 0.5, 0.7, 0.8, 0.9, 0.95])
+def test_sample_nucleus_of_smooth_rows(ops, V, p):
+    n = len(SMOOTH)
+    x = torch.randn(n, V, device="cuda", generator=_gen(V))
+    x = (x * torch.tensor([s for s, _ in SMOOTH], device="cuda")[:, None] + 0.3).half()
+    u = torch.rand(n, device="cuda", generator=_gen(int(100 * p)))
+    _check_draws(ops, x, u, [dict(p=p, T=T) for _, T in SMOOTH])
+    same = slice(0, n - 1)
+    _check_draws(ops, x[same], u[same], [dict(p=p)] * (n - 1))
+    tok, lp = ops.sample(x[same], u[same], top_p=p)
+    for times in (40, 240):
+        _check_alike(ops, x[same], u[same], tok, lp, times, top_p=p)
+
+
+@pytest.mark.parametrize("V,first", [(32000, 8192), (50256, 8192), (50256, 50000), (32000, 4096)])
+@pytest.mark.parametrize("p", [0.5, 0.9])
+def test_sample_nucleus_of_rows_that_begin_unlike_the_rest(ops, V, first, p):
+    """The first tokens masked, or far below or above all others: what they say about the row is wrong."""
+    x = (torch.randn(6, V, device="cuda", generator=_gen(V + first)) * 0.4).half()
+    x[0, :first] = -INF
+    x[1, :first] -= 4.0
+    x[2, :first] -= 20.0
+    x[3, :first] += 4.0
+    x[4, :first] += 2.0
+    x[5, first:] = -INF
+    u = torch.rand(6, device="cuda", generator=_gen(first))
+    _check_draws(ops, x, u, [dict(p=p)] * 6)
+    tok, lp = ops.sample(x, u, top_p=p)
+    _check_alike(ops, x, u, tok, lp, 30, top_p=p)
