@@ -521,7 +521,7 @@ struct SampleShared {
   u64 red64[32];
   uint32_t red[32];
   float redf[32][kGuess + 1];
-  uint32_t key, left, bin;
+  uint32_t key, left, bin, again;
   u64 before;
 };
 static_assert(2 * (sizeof(SampleShared<512>) + 1024) <= 233472, "two blocks an SM");
@@ -1032,10 +1032,10 @@ __global__ void __launch_bounds__(NT, 1024 / NT) sample_kernel(const SampleParam
           s.left = w ? (uint32_t)fmin(fmax(ceil(q), 1.0), (double)cnt) : cnt;
           // Too near to a border for the fp32 sum's error (about 3e-7 of it): once more with the safe limit, below
           // which lies a few hundredths of that weight.
-          s.bin = lkey > safe && fabs(q - rint(q)) * (double)w <= 3e-7 * (double)tail_mass ? 1u : 0u;
+          s.again = lkey > safe && fabs(q - rint(q)) * (double)w <= 3e-7 * (double)tail_mass ? 1u : 0u;
         }
         __syncthreads();
-        if (s.bin) {
+        if (s.again) {
           lkey = safe;
           __syncthreads();
           continue;
