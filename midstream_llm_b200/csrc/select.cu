@@ -119,6 +119,12 @@ __device__ __forceinline__ u64 warp_sum64(u64 v) {
   return v;
 }
 
+__device__ __forceinline__ double warp_sum_d(double v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+
 // Inclusive prefix sums over the lanes of a warp.
 template <typename T>
 __device__ __forceinline__ T warp_scan(T v) {
@@ -431,9 +437,9 @@ __global__ void __launch_bounds__(NT, 1024 / NT)
 //   - top-p without top-k: e < (1 - top_p) / V, since all such elements together weigh less than what top-p
 //     drops (the maximum alone weighs 1). That limit is low, so a higher one is tried first, which a part of the row
 //     says leaves three quarters of 1 - top_p below; whether it does is seen from the sums, and if not, the
-//     safe one is taken. What lies below the limit is summed in fp32, which only moves the place of the cut; where
-//     the cut is nearer to a border between two ranks than that sum's error, the row is taken again with the
-//     safe limit (about one row in a thousand).
+//     safe one is taken. What lies below the limit is summed from fp32 exponentials, which only moves the place of the
+//     cut; where the cut is nearer to a border between two ranks than that sum's error (kTailError of it), it is
+//     taken again with that sum in the weights' own units.
 // Lists of up to 256 entries together are ranked by counting, and the cuts are running sums over the ranks. Else a histogram
 // of the list's keys gives the threshold: counts alone where a bin is one key (its weight is the
 // count times one exponential), else counts and weights, the latter in four 11-bit limbs, since shared memory adds 32
@@ -444,6 +450,11 @@ constexpr int kGroups = 4096;    // groups of 256 elements of a whole row: vocab
 constexpr int kShort = 8192;     // rows up to here get small blocks, whose lists always hold them
 constexpr double kUnit = 4398046511104.0;  // 2^42: weights of a row of 2^20 elements sum to at most 2^62
 constexpr int kExpTab = 256;
+// Bound of the relative error of the weight below a limit: ex2.approx 2^-22, its argument rounded to fp32 2^-20 ln 2 up to
+// 2^5 octaves under the maximum and twice that up to 2^6 (further down nothing counts), the rounded factor c over
+// eight octaves about the place where it is made up for 2^-24 8 ln 2, three additions of fp32 numbers 3 2^-24;
+// everything after that is added in 64 bits. Together below 2.2e-6.
+constexpr double kTailError = 4e-6;
 constexpr int kGuess = 8;        // limits tried, 2.5 octaves of weight apart
 
 struct SampleParams {
@@ -544,6 +555,24 @@ __device__ __forceinline__ u64 draw_at(float u, u64 total) {
   const double ut = (double)u * (double)total;
   const u64 target = ut > 0.0 ? (u64)ut : 0ull;
   return target >= total ? total - 1 : target;
+}
+
+// What weighs below `lkey` in the row, exactly. Every thread of the block calls it.
+template <int NT>
+__device__ __noinline__ u64 exact_tail(const __half* row, int vocab, Weights wt, uint32_t lkey, u64* red) {
+  u64 sum = 0, total;
+  const int nvec = (vocab + 7) / 8;
+#pragma unroll 1
+  for (int i = threadIdx.x; i < nvec; i += NT) {
+    const Vec v = load_vec<kFillNegInf>(row, i, vocab);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const uint32_t key = order_key_num(v.bits(j));
+      if (key > kKeyNegInf && key < lkey) sum += to_units(wt.ex.value<true>(v.bits(j)));
+    }
+  }
+  block_scan<NT>(sum, red, &total);
+  return total;
 }
 
 constexpr int kFew = 256;
@@ -816,7 +845,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) sample_kernel(const SampleParam
     // The lists, and the weight of what stays out of them.
     limit = __half2half2(key_half(lkey));
     const float limit32 = __half2float(key_half(lkey));
-    float rest = 0.f;
+    double rest = 0.0;
     uint32_t mine = 0;
     int parts = 0, mark = lane == 0 ? v0 : 0x7fffffff;
     auto own_vec = [&](int i) {
@@ -847,19 +876,20 @@ __global__ void __launch_bounds__(NT, 1024 / NT) sample_kernel(const SampleParam
         }
       }
       if (tail) {
+        float pair[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const float2 f = __half22float2(as_half2(v.w[j]));
           const float e0 = ex2(fmaf(f.x, c, c0)), e1 = ex2(fmaf(f.y, c, c0));
-          if (f.x < limit32) rest += e0;
-          if (f.y < limit32) rest += e1;
+          pair[j] = (f.x < limit32 ? e0 : 0.f) + (f.y < limit32 ? e1 : 0.f);
         }
+        rest += (double)((pair[0] + pair[1]) + (pair[2] + pair[3]));
       }
     }
     if (lane == 0) s.listed[warp] = mine;
     if (tail) {
-      rest = warp_sum(rest);
-      if (lane == 0) s.redf[warp][0] = rest;
+      rest = warp_sum_d(rest);
+      if (lane == 0) s.red64[warp] = (u64)__double_as_longlong(rest);
     }
     __syncthreads();
     u64 tail_mass = 0;
@@ -868,9 +898,9 @@ __global__ void __launch_bounds__(NT, 1024 / NT) sample_kernel(const SampleParam
       // nat under it.
       const double lost = ((double)limit32 - (double)m32 - (double)T) * (1.4426950408889634 / (double)T - (double)c) +
                           (-(double)m32 * (double)c - (double)c0);
+      const double below = warp_sum_d(lane < NW ? __longlong_as_double((long long)s.red64[lane]) : 0.0);
       // (Up to 2^62: below a tried limit may lie most of a smooth row's weight, many times the maximum's.)
-      tail_mass = __double2ull_rn((double)warp_sum(lane < NW ? s.redf[lane][0] : 0.f) * (1.0 + 0.6931471805599453 * lost) *
-                                  kUnit);
+      tail_mass = __double2ull_rn(below * (1.0 + 0.6931471805599453 * lost) * kUnit);
     }
     lists = __reduce_max_sync(0xffffffffu, lane < NW ? s.listed[lane] : 0u) <= kOwn;
     if (kTryFew && !tail) {
@@ -936,7 +966,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) sample_kernel(const SampleParam
     }
     const uint32_t cabove = block_scan<NT>(csum, s.red, &ctotal);
     if (use_p) mabove = block_scan<NT>(msum, s.red64, &mtotal);
-    if (lkey > safe && (double)mtotal < (double)fmaxf(top_p, 0.f) * (double)(mtotal + tail_mass) * (1.0 + 1e-6)) {
+    if (lkey > safe && (double)mtotal < (double)fmaxf(top_p, 0.f) * (double)(mtotal + tail_mass) * (1.0 + kTailError)) {
       lkey = safe;  // the cut lies below the limit after all
       continue;
     }
@@ -997,23 +1027,24 @@ __global__ void __launch_bounds__(NT, 1024 / NT) sample_kernel(const SampleParam
     }
     if (use_p) {
       // Kept are the ranks with less than `target` before them, and the first.
-      const double target = fmax((double)top_p * (double)mtotal, 1.0);  // in units: the first has 2^42
-      if (tid == 0) s.bin = 0xffffffffu;
-      __syncthreads();
-      if ((double)mabove < target && (double)(mabove + msum) >= target) {  // one thread, if the target is within
-        u64 mb = mabove;
-        int i = b0;
-        for (; i < b1 - 1; ++i) {
-          const u64 m = bin_mass(i);
-          if ((double)(mb + m) >= target) break;
-          mb += m;
+      for (bool exact = !tail;; exact = true) {  // at most twice
+        const double target = fmax((double)top_p * (double)mtotal, 1.0);  // in units: the first has 2^42
+        if (tid == 0) s.bin = 0xffffffffu;
+        __syncthreads();
+        if ((double)mabove < target && (double)(mabove + msum) >= target) {  // one thread, if the target is within
+          u64 mb = mabove;
+          int i = b0;
+          for (; i < b1 - 1; ++i) {
+            const u64 m = bin_mass(i);
+            if ((double)(mb + m) >= target) break;
+            mb += m;
+          }
+          s.bin = i;
+          s.before = mb;
         }
-        s.bin = i;
-        s.before = mb;
-      }
-      __syncthreads();
-      const uint32_t bin = s.bin;
-      if (bin != 0xffffffffu) {
+        __syncthreads();
+        const uint32_t bin = s.bin;
+        if (bin == 0xffffffffu) break;
         if (shift) fill_sub(bin);
         if (tid == 0) {
           uint32_t key = mkey - (bin << shift), cnt = shift ? s.sub[0] : s.fine[bin];
@@ -1030,14 +1061,12 @@ __global__ void __launch_bounds__(NT, 1024 / NT) sample_kernel(const SampleParam
           const double q = w ? (target - (double)mb) / (double)w : 0.0;
           s.key = key;
           s.left = w ? (uint32_t)fmin(fmax(ceil(q), 1.0), (double)cnt) : cnt;
-          // Too near to a border for the fp32 sum's error (about 3e-7 of it): once more with the safe limit, below
-          // which lies a few hundredths of that weight.
-          s.again = lkey > safe && fabs(q - rint(q)) * (double)w <= 3e-7 * (double)tail_mass ? 1u : 0u;
+          // Too near to a border for the error of the weight below the limit: once more with the exact one.
+          s.again = !exact && fabs(q - rint(q)) * (double)w <= kTailError * (double)tail_mass ? 1u : 0u;
         }
         __syncthreads();
         if (s.again) {
-          lkey = safe;
-          __syncthreads();
+          mtotal += exact_tail<NT>(row, vocab, wt, lkey, s.red64) - tail_mass;
           continue;
         }
         // Never past the top-k threshold.
@@ -1045,6 +1074,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) sample_kernel(const SampleParam
           tau = s.key;
           left = s.left;
         }
+        break;
       }
     }
     if (mpkey > tau) {

@@ -511,3 +511,53 @@ def test_sample_nucleus_of_rows_that_begin_unlike_the_rest(ops, V, first, p):
     _check_draws(ops, x, u, [dict(p=p)] * 6)
     tok, lp = ops.sample(x, u, top_p=p)
     _check_alike(ops, x, u, tok, lp, 30, top_p=p)
+
+
+def _rows_cut_near_a_border(V, n, seed):
+    """Rows of two values whose nucleus ends within 1e-4 of a token's weight of a border between two tokens, just before
+    it and just behind it in turn: (logits, uniforms, settings). The tokens of the lower value lie below the list of
+    the larger ones, so the sum of their weights, all equal, sets the place of the cut. The definition's running sum
+    of up to V / 2 equal terms is off by at most V / 2 half steps of a number below V: 3e-5 for V of a million (the border
+    is 1e-4 to 1e-3 away there), below 1e-7 for 50256."""
+    rng, near = np.random.default_rng(seed), max(1e-5, 1e-10 * V)
+    x, settings = np.empty((n, V), np.float16), []
+    for r in range(n):
+        while True:
+            m, d = np.float16(rng.uniform(-9, 9)), np.float16(rng.uniform(2.1, 3.9))
+            low = np.float16(m - d)
+            e = math.exp(float(low) - float(m))
+            high = rng.integers(int(0.5 * V), int(0.8 * V), 20000)
+            p = rng.uniform(0.3, 0.75, 20000).astype(np.float32)
+            q = p.astype(np.float64) * (high + (V - high) * e)
+            off = q - np.rint(q)
+            want = (off < 0) if r % 2 else (off > 0)
+            fits = np.flatnonzero(want & (np.abs(off) > near) & (np.abs(off) < 10 * near))
+            if len(fits):
+                break
+        i = fits[0]
+        x[r] = np.where(rng.permutation(V) < high[i], m, low)
+        settings.append(dict(p=float(p[i])))
+    return torch.from_numpy(x).cuda(), torch.full((n,), 1.0 - 2 ** -24, device="cuda"), settings
+
+
+@pytest.mark.parametrize("V,n", [(8192, 12), (50256, 24), (1_000_000, 6)])
+def test_sample_nucleus_that_ends_at_a_border(ops, V, n):
+    """Which tokens are kept is decided in 64 bits, however many equal weights the sum below the list has. (With the last
+    kept token drawn, its place and probability both tell how many there are.)"""
+    x, u, settings = _rows_cut_near_a_border(V, n, V)
+    _check_draws(ops, x, u, settings)
+    p = torch.tensor([s["p"] for s in settings], device="cuda")
+    tok, lp = ops.sample(x, u, top_p=p)
+    for times in (200 // n, 1200 // n) if V < 10 ** 6 else ():
+        _check_alike(ops, x, u, tok, lp, times, top_p=p.repeat(times))
+
+
+def test_sample_nucleus_of_smooth_rows_of_a_large_vocabulary(ops):
+    V, n = 200_000, len(SMOOTH)
+    x = torch.randn(n, V, device="cuda", generator=_gen(V))
+    x = (x * torch.tensor([s for s, _ in SMOOTH], device="cuda")[:, None]).half()
+    u = torch.rand(n, device="cuda", generator=_gen(1))
+    for p in (0.3, 0.5, 0.8, 0.95):
+        _check_draws(ops, x, u, [dict(p=p, T=T) for _, T in SMOOTH])
+        tok, lp = ops.sample(x[:5], u[:5], top_p=p)
+        _check_alike(ops, x[:5], u[:5], tok, lp, 32, top_p=p)
