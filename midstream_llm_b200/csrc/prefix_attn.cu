@@ -29,10 +29,12 @@
 //
 // 224 threads, two blocks an SM (256 TMEM columns each):
 //   warp 0    TMA producer: Q of the item, K and V tiles (2 and 3 slots of 16 KB),
-//   warp 1    issues the first products; before the tile that holds a sequence's end it puts the new key and value
-//             into the tile (and the cache) and clears the values behind them, since 0 * garbage may be NaN,
+//   warp 1    issues the first products; into the tile that holds a sequence's end it first puts the new key (and into the
+//             cache),
 //   warps 2-5 softmax, one key per thread, and the parts' output,
-//   warp 6    issues the second products (with one warp for both, its twelve products a tile, their waits and
+//   warp 6    issues the second products, and puts the new value into such a tile and clears what is behind it, since
+//             0 * garbage may be NaN. It alone touches V's slots: it waits for every fill of theirs in turn, so no wait
+//             can take an earlier fill for its own (with one warp for both products, its twelve products a tile, their waits and
 //             commits follow each other: 36.4 against 35.4 us at 64 rows of 32749 keys, 29.4 against 27.6 at one).
 // 64 sequences of 16 heads on a prefix of 32749, 1 to 1000 own tokens: 59 us, 4.5 TB/s; the prefix's tiles are bound by
 // the chain scores - exponents - exponentials - product of a tile (about 3300 cycles with two blocks an SM), not by memory.
@@ -530,31 +532,24 @@ __global__ void __launch_bounds__(kThreads, 2)
     const uint64_t dQ0 = smem_desc_sw128(smem_u32(sQ), 16, 1024), dQp = smem_desc_sw128(smem_u32(sQp), 16, 1024);
     for (uint32_t ts = 0; c.advance(s, lens); ++ts) {
       const int x = ts & 1;
-      const uint32_t ks = ts % kKSlots, vs = ts % kVSlots;
+      const uint32_t ks = ts % kKSlots;
       const int q = c.is_own ? (c.iown & 1) : 2;
       if (c.j == 0) {
         const uint32_t use = c.is_own ? (uint32_t)(c.iown >> 1) : (uint32_t)c.ipre;
         if (!warp_wait(&bars->q_full[q], use & 1, abort_flag, status, kMma)) break;
       }
       const bool ends = c.ends();
-      const bool is_v = lane >= 8;
-      const int ch = lane & 7;
-      uint4 fresh = make_uint4(0, 0, 0, 0);  // lanes 0-7: the new key, 8-15: the new value
-      if (ends && lane < 16)
-        fresh = *reinterpret_cast<const uint4*>(p.qkv + (int64_t)c.b * p.ld_qkv + (s.H + c.h + (is_v ? s.Hkv : 0)) * D + ch * 8);
+      uint4 fresh = make_uint4(0, 0, 0, 0);  // lanes 0-7: the new key
+      if (ends && lane < 8)
+        fresh = *reinterpret_cast<const uint4*>(p.qkv + (int64_t)c.b * p.ld_qkv + (s.H + c.h) * D + lane * 8);
       if (!warp_wait(&bars->k_full[ks], (ts / kKSlots) & 1, abort_flag, status, kMma)) break;
-      if (ends) {
-        // The sequence ends in this tile: row `last` is the new token's.
-        if (!warp_wait(&bars->v_full[vs], (ts / kVSlots) & 1, abort_flag, status, kMma)) break;
+      if (ends) {  // the sequence ends in this tile: row `last` is the new token's
         const int last = c.limit - 1 - c.key();
-        if (lane < 16) {
-          uint8_t* tile = is_v ? sV + vs * kTile : sK + ks * kTile;
-          *reinterpret_cast<uint4*>(tile + last * 128 + ((ch ^ (last & 7)) << 4)) = fresh;
-          *reinterpret_cast<uint4*>((is_v ? p.vcache : p.kcache) + (int64_t)c.b * p.batch_stride +
-                                    (int64_t)(c.limit - 1) * p.ld_cache + c.h * D + ch * 8) = fresh;
+        if (lane < 8) {
+          *reinterpret_cast<uint4*>(sK + ks * kTile + last * 128 + ((lane ^ (last & 7)) << 4)) = fresh;
+          *reinterpret_cast<uint4*>(p.kcache + (int64_t)c.b * p.batch_stride + (int64_t)(c.limit - 1) * p.ld_cache + c.h * D +
+                                    lane * 8) = fresh;
         }
-        for (int i = (last + 1) * 8 + lane; i < BKV * 8; i += 32)
-          *reinterpret_cast<uint4*>(sV + vs * kTile + i * 16) = make_uint4(0, 0, 0, 0);
         fence_proxy_async_smem();
         __syncwarp();
       }
@@ -574,19 +569,36 @@ __global__ void __launch_bounds__(kThreads, 2)
       __syncwarp();
     }
   } else if (warp == 6) {
-    if (lane == 0) {
-      const uint64_t dP0 = smem_desc_sw128(smem_u32(sP), 8192, 1024);
-      // A of the second product for slot 0 and keys 0-15: rows 0-63 are V^T, rows 64-127, one leading offset on, ones.
-      // 16 keys (2 KB) or a slot further, the start moves up and the leading offset down by as much, both in units of 16.
-      const uint64_t dV0 = smem_desc_sw128(smem_u32(sV), smem_u32(s1) - smem_u32(sV), 1024);
-      constexpr uint64_t kStep = 2048 / 16, kSlot = kTile / 16;
-      for (uint32_t tp = 0; c.advance(s, lens); ++tp) {
-        const uint32_t vs = tp % kVSlots;
+    const uint64_t dP0 = smem_desc_sw128(smem_u32(sP), 8192, 1024);
+    // A of the second product for slot 0 and keys 0-15: rows 0-63 are V^T, rows 64-127, one leading offset on, ones.
+    // 16 keys (2 KB) or a slot further, the start moves up and the leading offset down by as much, both in units of 16.
+    const uint64_t dV0 = smem_desc_sw128(smem_u32(sV), smem_u32(s1) - smem_u32(sV), 1024);
+    constexpr uint64_t kStep = 2048 / 16, kSlot = kTile / 16;
+    for (uint32_t tp = 0; c.advance(s, lens); ++tp) {
+      const uint32_t vs = tp % kVSlots;
+      const bool ends = c.ends();
+      uint4 fresh = make_uint4(0, 0, 0, 0);  // lanes 0-7: the new value
+      if (ends && lane < 8)
+        fresh = *reinterpret_cast<const uint4*>(p.qkv + (int64_t)c.b * p.ld_qkv + (s.H + s.Hkv + c.h) * D + lane * 8);
+      if (!warp_wait(&bars->v_full[vs], (tp / kVSlots) & 1, abort_flag, status, kMma)) break;
+      if (ends) {
+        const int last = c.limit - 1 - c.key();
+        uint8_t* tile = sV + vs * kTile;
+        if (lane < 8) {
+          *reinterpret_cast<uint4*>(tile + last * 128 + ((lane ^ (last & 7)) << 4)) = fresh;
+          *reinterpret_cast<uint4*>(p.vcache + (int64_t)c.b * p.batch_stride + (int64_t)(c.limit - 1) * p.ld_cache + c.h * D +
+                                    lane * 8) = fresh;
+        }
+        for (int i = (last + 1) * 8 + lane; i < BKV * 8; i += 32)
+          *reinterpret_cast<uint4*>(tile + i * 16) = make_uint4(0, 0, 0, 0);
+        fence_proxy_async_smem();
+        __syncwarp();
+      }
+      if (!warp_wait(&bars->p_full, tp & 1, abort_flag, status, kMma)) break;
+      tc_fence_after();
+      if (lane == 0) {
         const uint32_t idesc = idesc_f16_f32(128, 0, true, true) | ((uint32_t)(c.rows(s) + 15) >> 4) << 18;
         const uint64_t dv = dV0 + vs * (kSlot - (kSlot << 16));
-        if (!wait(&bars->v_full[vs], (tp / kVSlots) & 1, abort_flag, status, kMma)) break;
-        if (!wait(&bars->p_full, tp & 1, abort_flag, status, kMma)) break;
-        tc_fence_after();
 #pragma unroll
         for (int kk = 0; kk < BKV / 16; ++kk)
           umma_f16(tmem + 128, dv + kk * (kStep - (kStep << 16)), desc_adv(dP0, kk * 2048), idesc,
@@ -594,8 +606,8 @@ __global__ void __launch_bounds__(kThreads, 2)
         umma_commit(&bars->v_empty[vs]);
         umma_commit(&bars->p_empty);
       }
+      __syncwarp();
     }
-    __syncwarp();
   } else {
     bool ok = true;
     for (uint32_t g = 0; ok && c.advance(s, lens);) {
