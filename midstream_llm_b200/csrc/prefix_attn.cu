@@ -9,11 +9,17 @@
 // transposed, with the keys along the matrix unit's 128 rows: then a thread owns one key, and the softmax's work is
 // in proportion to the query rows and spread over all four warps however few they are. For every 128 keys
 //   S^T = K Q^T        (tcgen05, M 128 keys, N 16-64 rows, K 64, both from shared memory)          -> TMEM
-//   P   = exp2(S scale - m) as fp16, against a reference m per row                                 -> shared memory
-//   [O^T; l] += [V^T; 1] P  (tcgen05, M 128 = 64 head columns and the sum's row, N rows, K 128 keys) -> TMEM
-// m is the row's maximum over the first tile and is raised only when a later P passes 2^8 (a rare step that
-// rescales O^T), so no other tile needs a maximum across threads. The sum l comes out of the same product from
-// the same rounded P, by a block of ones behind V^T.
+//   P   = exp2(S scale - m) as two fp16 numbers, against a reference m per row                     -> shared memory
+//   [O^T; l] += [V^T; 1] P  (tcgen05, M 128 = 64 head columns and the sum's row, N twice the rows, K 128 keys) -> TMEM
+// m lies 7 (log2 units) below the row's maximum over the first tile and is raised only when a later P passes 2^15 (a rare
+// step that rescales O^T), so no other tile needs a maximum across threads. The sum l comes out of the same product
+// from the same P, by a block of ones behind V^T.
+//
+// A probability is held in 22 bits at least, as what fp16 leaves of it is an fp16 number of its own: the rest's columns stand
+// behind P's, so the same product takes both, and their results are added where a part is written. P in fp16 alone
+// would leave 2^-12 of each: 2.9e-4 of the output's norm from the exact one, instead of 2.1e-4, which its own rounding to fp16
+// makes. It costs conversions and stores in the softmax warps: 59.1 -> 62.8 us for 64 sequences behind 32749 keys,
+// 42.9 -> 47.6 us for 96 of 32 heads on 8 key heads, less than 2 % for 16 rows and fewer.
 //
 // A sequence's own keys belong to no other, so a product has only its G heads as rows, and an item as short as a few
 // keys still pays the whole chain from TMA to the output (about 3 us). With up to four heads a key head they are
@@ -28,7 +34,7 @@
 // workspace, the second kernel joins them. The schedule is fixed by the sizes, so results repeat bit for bit.
 //
 // 224 threads, two blocks an SM (256 TMEM columns each):
-//   warp 0    TMA producer: Q of the item, K and V tiles (2 and 3 slots of 16 KB),
+//   warp 0    TMA producer: Q of the item, K and V tiles (2 slots of 16 KB each),
 //   warp 1    issues the first products; into the tile that holds a sequence's end it first puts the new key (and into the
 //             cache),
 //   warps 2-5 softmax, one key per thread, and the parts' output,
@@ -55,10 +61,17 @@ constexpr int kThreads = 224;
 constexpr uint32_t kTile = BKV * D * 2;   // 16 KiB
 constexpr uint32_t kQTile = kRows * D * 2;  // 8 KiB
 constexpr uint32_t kOnes = 2048;          // 16 keys x 64 ones
-constexpr int kKSlots = 2, kVSlots = 3;
+constexpr int kKSlots = 2, kVSlots = 2;
 constexpr int kLens = 512;  // lengths kept in shared memory
-constexpr uint32_t kTmemCols = 256;  // S^T [0,64) and [64,128), [O^T; l] [128,192)
+constexpr uint32_t kTmemCols = 256;  // S^T [0,64) and [64,128), [O^T; l] and that of P's rest [128,256)
 
+// A row's reference is its maximum less kLift (log2 units) and may be passed by kLift + 8, so P is 2^7 at the maximum and at
+// most 2^15, and what fp16 has below 1 goes to the keys far under the maximum. The rest of P, at most 2^-11 of it, is
+// held kRest times as large.
+constexpr float kLift = 7.f;
+constexpr float kRest = 2048.f;
+// Where the rest's columns stand behind P's, by the rows of an item.
+__host__ __device__ constexpr int rest_at(int rows) { return rows <= 16 ? 16 : rows <= 32 ? 32 : 64; }
 constexpr float kNoKey = -1e30f;  // the running maximum before the first key: below every product of fp16 numbers, and
                                  // a score of -infinity less it is no NaN
 
@@ -281,6 +294,7 @@ __device__ __forceinline__ bool softmax_item(const Params& p, Cursor& c, const i
   const int key = quarter * 32 + lane;
   const uint32_t base = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
   uint8_t* prow = sP + key * 128;
+  constexpr int R = rest_at(W);
   const float scale = p.scale_log2;
   for (c.j = 0; c.j < c.n; ++c.j, ++g) {
     const int x = g & 1;
@@ -309,7 +323,7 @@ __device__ __forceinline__ bool softmax_item(const Params& p, Cursor& c, const i
           r[2] = __float_as_uint(y1.x), r[3] = __float_as_uint(y1.y);
         }
       }
-      return !past && fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) > 8.f;
+      return !past && fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) > kLift + 8.f;
     };
     bool raise = c.j == 0;
     if (!raise) raise = softmax_any(exponents());
@@ -334,7 +348,7 @@ __device__ __forceinline__ bool softmax_item(const Params& p, Cursor& c, const i
         float mx = INFINITY;
         if (i < rows) {
           mx = fmaxf(fmaxf(bars->wmax[0][i], bars->wmax[1][i]), fmaxf(bars->wmax[2][i], bars->wmax[3][i])) * scale;
-          mx = fmaxf(mx, kNoKey);  // (scores of -infinity alone)
+          mx = fmaxf(mx - kLift, kNoKey);  // (scores of -infinity alone)
           if (c.j > 0) {
             const float old = -bars->m[i];
             mx = fmaxf(mx, old);
@@ -359,38 +373,51 @@ __device__ __forceinline__ bool softmax_item(const Params& p, Cursor& c, const i
       tc_fence_after();
 #pragma unroll 1
       for (int q = 0; q < W; q += 8) {
-        uint32_t orr[8];
-        load_cols(base + 128 + q, orr);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) orr[i] = __float_as_uint(__uint_as_float(orr[i]) * bars->alpha[q + i]);
-        tmem_st8(base + 128 + q, orr);
+        for (int at = 128; at <= 128 + R; at += R) {
+          uint32_t orr[8];
+          load_cols(base + at + q, orr);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) orr[i] = __float_as_uint(__uint_as_float(orr[i]) * bars->alpha[q + i]);
+          tmem_st8(base + at + q, orr);
+        }
       }
       tmem_st_wait();
       tc_fence_before();
     }
 #pragma unroll
     for (int q = 0; q < W / 8; ++q) {
-      uint32_t pw[4];
+      uint32_t pw[4], pr[4];
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const float p0 = ex2(__uint_as_float(sr[q * 8 + 2 * e])), p1 = ex2(__uint_as_float(sr[q * 8 + 2 * e + 1]));
         const __half2 hp = __floats2half2_rn(p0, p1);
+        const float2 b = __half22float2(hp);
+        const float2 d = __ffma2_rn(b, make_float2(-kRest, -kRest), __fmul2_rn(make_float2(p0, p1), make_float2(kRest, kRest)));
+        const __half2 hr = __floats2half2_rn(d.x, d.y);
         pw[e] = past ? 0u : *reinterpret_cast<const uint32_t*>(&hp);
+        pr[e] = past ? 0u : *reinterpret_cast<const uint32_t*>(&hr);
       }
       *reinterpret_cast<uint4*>(prow + ((q ^ (key & 7)) << 4)) = make_uint4(pw[0], pw[1], pw[2], pw[3]);
+      *reinterpret_cast<uint4*>(prow + R / 64 * kTile + (((R % 64 / 8 + q) ^ (key & 7)) << 4)) =
+          make_uint4(pr[0], pr[1], pr[2], pr[3]);
     }
     fence_proxy_async_smem();
     __syncwarp();
     if (lane == 0) mbar_arrive(&bars->p_full);
   }
-  // The item's part: columns of [O^T; l], 64 values from two warps, the sum from the third.
+  // The item's part: columns of [O^T; l] and of the rest's, 64 values from two warps, the sum from the third.
   if (!warp_wait(&bars->p_empty, (g - 1) & 1, abort_flag, status, kSoftmax)) return false;
   tc_fence_after();
   if (quarter < 3) {
 #pragma unroll 1
     for (int q = 0; q < rows; q += 8) {
-      uint32_t orr[8];
+      uint32_t orr[8], rest[8];
       load_cols(base + 128 + q, orr);
+      load_cols(base + 128 + R + q, rest);
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        orr[i] = __float_as_uint(fmaf(__uint_as_float(rest[i]), 1.f / kRest, __uint_as_float(orr[i])));
       int at[8];
       *reinterpret_cast<int4*>(&at[0]) = *reinterpret_cast<const int4*>(&bars->at[q]);
       *reinterpret_cast<int4*>(&at[4]) = *reinterpret_cast<const int4*>(&bars->at[q + 4]);
@@ -419,7 +446,7 @@ __global__ void __launch_bounds__(kThreads, 2)
                             const Params p, int* status) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  // Queries of own items (two, G rows each), of a prefix item, K and V slots, P, ones. The matrix unit reads the
+  // Queries of own items (two, G rows each), of a prefix item, K and V slots, P and its rest, ones. The matrix unit reads the
   // rows of a query tile in sixteens; behind an own item's G rows it finds other data, which only reaches columns
   // of S^T and O^T that nobody reads.
   uint8_t* sQ = smem;
@@ -427,7 +454,7 @@ __global__ void __launch_bounds__(kThreads, 2)
   uint8_t* sK = sQp + kQTile;
   uint8_t* sV = sK + kKSlots * kTile;
   uint8_t* sP = sV + kVSlots * kTile;
-  uint8_t* s1 = sP + kTile;
+  uint8_t* s1 = sP + 2 * kTile;
   Bars* bars = reinterpret_cast<Bars*>(s1 + kOnes);
   volatile int* abort_flag = &bars->abort;
   const Sched& s = p.s;
@@ -569,7 +596,7 @@ __global__ void __launch_bounds__(kThreads, 2)
       __syncwarp();
     }
   } else if (warp == 6) {
-    const uint64_t dP0 = smem_desc_sw128(smem_u32(sP), 8192, 1024);
+    const uint64_t dP0 = smem_desc_sw128(smem_u32(sP), kTile, 1024);
     // A of the second product for slot 0 and keys 0-15: rows 0-63 are V^T, rows 64-127, one leading offset on, ones.
     // 16 keys (2 KB) or a slot further, the start moves up and the leading offset down by as much, both in units of 16.
     const uint64_t dV0 = smem_desc_sw128(smem_u32(sV), smem_u32(s1) - smem_u32(sV), 1024);
@@ -597,7 +624,7 @@ __global__ void __launch_bounds__(kThreads, 2)
       if (!warp_wait(&bars->p_full, tp & 1, abort_flag, status, kMma)) break;
       tc_fence_after();
       if (lane == 0) {
-        const uint32_t idesc = idesc_f16_f32(128, 0, true, true) | ((uint32_t)(c.rows(s) + 15) >> 4) << 18;
+        const uint32_t idesc = idesc_f16_f32(128, 0, true, true) | (uint32_t)rest_at(c.rows(s)) >> 3 << 18;  // both parts
         const uint64_t dv = dV0 + vs * (kSlot - (kSlot << 16));
 #pragma unroll
         for (int kk = 0; kk < BKV / 16; ++kk)
@@ -1031,7 +1058,7 @@ extern "C" int jx_attn_decode_prefix(const void* qkv, int64_t ld_qkv, const void
   p.q_own_bytes = G * 128;
   p.q_own_stride = (G + 7) / 8 * 1024;
   p.q_pre_bytes = p.s.nb * G * 128;
-  constexpr size_t kFixed = 1024 + pfx::kQTile + (pfx::kKSlots + pfx::kVSlots + 1) * pfx::kTile + pfx::kOnes + sizeof(pfx::Bars);
+  constexpr size_t kFixed = 1024 + pfx::kQTile + (pfx::kKSlots + pfx::kVSlots + 2) * pfx::kTile + pfx::kOnes + sizeof(pfx::Bars);
   static_assert(kFixed + 2 * 1024 + 1024 <= 233472 / 2, "two blocks an SM with up to eight heads a key / value head");
   const size_t smem = kFixed + 2 * p.q_own_stride;
   static std::atomic<uint64_t> done{0};
