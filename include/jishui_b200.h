@@ -294,7 +294,8 @@ int jx_distill_fwd(const void* logits16, int64_t rows, int vocab, int64_t ld, co
                    jx_stream_t stream);
 /* out16 = f16(g (alpha temperature (q_j - sum_{k: id_k = j} p_k) + (1 - alpha) (q1_j - [j = y]))) with
  * g = (*grad_loss) / (*count); zero rows where the target is ignored or invalid. out16 may be logits16 (with the
- * same row stride), but not overlap it otherwise. */
+ * same row stride), but not overlap it otherwise. Where a row's statistics exceed 64 in size (low temperatures, large
+ * logits), fp32 does not hold them to enough places, and its sums are taken again from the logits. */
 int jx_distill_bwd(const void* logits16, int64_t rows, int vocab, int64_t ld, const int64_t* teacher_ids,
                    const void* teacher_logits, int teacher_is_f16, int K, const int64_t* targets, int64_t ignore_index,
                    float temperature, float alpha, const float* stats, const float* grad_loss, const float* count,

@@ -229,7 +229,10 @@ __global__ void __launch_bounds__(NT, 1024 / NT) distill_fwd_kernel(const Params
     return;
   }
   if (tid == 0) rbad = 0;
-  float m = -INFINITY, s = 0.f, s1 = 0.f;
+  // Exponents are x ce - m ce in one rounding, but m ce has been rounded before: fix and fix1 make up for that in the sums (at
+  // m ce = 1e4 it is 5e-4 of them).
+  float m = -INFINITY, s = 0.f, s1 = 0.f, fix = 1.f, fix1 = 1.f;
+  const float ce = MODE == kPow1h ? kLog2e / 3.f : c;  // of the exponential that is taken
   for (int base = 0; base < nvec; base += NT * VPT) {
     uint4 v[VPT];
 #pragma unroll
@@ -259,8 +262,13 @@ __global__ void __launch_bounds__(NT, 1024 / NT) distill_fwd_kernel(const Params
         s1 *= ex2((m - nm) * kLog2e);
       }
       m = nm;
+      const float w = ex2(-fmaf(m, ce, -m * ce));
+      fix = MODE == kPow1h ? w * w : w;
+      if constexpr (MODE == kBoth)
+        fix1 = ex2(-fmaf(m, kLog2e, -m * kLog2e));
+      else if constexpr (kTwo)
+        fix1 = power<MODE>(w);
     }
-    const float ce = MODE == kPow1h ? kLog2e / 3.f : c;  // of the exponential that is taken
     const float mc = -m * ce, mc1 = -m * kLog2e;
     float a[4] = {0.f, 0.f, 0.f, 0.f}, b[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -277,8 +285,8 @@ __global__ void __launch_bounds__(NT, 1024 / NT) distill_fwd_kernel(const Params
           b[j] += power<MODE>(w0) + power<MODE>(w1);
       }
     }
-    s += (a[0] + a[1]) + (a[2] + a[3]);
-    if constexpr (kTwo) s1 += (b[0] + b[1]) + (b[2] + b[3]);
+    s = fmaf((a[0] + a[1]) + (a[2] + a[3]), fix, s);
+    if constexpr (kTwo) s1 = fmaf((b[0] + b[1]) + (b[2] + b[3]), fix1, s1);
   }
   const float wm = warp_max(m);
   if (m != -INFINITY) {
@@ -318,10 +326,69 @@ __global__ void __launch_bounds__(NT, 1024 / NT) distill_fwd_kernel(const Params
   finish_row(p, row, lse, lse1, slots, slots + p.K, rbad != 0, zy, row_loss, status);
 }
 
+// The maximum and the logarithms (base 2) of the sums of 2^((z - max) c) and (kTwo) 2^((z - max) log2 e) of a row, by a block.
+struct RowSums {
+  float m, l, l1;
+};
+
+template <int NT, bool kTwo>
+__device__ __noinline__ RowSums row_sums(const __half* z, int vocab, float c) {
+  __shared__ float red[3][NT / 32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nvec = (vocab + 7) / 8;
+  float m = -INFINITY;
+#pragma unroll 4
+  for (int i = threadIdx.x; i < nvec; i += NT) {
+    const uint4 v = load8(z, 8 * (int64_t)i, vocab, 0xfc00u);
+    const __half2* h = reinterpret_cast<const __half2*>(&v);
+    const __half2 hm = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
+    m = fmaxf(m, fmaxf(__low2float(hm), __high2float(hm)));
+  }
+  m = warp_max(m);
+  if (lane == 0) red[0][warp] = m;
+  __syncthreads();
+  m = warp_max(lane < NT / 32 ? red[0][lane] : -INFINITY);
+  float s = 0.f, s1 = 0.f;
+#pragma unroll 4
+  for (int i = threadIdx.x; i < nvec; i += NT) {
+    const uint4 v = load8(z, 8 * (int64_t)i, vocab, 0xfc00u);
+    const __half2* h = reinterpret_cast<const __half2*>(&v);
+    float a = 0.f, b = 0.f;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float2 f = __half22float2(h[j]);
+      a += ex2((f.x - m) * c) + ex2((f.y - m) * c);
+      if constexpr (kTwo) b += ex2((f.x - m) * kLog2e) + ex2((f.y - m) * kLog2e);
+    }
+    s += a, s1 += b;
+  }
+  s = warp_sum(s), s1 = warp_sum(s1);
+  if (lane == 0) red[1][warp] = s, red[2][warp] = s1;
+  __syncthreads();
+  s = warp_sum(lane < NT / 32 ? red[1][lane] : 0.f);
+  s1 = warp_sum(lane < NT / 32 ? red[2][lane] : 0.f);
+  return {m, log2f(s), log2f(s1)};
+}
+
+// The same of a row's K teacher logits at 2^((t - max) c), by every warp for itself.
+__device__ __noinline__ float2 slot_sums(const float* t, int K, float c) {
+  const int lane = threadIdx.x & 31;
+  float m = -INFINITY, s = 0.f;
+  for (int k = lane; k < K; k += 32) m = fmaxf(m, t[k]);
+  m = warp_max(m);
+  for (int k = lane; k < K; k += 32) s += ex2((t[k] - m) * c);
+  return make_float2(m, log2f(warp_sum(s)));
+}
+
+// Whether a log-sum-exp is so large that its rounding to fp32 shows in a weight: at 64 half a step is 2e-6 of the weight.
+__device__ __forceinline__ bool far_off(float lse) { return fabsf(lse) > 64.f && fabsf(lse) < INFINITY; }
+
 // The gradient. One block per row; the slots' logits are read before anything is stored (out may be the logits).
 // Every element gets the dense part, then the slots' elements and the target's are stored once more with
 // their own terms, each by the first slot that names it, so that each is rounded once.
 // (Its time is that of its reads and writes, 343 us for 16384 x 32000, with one exponential or two.)
+// A row whose logits are large (against the temperature) has its sums taken again from its logits, relative to their
+// maximum, which its statistics in fp32 cannot hold to enough places (a weight would be off by 1.5e-5 at temperature 0.1,
+// by 3e-3 at 0.001). That reads the row twice more: loss and gradient of 16384 x 32000 at temperature 0.1 600 -> 970 us.
 template <int NT, int VPT, bool kTwo>
 __global__ void __launch_bounds__(NT, 1024 / NT) distill_bwd_kernel(const Params p, const float* __restrict__ grad_loss,
                                                                     const float* __restrict__ count, __half* out,
@@ -362,11 +429,23 @@ __global__ void __launch_bounds__(NT, 1024 / NT) distill_bwd_kernel(const Params
     slot_z[K] = __half2float(z[y]);
     delta[K] = -gb;
   }
-  const float c = kLog2e / p.tau, b = -lse * kLog2e, b1 = -lse1 * kLog2e;
-  auto dense = [&](float x) {
-    const float w = ex2(fmaf(x, c, b));
-    if constexpr (kTwo) return fmaf(gb, ex2(fmaf(x, kLog2e, b1)), ga * w);
-    return (ga + gb) * w;  // tau = 1, or gb = 0
+  const float c = kLog2e / p.tau;
+  const bool far = far_off(lse) || far_off(lse1) || far_off(lse_t);
+  float m = 0.f, b = -lse * kLog2e, b1 = -lse1 * kLog2e;  // exponents (x - m) c + b and (x - m) log2 e + b1
+  if (far) {
+    const RowSums r = row_sums<NT, kTwo>(z, p.vocab, c);
+    m = r.m, b = -r.l, b1 = -r.l1;
+  }
+  auto both = [](float x) { return make_float2(x, x); };
+  auto dense = [&](float2 x) {
+    x = __fadd2_rn(x, both(-m));
+    const float2 e = __ffma2_rn(x, both(c), both(b));
+    const float2 w = make_float2(ex2(e.x), ex2(e.y));
+    if constexpr (kTwo) {
+      const float2 e1 = __ffma2_rn(x, both(kLog2e), both(b1));
+      return __ffma2_rn(both(gb), make_float2(ex2(e1.x), ex2(e1.y)), __fmul2_rn(both(ga), w));
+    }
+    return __fmul2_rn(both(ga + gb), w);  // tau = 1, or gb = 0
   };
   for (int base = 0; base < nvec; base += NT * VPT) {
     uint4 v[VPT];
@@ -374,9 +453,15 @@ __global__ void __launch_bounds__(NT, 1024 / NT) distill_bwd_kernel(const Params
     for (int i = 0; i < VPT; ++i) v[i] = load8(z, 8 * (int64_t)(base + i * NT + tid), p.vocab, 0xfc00u);
     if (base == 0) {
       __syncthreads();  // every slot's logit has been read
+      float2 ts = make_float2(0.f, 0.f);
+      if (far) {
+        ts = slot_sums(delta, K, c);
+        __syncthreads();
+      }
       for (int k = tid; k < K; k += NT) {
         const float t = delta[k];
-        delta[k] = t == -INFINITY ? 0.f : -ga * exp2f((t / p.tau - lse_t) * kLog2e);
+        const float e = far && fabsf(lse_t) < INFINITY ? fmaf(t - ts.x, c, -ts.y) : (t / p.tau - lse_t) * kLog2e;
+        delta[k] = t == -INFINITY ? 0.f : -ga * exp2f(e);
       }
       for (int k = tid; k <= K; k += NT) {
         const int id = slot_id[k];
@@ -390,8 +475,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) distill_bwd_kernel(const Params
       __half2* h = reinterpret_cast<__half2*>(&v[i]);
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const float2 f = __half22float2(h[j]);
-        h[j] = __floats2half2_rn(dense(f.x), dense(f.y));
+        h[j] = __float22half2_rn(dense(__half22float2(h[j])));
       }
       if (first + 8 <= p.vocab) {
         *reinterpret_cast<uint4*>(o + first) = v[i];
@@ -420,7 +504,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) distill_bwd_kernel(const Params
         d += delta[j];
       }
     }
-    if (mine) o[id] = __float2half_rn(dense(slot_z[k]) + d);
+    if (mine) o[id] = __float2half_rn(dense(both(slot_z[k])).x + d);
   }
 }
 

@@ -243,3 +243,60 @@ def test_refusals(ops):
         ops.distill_bwd(x, ids, t, y, stats, one, one, out=torch.empty(4, 264, device="cuda", dtype=torch.float16))
     with pytest.raises(ValueError, match="one value"):
         ops.distill_bwd(x, ids, t, y, stats, rows, one)
+
+
+def _cold_rows(V, K, tau, scales, shift, seed):
+    """Rows whose teacher has the student's own largest logits, at several sizes of the logits, with ties at the top."""
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    x = torch.randn(len(scales), (V + 7) // 8 * 8, device="cuda", generator=g) * torch.tensor(scales, device="cuda")[:, None] + shift
+    x = x.half()
+    x = x[:, :V]
+    top = x.float().argmax(1)
+    rows = torch.arange(len(scales), device="cuda")
+    x[rows, (top + 1) % V] = x[rows, top]  # (a tie: the two largest weigh the same at any temperature)
+    t, ids = x.float().topk(K, dim=1)
+    y = torch.randint(0, V, (len(scales),), device="cuda", generator=g)
+    return x, ids, t, y
+
+
+def _define_by_logs(x, ids, t, y, tau, alpha, scale):
+    """_define for rows that use every slot and ids that differ, from log-softmaxes: no weight underflows to 0 log 0."""
+    x, rows = x.double(), torch.arange(x.shape[0], device="cuda")
+    lp, lq, l1 = (torch.log_softmax(v, 1) for v in (t.double() / tau, x / tau, x))
+    loss = alpha * tau ** 2 * (lp.exp() * (lp - lq.gather(1, ids))).sum(1) - (1 - alpha) * l1[rows, y]
+    grad = alpha * tau * lq.exp() + (1 - alpha) * l1.exp()
+    mag = grad.clone().scatter_add_(1, ids, alpha * tau * lp.exp())
+    grad.scatter_add_(1, ids, -alpha * tau * lp.exp())
+    grad[rows, y] -= 1 - alpha
+    mag[rows, y] += 1 - alpha
+    return loss, grad * scale, mag * scale
+
+
+@pytest.mark.parametrize("V,K,R", [(1000, 16, 8), (24000, 64, 8), (24000, 5, 320)])
+@pytest.mark.parametrize("tau,alpha,shift", [(0.001, 1.0, 0.0), (0.01, 1.0, 3.0), (0.01, 0.5, 0.0), (0.1, 1.0, -9.0), (0.1, 0.7, 20.0),
+                                             (1.0, 1.0, 2000.0), (1.0, 0.5, -30000.0), (1.5, 0.5, 5000.0), (2.0, 0.4, -9000.0),
+                                             (3.0, 0.4, 700.0), (7.0, 0.4, 700.0)])
+@pytest.mark.parametrize("other", [False, True])
+def test_low_temperatures_and_large_logits(ops, V, K, R, tau, alpha, shift, other):
+    """Logits that are large against the temperature: the result is as good as for small ones, also where the teacher is
+    the student and every term cancels. A loss may be off by what the sums of both softmaxes may (5e-6 each in the
+    logarithm), and by what fp32 weights leave of the slots' differences (2^-17 of them: an exponential's argument up to
+    40 rounded to fp32, and sums); the gradient by _check's bounds."""
+    scales = [(0.01, 0.1, 0.5, 1.0, 2.0, 3.0, 5.0, 7.0)[r % 8] for r in range(R)]
+    x, ids, t, y = _cold_rows(V, K, tau, scales, shift, seed=V + K)
+    if other:  # a teacher of its own, by a few steps of temperature
+        g = torch.Generator(device="cuda").manual_seed(1)
+        t = t + torch.randn(t.shape, device="cuda", generator=g) * tau
+    want, gwant, mag = _define_by_logs(x, ids, t, y, tau, alpha, 512.0 / R)
+    stats, rows = ops.distill_fwd(x, ids, t, y, temperature=tau, alpha=alpha)
+    td, zd = t.double(), x.gather(1, ids).double()
+    slots = (torch.softmax(td / tau, 1) * (td - zd).abs()).sum(1) / tau
+    tol = alpha * tau ** 2 * (1e-5 + 2 ** -17 * slots) + (1 - alpha) * 5e-6 + 2 ** -24 * want.abs()
+    err = (rows.double() - want).abs()
+    assert bool((err <= tol).all()), float((err / tol).max())
+    for out in (torch.empty_like(x), None):
+        got = ops.distill_bwd(x, ids, t, y, stats, torch.full((1,), 512.0, device="cuda"), torch.full((1,), float(R), device="cuda"),
+                              temperature=tau, alpha=alpha, out=out)
+        gtol = 2 ** -11 * gwant.abs() + 2 ** -25 + 1e-5 * mag
+        gerr = (got.double() - gwant).abs()
+        assert bool((gerr <= gtol).all()), float((gerr / gtol).max())
