@@ -47,6 +47,14 @@ def _prefill(model: JishuiForCausalLM, fl, ctx: list[int], keys, values) -> torc
     return ws.xs[L % 2][T - 1:T]
 
 
+def _flat_on(model: JishuiForCausalLM, device: torch.device):
+    """The model's flat weight storage, which must be on the device of what is kept for it."""
+    fl = model.flat()
+    if fl.device != device:
+        raise RuntimeError(f"the model has moved to {fl.device} since this was built for it on {device}")
+    return fl
+
+
 class KVCacheDecoder:
     """Per-model decoding state: keys / values of the last context for every layer (batch 1). The cache is
     rebuilt when the context does not extend the previous one or the weights changed since."""
@@ -55,7 +63,7 @@ class KVCacheDecoder:
         c = model.config
         self.model = model
         self.max_len = max_len or c.max_position_embeddings
-        dev = next(model.parameters()).device
+        dev = self.device = next(model.parameters()).device
         if dev.type != "cuda":
             raise RuntimeError("KVCacheDecoder: the model must be on a CUDA device (there is no CPU path)")
         L, d, F, H, hd = c.num_hidden_layers, c.hidden_size, c.intermediate_size, c.num_attention_heads, c.head_dim
@@ -101,7 +109,7 @@ class KVCacheDecoder:
             for p in range(n, len(ctx)):
                 self._decode(ctx[p], p)
         else:
-            fl = self.model.flat()
+            fl = _flat_on(self.model, self.device)
             fl.refresh_f16()
             self._fl = fl
             self._prefill(ctx)
@@ -168,9 +176,9 @@ class KVCacheDecoder:
 
 def next_token_logits(model: JishuiForCausalLM, context: Sequence[int], device=None) -> np.ndarray:
     """Drop-in for generate_torch.next_token_logits: the same result, with a KV cache kept on the model
-    across calls."""
+    across calls (a model on another device gets a new one)."""
     dec = getattr(model, "_kv_decoder", None)
-    if dec is None:
+    if dec is None or dec.device != next(model.parameters()).device:
         dec = model._kv_decoder = KVCacheDecoder(model)
     return dec.next_token_logits(context)
 
@@ -201,7 +209,7 @@ class PromptSampler:
         self.max_len = max_len or c.max_position_embeddings
         if n < 1 or max_new_tokens < 1 or self.max_len > c.max_position_embeddings:
             raise ValueError("PromptSampler: n and max_new_tokens must be positive, max_len within the model's context")
-        dev = next(model.parameters()).device
+        dev = self.device = next(model.parameters()).device
         if dev.type != "cuda":
             raise RuntimeError("PromptSampler: the model must be on a CUDA device (there is no CPU path)")
         L, d, F, hd = c.num_hidden_layers, c.hidden_size, c.intermediate_size, c.head_dim
@@ -280,7 +288,7 @@ class PromptSampler:
     def _start(self, ctx: list[int], end: int) -> None:
         """Prefills the prompt; self.logits then holds its next-token logits in every row."""
         m, c = self.model, self.model.config
-        fl = self._fl = m.flat()
+        fl = self._fl = _flat_on(m, self.device)
         fl.refresh_f16()
         self.prefix_len = len(ctx)
         x_last = _prefill(m, fl, ctx, self.kp, self.vp)
@@ -352,8 +360,9 @@ class PromptSampler:
 
 def generate(model: JishuiForCausalLM, prompt: Sequence[int], n: int = 1, max_new_tokens: int = 256, **settings) -> Completions:
     """`n` completions of `prompt` (PromptSampler.generate has the settings), with a sampler kept on the model across
-    calls of the same n and number of new tokens."""
+    calls of the same n and number of new tokens while the model stays on its device."""
     sampler = getattr(model, "_prompt_sampler", None)
-    if sampler is None or (sampler.n, sampler.max_new) != (n, max_new_tokens):
+    here = next(model.parameters()).device
+    if sampler is None or (sampler.n, sampler.max_new, sampler.device) != (n, max_new_tokens, here):
         sampler = model._prompt_sampler = PromptSampler(model, n, max_new_tokens)
     return sampler.generate(prompt, **settings)

@@ -122,3 +122,46 @@ def test_prefix_schedule_gives_every_tile_to_one_block():
         room = min(NT, -(-(NT - 1) // per) + 1)
         for u in range(units):
             assert block_of(u * NT + NT - 1) - block_of(u * NT) + 1 <= room
+
+
+@pytest.mark.parametrize("what", ["generate", "next_token_logits"])
+def test_decoding_state_follows_the_model_to_another_device(monkeypatch, what):
+    """What is kept on the model between calls belongs to a device: on another one it is built anew."""
+    from midstream_llm_b200 import decode
+    made = []
+
+    class Kept:
+        def __init__(self, model, n=0, max_new=0):
+            self.n, self.max_new, self.device = n, max_new, next(model.parameters()).device
+            made.append(self.device.type)
+
+        def generate(self, prompt, **settings):
+            return self
+
+        def next_token_logits(self, context):
+            return self
+
+    monkeypatch.setattr(decode, "PromptSampler", Kept)
+    monkeypatch.setattr(decode, "KVCacheDecoder", Kept)
+    model = torch.nn.Linear(2, 2)
+    run = {"generate": lambda: decode.generate(model, [1], n=2, max_new_tokens=4),
+           "next_token_logits": lambda: decode.next_token_logits(model, [1])}[what]
+    first = run()
+    assert run() is first
+    model.to("meta")
+    second = run()
+    assert second is not first and second.device.type == "meta" and run() is second
+    assert made == ["cpu", "meta"]
+
+
+def test_decoding_state_refuses_a_model_that_has_moved():
+    from types import SimpleNamespace
+
+    from midstream_llm_b200 import decode
+    fl = SimpleNamespace(device=torch.device("cpu"))
+    model = SimpleNamespace(flat=lambda: fl)
+    assert decode._flat_on(model, torch.device("cpu")) is fl
+    sampler = object.__new__(decode.PromptSampler)
+    sampler.model, sampler.device = SimpleNamespace(flat=lambda: fl, config=None), torch.device("cuda:1")
+    with pytest.raises(RuntimeError, match="moved to cpu"):
+        sampler._start([1], -1)
