@@ -217,7 +217,7 @@ int jx_attn_decode(const void* qkv, int64_t ld_qkv, void* kcache, void* vcache, 
  * sequence (its output row is zero, its cache untouched), more than max_len does too and sets the device status
  * word to 204. Cache rows at and past lens[b] are never used and, but for the appended one, never written.
  * workspace: caller scratch of jx_attn_decode_prefix_workspace_bytes (-1 for a bad shape), with the same sizes;
- * calls that may overlap need their own. head_dim must be 64. Results repeat bit for bit. */
+ * calls that may overlap need their own. head_dim must be 64, scale at least 0. Results repeat bit for bit. */
 int64_t jx_attn_decode_prefix_workspace_bytes(int B, int H, int Hkv, int64_t prefix_len, int64_t max_len);
 int jx_attn_decode_prefix(const void* qkv, int64_t ld_qkv, const void* kprefix, const void* vprefix, int64_t ld_prefix,
                           int64_t prefix_len, void* kcache, void* vcache, int64_t ld_cache, int64_t cache_batch_stride,

@@ -1012,6 +1012,8 @@ extern "C" int jx_attn_decode_prefix(const void* qkv, int64_t ld_qkv, const void
                                      jx_stream_t stream) {
   const char* name = "jx_attn_decode_prefix";
   JX_CHECK_ARG(Dh == 64, "%s: head_dim must be 64 (got %d)", name, Dh);
+  // (The row maximum is taken before the scale.)
+  JX_CHECK_ARG(scale >= 0.f && scale <= 1e30f, "%s: scale must be a number of at least 0 (got %g)", name, scale);
   JX_CHECK_ARG(qkv && kcache && vcache && lens && workspace && out && (prefix_len == 0 || (kprefix && vprefix)),
                "%s: NULL argument", name);
   pfx::Params p{};

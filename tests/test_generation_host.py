@@ -165,3 +165,10 @@ def test_decoding_state_refuses_a_model_that_has_moved():
     sampler.model, sampler.device = SimpleNamespace(flat=lambda: fl, config=None), torch.device("cuda:1")
     with pytest.raises(RuntimeError, match="moved to cpu"):
         sampler._start([1], -1)
+
+
+@pytest.mark.parametrize("scale", [-0.125, float("nan"), float("inf"), -float("inf")])
+def test_prefix_attention_refuses_a_scale_without_order(scale):
+    from midstream_llm_b200 import _lib
+    with pytest.raises(_lib.JxError, match="scale"):
+        _call("jx_attn_decode_prefix", *_prefix(scale=scale))
