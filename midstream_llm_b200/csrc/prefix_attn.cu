@@ -958,7 +958,8 @@ __global__ void __launch_bounds__(NT, (G <= 2 ? 640 : G == 3 ? 512 : 384) / NT) 
 // The schedule, from sizes and the SM count alone.
 bool plan(int B, int H, int Hkv, int64_t prefix_len, int64_t max_len, Sched* s, int* grid) {
   if (B <= 0 || Hkv <= 0 || H <= 0 || H % Hkv || H / Hkv > kRows || prefix_len < 0 || max_len <= 0) return false;
-  if (prefix_len > (1 << 28) || max_len > (1 << 28) || (int64_t)B * H > (1 << 24)) return false;
+  // (Columns of a row of qkv are counted in 32 bits.)
+  if (prefix_len > (1 << 28) || max_len > (1 << 28) || (int64_t)B * H > (1 << 24) || H > (1 << 22)) return false;
   const int blocks = 2 * num_sms();
   s->B = B, s->H = H, s->Hkv = Hkv, s->G = H / Hkv;
   s->nb = std::min(kRows / s->G, B);
@@ -1021,13 +1022,14 @@ extern "C" int jx_attn_decode_prefix(const void* qkv, int64_t ld_qkv, const void
   JX_CHECK_ARG(pfx::plan(B, H, Hkv, prefix_len, max_len, &p.s, &grid),
                "%s: bad shape B %d, H %d, Hkv %d (at most %d query heads per key head), prefix %lld, max_len %lld", name, B, H,
                Hkv, pfx::kRows, (long long)prefix_len, (long long)max_len);
-  const int G = p.s.G, width = (H + 2 * Hkv) * 64;
+  const int G = p.s.G;
+  const int64_t width = (H + 2 * (int64_t)Hkv) * 64, own_width = (int64_t)Hkv * 64;
   JX_CHECK_ARG(aligned16(qkv) && aligned16(kcache) && aligned16(vcache) && aligned16(workspace) &&
                    aligned16(kprefix) && aligned16(vprefix) && ((uintptr_t)out & 3) == 0,
                "%s: operands must be 16-byte aligned", name);
-  JX_CHECK_ARG(ld_qkv % 8 == 0 && ld_qkv >= width && ld_out % 2 == 0 && ld_out >= H * 64 && ld_cache % 8 == 0 &&
-                   ld_cache >= Hkv * 64 && cache_batch_stride % 8 == 0 && cache_batch_stride >= 0 &&
-                   (prefix_len == 0 || (ld_prefix % 8 == 0 && ld_prefix >= Hkv * 64)),
+  JX_CHECK_ARG(ld_qkv % 8 == 0 && ld_qkv >= width && ld_out % 2 == 0 && ld_out >= (int64_t)H * 64 && ld_cache % 8 == 0 &&
+                   ld_cache >= own_width && cache_batch_stride % 8 == 0 && cache_batch_stride >= 0 &&
+                   (prefix_len == 0 || (ld_prefix % 8 == 0 && ld_prefix >= own_width)),
                "%s: row strides must be multiples of 8 and hold a row", name);
   // Queries as [sequence][head][64]: one box holds G heads of one sequence, or of a row tile's sequences.
   CUtensorMap qp{}, qo{}, kp{}, vp{}, kc{}, vc{};  // those of what there is

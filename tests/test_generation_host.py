@@ -172,3 +172,11 @@ def test_prefix_attention_refuses_a_scale_without_order(scale):
     from midstream_llm_b200 import _lib
     with pytest.raises(_lib.JxError, match="scale"):
         _call("jx_attn_decode_prefix", *_prefix(scale=scale))
+
+
+@pytest.mark.parametrize("H", [1 << 22, 1 << 23, 1 << 24])
+def test_prefix_attention_counts_the_columns_of_many_heads(H):
+    """Rows of 2^30 elements and more, whose count does not fit 32 bits: too short a stride is seen, more heads are refused."""
+    from midstream_llm_b200 import _lib
+    with pytest.raises(_lib.JxError, match="strides|bad shape"):
+        _call("jx_attn_decode_prefix", *_prefix(B=1, H=H, kv=H, ld_qkv=64, ld_p=H * 64, ld_c=H * 64, ld_out=H * 64, P=4, max_len=4))
