@@ -213,7 +213,7 @@ int jx_attn_decode(const void* qkv, int64_t ld_qkv, void* kcache, void* vcache, 
  * its own k / v, appended to the cache at lens[b]-1. qkv rows are q (H heads) | k (Hkv) | v (Hkv); H must be a
  * multiple of Hkv (at most 64 times), query head h reads key / value head h / (H / Hkv). kprefix / vprefix:
  * [prefix_len, Hkv*64], row stride ld_prefix (prefix_len may be 0); kcache / vcache: row stride ld_cache, sequence
- * stride cache_batch_stride, room for max_len rows per sequence. lens: device int32 [B]; 0 or less marks an idle
+ * stride cache_batch_stride, room for max_len rows per sequence, none of which is another's. lens: device int32 [B]; 0 or less marks an idle
  * sequence (its output row is zero, its cache untouched), more than max_len does too and sets the device status
  * word to 204. Cache rows at and past lens[b] are never used and, but for the appended one, never written.
  * workspace: caller scratch of jx_attn_decode_prefix_workspace_bytes (-1 for a bad shape), with the same sizes;

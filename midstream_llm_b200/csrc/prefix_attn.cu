@@ -1031,6 +1031,10 @@ extern "C" int jx_attn_decode_prefix(const void* qkv, int64_t ld_qkv, const void
                    ld_cache >= own_width && cache_batch_stride % 8 == 0 && cache_batch_stride >= 0 &&
                    (prefix_len == 0 || (ld_prefix % 8 == 0 && ld_prefix >= own_width)),
                "%s: row strides must be multiples of 8 and hold a row", name);
+  // Sequence by sequence or position by position; each appends to its own.
+  JX_CHECK_ARG(B == 1 || (cache_batch_stride >= own_width && (cache_batch_stride >= (max_len - 1) * ld_cache + own_width ||
+                                                              ld_cache >= (B - 1) * cache_batch_stride + own_width)),
+               "%s: the sequences' caches overlap", name);
   // Queries as [sequence][head][64]: one box holds G heads of one sequence, or of a row tile's sequences.
   CUtensorMap qp{}, qo{}, kp{}, vp{}, kc{}, vc{};  // those of what there is
   const uint64_t qdims[3] = {64, (uint64_t)H, (uint64_t)B}, qstr[2] = {128, (uint64_t)ld_qkv * 2};

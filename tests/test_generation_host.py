@@ -180,3 +180,11 @@ def test_prefix_attention_counts_the_columns_of_many_heads(H):
     from midstream_llm_b200 import _lib
     with pytest.raises(_lib.JxError, match="strides|bad shape"):
         _call("jx_attn_decode_prefix", *_prefix(B=1, H=H, kv=H, ld_qkv=64, ld_p=H * 64, ld_c=H * 64, ld_out=H * 64, P=4, max_len=4))
+
+
+@pytest.mark.parametrize("B,bs,ld_c", [(2, 0, 256), (2, 8, 256), (2, 248, 512), (2, 256, 256), (3, 256, 512), (2, 25592, 256),
+                                       (2, 12800, 256)])
+def test_prefix_attention_refuses_caches_that_overlap(B, bs, ld_c):
+    from midstream_llm_b200 import _lib
+    with pytest.raises(_lib.JxError, match="overlap"):
+        _call("jx_attn_decode_prefix", *_prefix(B=B, bs=bs, ld_c=ld_c))
