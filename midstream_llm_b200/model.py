@@ -609,6 +609,16 @@ class JishuiForCausalLM(nn.Module):
         self._norm_bwd(ws.dh, x_in, A.mean1, A.rstd1, w["g1"], w["gg1"], w["gb1"], acc, ws.dxmid, ws.dx, ws.norm_part)
 
 
+def _claim_logits(ctx) -> Workspace:
+    """The forward's workspace, for the one backward whose logit gradient takes the logits' place."""
+    if ctx.model._gen != ctx.gen:
+        raise RuntimeError("another training forward ran before this backward; activations were overwritten")
+    if ctx.spent:
+        raise RuntimeError("a second backward of the same loss: the first one overwrote the logits")
+    ctx.spent = True
+    return ctx.ws
+
+
 class _LossFn(torch.autograd.Function):
     """Whole-model forward + fused CE; backward writes every parameter's .grad
     directly (the flat gradient buffer) and returns None for the parameters."""
@@ -619,16 +629,14 @@ class _LossFn(torch.autograd.Function):
         tg = targets.reshape(-1)
         out = model._ce_forward(ws, tg, ignore_index)
         model._gen += 1
-        ctx.model, ctx.gen, ctx.ws = model, model._gen, ws
+        ctx.model, ctx.gen, ctx.ws, ctx.spent = model, model._gen, ws, False
         ctx.ignore_index = ignore_index
         ctx.save_for_backward(ids, tg, out)
         return out[2].clone()
 
     @staticmethod
     def backward(ctx, grad_loss):
-        model, ws = ctx.model, ctx.ws
-        if model._gen != ctx.gen:
-            raise RuntimeError("another training forward ran before this backward; activations were overwritten")
+        model, ws = ctx.model, _claim_logits(ctx)
         ids, tg, out = ctx.saved_tensors
         g = grad_loss.detach().to(torch.float32).reshape(1).contiguous()
         ops.ce_bwd(ws.logits, tg, ws.ce_lse, g, out[1:2], ctx.ignore_index)
@@ -643,16 +651,14 @@ class _DistillFn(torch.autograd.Function):
     def forward(ctx, model: JishuiForCausalLM, ids, tg, t_ids, t_logits, temperature, alpha, ignore_index, *params):
         ws, stats, out = model._distill_forward(ids, True, tg, t_ids, t_logits, temperature, alpha, ignore_index)
         model._gen += 1
-        ctx.model, ctx.gen, ctx.ws = model, model._gen, ws
+        ctx.model, ctx.gen, ctx.ws, ctx.spent = model, model._gen, ws, False
         ctx.settings = dict(temperature=temperature, alpha=alpha, ignore_index=ignore_index)
         ctx.save_for_backward(ids, tg, t_ids, t_logits, stats, out)
         return out[2].clone()
 
     @staticmethod
     def backward(ctx, grad_loss):
-        model, ws = ctx.model, ctx.ws
-        if model._gen != ctx.gen:
-            raise RuntimeError("another training forward ran before this backward; activations were overwritten")
+        model, ws = ctx.model, _claim_logits(ctx)
         ids, tg, t_ids, t_logits, stats, out = ctx.saved_tensors
         g = grad_loss.detach().to(torch.float32).reshape(1).contiguous()
         ops.distill_bwd(ws.logits, t_ids, t_logits, tg, stats, g, out[1:2], **ctx.settings)

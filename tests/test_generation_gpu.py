@@ -207,3 +207,17 @@ def test_generate_refuses_settings_without_a_meaning():
     for bad in (dict(temperature=-1.0), dict(temperature=[1.0, -0.5]), dict(top_p=float("nan")), dict(min_p=[0.0, float("nan")])):
         with pytest.raises(ValueError, match="bad"):
             generate(mine, [1, 2, 3], n=2, max_new_tokens=4, **bad)
+
+
+@pytest.mark.parametrize("distill", [False, True])
+def test_a_second_backward_of_the_same_loss_is_refused(distill):
+    """The first one leaves the logits' gradient in their place."""
+    _, mine = _pairs()
+    x, y = _batch(mine.config, 1, 256, 1)
+    t, ids = mine.top_logits(x, 8)
+    loss = mine.distill_loss(x, y, ids, t, temperature=2.0) if distill else mine.loss(x, y)
+    loss.backward(retain_graph=True)
+    first = mine.embed_tokens.weight.grad.clone()
+    with pytest.raises(RuntimeError, match="backward"):
+        loss.backward()
+    assert torch.equal(mine.embed_tokens.weight.grad, first)
