@@ -251,6 +251,8 @@ class PromptSampler:
         ctx = [int(t) for t in prompt]
         if not ctx:
             raise ValueError("empty prompt")
+        if min(ctx) < 0 or max(ctx) >= self.model.config.vocab_size:
+            raise ValueError(f"prompt tokens must lie in the vocabulary of {self.model.config.vocab_size}")
         if not 1 <= steps <= self.max_new or len(ctx) + steps > self.max_len:
             raise ValueError(f"{len(ctx)} prompt tokens and {steps} new ones exceed the sampler's {self.max_len} positions "
                              f"or its {self.max_new} new tokens")

@@ -221,3 +221,15 @@ def test_a_second_backward_of_the_same_loss_is_refused(distill):
     with pytest.raises(RuntimeError, match="backward"):
         loss.backward()
     assert torch.equal(mine.embed_tokens.weight.grad, first)
+
+
+@pytest.mark.parametrize("bad", [[5, -1], [5, 1 << 30]])
+def test_generate_refuses_tokens_outside_the_vocabulary(bad):
+    from midstream_llm_b200 import _lib, generate
+    _, mine = _pairs()
+    _lib.device_status()
+    with pytest.raises(ValueError, match="vocabulary"):
+        generate(mine, bad, n=2, max_new_tokens=4)
+    with pytest.raises(ValueError, match="vocabulary"):
+        generate(mine, [5, mine.config.vocab_size], n=2, max_new_tokens=4)
+    assert _lib.device_status() == 0
