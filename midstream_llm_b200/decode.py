@@ -276,7 +276,7 @@ class PromptSampler:
             self._advance()
             taken += 1
         tokens, logprobs = self.tokens[:taken].t().contiguous(), self.logprobs[:taken].t().contiguous()
-        if bool((tokens < 0).any()):
+        if bool(logprobs.isnan().any()):
             raise FloatingPointError("non-finite logits")
         lengths = [taken] * self.n
         if eos_token_id is not None:
@@ -315,8 +315,10 @@ class PromptSampler:
         """Draws the next token of every row from self.logits and records it (graph-capturable: no host reads)."""
         torch.index_select(self.uniforms, 0, self.step, out=self.u.view(1, -1))
         ops.sample(self.logits, self.u, **self.settings, tokens=self.tok, logprobs=self.logp)
-        # An ended completion repeats its end token.
-        self.tok.copy_(torch.where(self.done, self.end, self.tok))
+        # An ended completion repeats its end token. A row without a token to draw (-1; its log probability is NaN) goes on
+        # with token 0 until the call ends with an error.
+        torch.where(self.done, self.end, self.tok, out=self.tok)
+        self.tok.clamp_(min=0)
         self.logp.masked_fill_(self.done, 0.0)
         self.tokens.index_copy_(0, self.step, self.tok.view(1, -1))
         self.logprobs.index_copy_(0, self.step, self.logp.view(1, -1))

@@ -233,3 +233,16 @@ def test_generate_refuses_tokens_outside_the_vocabulary(bad):
     with pytest.raises(ValueError, match="vocabulary"):
         generate(mine, [5, mine.config.vocab_size], n=2, max_new_tokens=4)
     assert _lib.device_status() == 0
+
+
+def test_non_finite_logits_leave_no_status_behind():
+    """Rows without a token to draw end the call with an error; what is fed meanwhile is a token of the vocabulary."""
+    from midstream_llm_b200 import _lib, generate
+    _, mine = _pairs()
+    with torch.no_grad():
+        mine.norm.weight[0] = float("nan")
+    for end in (None, 0, 7):
+        _lib.device_status()
+        with pytest.raises(FloatingPointError, match="non-finite"):
+            generate(mine, [5, 6], n=2, max_new_tokens=6, eos_token_id=end)
+        assert _lib.device_status() == 0
