@@ -87,7 +87,6 @@ class KVCacheDecoder:
         self._slot = 0
         self.use_graph = True
         self._graph = None
-        self._graph_key = None
         self.context: list[int] = []
         self._generation = -1  # weights generation the cache was built with
         self._fl = None        # the model's flat weight storage the cache and graph were built with
@@ -111,7 +110,8 @@ class KVCacheDecoder:
         else:
             fl = _flat_on(self.model, self.device)
             fl.refresh_f16()
-            self._fl = fl
+            if fl is not self._fl:
+                self._fl, self._graph = fl, None  # the captured step reads the old storage
             self._prefill(ctx)
         self.context = ctx
         self._generation = fl.generation
@@ -129,7 +129,7 @@ class KVCacheDecoder:
 
     def _decode(self, token: int, p: int) -> None:
         """One new token at position p: a replay of the captured step (token and position are device inputs),
-        or an eager step that also captures the graph when there is none for the current weights buffers."""
+        or an eager step that also captures the graph when there is none (for the current weights storage)."""
         j = self._slot % self.host_in.shape[0]
         if j == 0 and self._slot:
             torch.cuda.current_stream().synchronize()  # every slot's copy has landed before the ring wraps
@@ -137,8 +137,7 @@ class KVCacheDecoder:
         self.host_in[j, 0], self.host_in[j, 1] = token, p
         self.tok.copy_(self.host_in[j, :1], non_blocking=True)
         self.pos.copy_(self.host_in[j, 1:], non_blocking=True)
-        key = id(self._fl)
-        if self._graph is not None and self._graph_key == key:
+        if self._graph is not None:
             self._graph.replay()
             return
         self._step()  # eager (and the first use of every kernel of the step, outside any capture)
@@ -146,7 +145,7 @@ class KVCacheDecoder:
             g = torch.cuda.CUDAGraph()
             with torch.cuda.graph(g):
                 self._step()
-            self._graph, self._graph_key = g, key
+            self._graph = g
 
     def _step(self) -> None:
         """The decode step on device inputs self.tok / self.pos (graph-capturable: no host reads)."""

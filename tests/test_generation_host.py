@@ -188,3 +188,26 @@ def test_prefix_attention_refuses_caches_that_overlap(B, bs, ld_c):
     from midstream_llm_b200 import _lib
     with pytest.raises(_lib.JxError, match="overlap"):
         _call("jx_attn_decode_prefix", *_prefix(B=B, bs=bs, ld_c=ld_c))
+
+
+def test_a_captured_step_goes_with_the_weight_storage_it_reads():
+    """A storage that takes the place (and may take the address) of the one that a step was captured with ends that step's use."""
+    from types import SimpleNamespace
+
+    from midstream_llm_b200 import decode
+    new = lambda: SimpleNamespace(device=torch.device("cpu"), generation=0, refresh_f16=lambda: None)  # noqa: E731
+    model = SimpleNamespace(_flat=None)
+    model.flat = lambda: model._flat
+    dec = object.__new__(decode.KVCacheDecoder)
+    dec.model, dec.device, dec.max_len, dec.logits = model, torch.device("cpu"), 8, torch.zeros(1, 4)
+    dec.context, dec._fl, dec._generation, dec._graph = [], None, -1, None
+    dec._prefill = lambda ctx: None
+    model._flat = new()
+    dec.next_token_logits([1, 2])
+    dec._graph = object()
+    kept = dec._graph
+    dec.next_token_logits([3])  # another prompt, the same storage
+    assert dec._graph is kept
+    model._flat = new()
+    dec.next_token_logits([3])
+    assert dec._graph is None and dec._fl is model._flat
