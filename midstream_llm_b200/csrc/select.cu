@@ -450,11 +450,11 @@ constexpr int kGroups = 4096;    // groups of 256 elements of a whole row: vocab
 constexpr int kShort = 8192;     // rows up to here get small blocks, whose lists always hold them
 constexpr double kUnit = 4398046511104.0;  // 2^42: weights of a row of 2^20 elements sum to at most 2^62
 constexpr int kExpTab = 256;
-// Bound of the relative error of the weight below a limit: ex2.approx 2^-22, its argument rounded to fp32 2^-20 ln 2 up to
-// 2^5 octaves under the maximum and twice that up to 2^6 (further down nothing counts), the rounded factor c over
-// eight octaves about the place where it is made up for 2^-24 8 ln 2, three additions of fp32 numbers 3 2^-24;
-// everything after that is added in 64 bits. Together below 2.2e-6.
-constexpr double kTailError = 4e-6;
+// Bound of the error of the weight below a limit, relative: ex2.approx 2^-22; its argument, up to 2^5 octaves under the
+// maximum, rounded to fp32, 2^-20 ln 2; the rounded factor c, made up for at one place, at most 2^5 octaves from there, 2^-24
+// 2^5 ln 2; three additions of fp32 numbers, 3 2^-24; all that follows is added in 64 bits: together below 2.4e-6.
+// Further down than 2^5 octaves lies at most 2^20 2^-32 in all, good to 4e-6, which is below 2^-30 (4096 units).
+constexpr double kTailError = 2.4e-6, kTailFar = 4300.0;
 constexpr int kGuess = 8;        // limits tried, 2.5 octaves of weight apart
 
 struct SampleParams {
@@ -966,7 +966,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) sample_kernel(const SampleParam
     }
     const uint32_t cabove = block_scan<NT>(csum, s.red, &ctotal);
     if (use_p) mabove = block_scan<NT>(msum, s.red64, &mtotal);
-    if (lkey > safe && (double)mtotal < (double)fmaxf(top_p, 0.f) * (double)(mtotal + tail_mass) * (1.0 + kTailError)) {
+    if (lkey > safe && (double)mtotal < (double)fmaxf(top_p, 0.f) * (double)(mtotal + tail_mass) * (1.0 + kTailError) + kTailFar) {
       lkey = safe;  // the cut lies below the limit after all
       continue;
     }
@@ -1062,7 +1062,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) sample_kernel(const SampleParam
           s.key = key;
           s.left = w ? (uint32_t)fmin(fmax(ceil(q), 1.0), (double)cnt) : cnt;
           // Too near to a border for the error of the weight below the limit: once more with the exact one.
-          s.again = !exact && fabs(q - rint(q)) * (double)w <= kTailError * (double)tail_mass ? 1u : 0u;
+          s.again = !exact && fabs(q - rint(q)) * (double)w <= kTailError * (double)tail_mass + kTailFar ? 1u : 0u;
         }
         __syncthreads();
         if (s.again) {
