@@ -422,6 +422,15 @@ def bench_distill(iters: int) -> None:
         _emit(f"distill_fwd [{M},{V}] K {K} tau {tau} alpha {alpha}", t, 2.0 * M * V + 10.0 * M * K, "GB/s", pk["hbm_gbs"])
         t = _time(lambda: ops.distill_bwd(x, ids, v, y, stats, grad, count, out=out, **kw), iters)
         _emit(f"distill_bwd [{M},{V}] K {K} tau {tau} alpha {alpha}", t, 4.0 * M * V + 10.0 * M * K, "GB/s", pk["hbm_gbs"])
+    # With the head's block statistics, as model.distill_loss has them: at temperature 1 a row's statistics and the logits at its
+    # slots and target (a sector of 32 bytes each) are read, at another one the logits too.
+    h, e = (torch.randn(n, 64, device="cuda", generator=g).half() for n in (M, V))
+    _, parts = ops.gemm_f16_ce_parts(h, e, out=x)
+    for tau, alpha in ((1.0, 1.0), (2.0, 0.7)):
+        kw = dict(temperature=tau, alpha=alpha, parts=parts)
+        t = _time(lambda: ops.distill_fwd(x, ids, v, y, stats=stats, row_loss=rows, **kw), iters)
+        work = 8.0 * M * ops.ce_parts_blocks(V) + 10.0 * M * K + (32.0 * M * (K + 1) if tau == 1.0 else 2.0 * M * V)
+        _emit(f"distill_fwd [{M},{V}] K {K} tau {tau} alpha {alpha}, head's statistics", t, work, "GB/s", pk["hbm_gbs"])
 
 
 def main() -> None:
