@@ -24,9 +24,10 @@ __device__ __forceinline__ float ex2(float x) {
 }
 
 // What a row's softmax at temperature 1 costs the forward next to the one at tau: nothing (kOne: tau = 1, alpha = 1 or given block
-// statistics), multiplications (tau = 2, 3, 4: exp(z) is a power of exp(z / tau); tau = 1.5: both are powers of exp(z / 3)) or
-// a second exponential (kBoth). The exponential unit takes 2000 cycles of an SM for 32000 logits where memory takes 2700,
-// so a second one would set the time (loss of 16384 x 32000: kBoth 271 us, kPow2 190 us, kPow1h 196 us, kOne 178 us; the
+// statistics), multiplications or a second exponential (kBoth). Multiplications do at temperatures a / b with a of 2 to 4 and b
+// of 1 or 2, where exp(z / tau) and exp(z) are the b-th and the a-th power of exp(z / a), two products each at most: tau = 2, 3,
+// 4, and 3 / 2. The exponential unit takes 2000 cycles of an SM for 32000 logits where memory takes 2700,
+// so a second one would set the time (loss of 16384 x 32000: kBoth 270 us, kPow2 187 us, kPow1h 194 us, kOne 175 us; the
 // logits' read alone is 160 us at the copy rate).
 enum Mode : int { kOne = 0, kBoth = 1, kPow2 = 2, kPow3 = 3, kPow4 = 4, kPow1h = 5 };
 
@@ -183,7 +184,8 @@ __device__ __forceinline__ double parts_lse(const float2* parts, int nblk, float
 }
 
 // Temperature 1 with the head's block statistics: the logits are read at the slots and the target only. One
-// warp per row.
+// warp per row. (16384 x 32000, K 64: 44 us; its 77 MB of statistics, ids, logits and gathered sectors are 12 us at the copy
+// rate, so latency sets it: a warp's loads of a row follow one another, logits at the slots after their ids.)
 constexpr int kPartWarps = 4;
 
 __global__ void __launch_bounds__(kPartWarps * 32) distill_parts_kernel(const Params p, float* __restrict__ row_loss,

@@ -42,8 +42,9 @@
 //             0 * garbage may be NaN. It alone touches V's slots: it waits for every fill of theirs in turn, so no wait
 //             can take an earlier fill for its own (with one warp for both products, its twelve products a tile, their waits and
 //             commits follow each other: 36.4 against 35.4 us at 64 rows of 32749 keys, 29.4 against 27.6 at one).
-// 64 sequences of 16 heads on a prefix of 32749, 1 to 1000 own tokens: 59 us, 4.5 TB/s; the prefix's tiles are bound by
-// the chain scores - exponents - exponentials - product of a tile (about 3300 cycles with two blocks an SM), not by memory.
+// 64 sequences of 16 heads on a prefix of 32749, 1 to 1000 own tokens: 63 us, 4.2 TB/s. The prefix's tiles are bound by
+// the chain scores - exponents - exponentials - product of a tile, not by memory: with one own token each 43.8 us, of which
+// about 4 are the join, for 4096 tiles in 296 blocks: 2.9 us a tile in a block, 1.4 us a tile and SM, as two blocks share one.
 #include <algorithm>
 #include <atomic>
 #include <type_traits>
@@ -722,9 +723,9 @@ __global__ void __launch_bounds__(128) attn_prefix_join_kernel(const Params p, i
 //
 // What bounds it is how many bytes are on their way: copies go to a ring of two 16-key steps a warp in shared memory
 // (loads straight to registers, a step at a time: 72.2 us for 64 sequences of 16 heads, up to 1000 own keys behind 32749;
-// rings of two, three and four steps 59.0, 59.8 and 73.8, since four leave too few blocks an SM). The own keys' share of
-// that is about 21 us, 6.3 TB/s. With four heads a key head it is bound by their instructions: 96 sequences of 32 heads,
-// up to 500 keys, 18.9 us.
+// rings of two, three and four steps 59.0, 59.8 and 73.8, since four leave too few blocks an SM; all with the prefix's P in
+// one fp16 number). Without a prefix the same sequences take 25.5 us, 5.2 TB/s. With four heads a key head it is bound by
+// their instructions: 96 sequences of 32 heads, up to 500 keys, add 18.9 us.
 constexpr int kOwnStages = 2, kOwnStage = 4096;  // bytes of 16 keys and values
 
 template <int G, int NT>
@@ -975,8 +976,8 @@ bool plan(int B, int H, int Hkv, int64_t prefix_len, int64_t max_len, Sched* s, 
   s->more = s->gp > 0 ? s->T % s->gp : 0;
   s->max_len = (int)max_len;
   // One block per pair reads few keys, or there are pairs enough to fill the GPU; up to four heads' state in registers.
-  // Four sequences of 16 heads, up to 1000 own keys behind 2000: 12.8 us plain, 13.6 as products; up to 2000 own keys
-  // 16.2 and 14.5. With 64 heads on the 16 and up to 1000 keys, 16 sequences: 24.8 and 21.5.
+  // Four sequences of 16 heads, up to 1000 own keys behind 2000: 11.9 us plain, 14.0 as products; up to 2000 own keys
+  // 15.3 and 15.3. With 64 heads on the 16, 16 sequences, up to 512 keys 21.0 and 20.3, up to 1000 keys 25.5 and 22.9.
   s->plain = s->G <= 4 && (max_len <= (s->G == 1 ? 1024 : 512) || (int64_t)B * Hkv >= blocks);
   // Enough items to even out ragged lengths, few parts to join.
   s->OC = (int)std::max<int64_t>(1, (own_all + 3 * blocks - 1) / (3 * blocks));

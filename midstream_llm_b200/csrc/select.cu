@@ -1272,7 +1272,7 @@ int launch_sample_as(const SampleParams& p, int64_t rows, cudaStream_t s) {
   return JX_OK;
 }
 
-// Short lists are worth the look where top-k or min-p may make them (one row of 32000 with all filters 15.7 -> 10.6 us, 20000
+// Short lists are worth the look where top-k or min-p may make them (one row of 32000 with all filters 15.7 -> 10.7 us, 20000
 // rows of 2000 483 -> 246). Where neither can, the code for them would only cost the long lists' loops registers (1024
 // rows of 50257 with top-p 199 -> 217 us).
 template <int NT>
@@ -1316,7 +1316,7 @@ extern "C" int jx_sample(const void* logits16, int64_t rows, int vocab, int64_t 
                       temperature, top_p, min_p, top_k, tokens, logprobs};
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   // Two blocks of 512 threads share an SM where there are rows for them, else a row gets 1024 (one row of 32000 with top-k
-  // and top-p: 10.6 us, 1024 rows of 50257 with top-p 198 us). Five small blocks where rows are short and
+  // and top-p: 10.7 us, 1024 rows of 50257 with top-p 178 us). Five small blocks where rows are short and
   // many waves of them come (20000 rows of 2000 with top-p 1026 -> 530 us; 400 rows of 4000 31 -> 43).
   if (rows > 8 * num_sms() && vocab <= sel::kShort) return sel::launch_sample<128>(p, rows, s);
   return rows > num_sms() ? sel::launch_sample<512>(p, rows, s) : sel::launch_sample<1024>(p, rows, s);
