@@ -232,7 +232,8 @@ int jx_attn_decode_prefix(const void* qkv, int64_t ld_qkv, const void* kprefix, 
  * whole sum; uniforms f32 in [0, 1). T <= 0 takes the lowest index of the maximum. Each setting is one value for
  * all rows or, where its pointer is not NULL, a device array of one per row. tokens int64 [rows]; logprobs f32
  * [rows] (may be NULL): log of the token's share of the kept sum. A row with a NaN, or whose logits are all -inf,
- * gives token -1 and a NaN. Probabilities are held in 64 bits and results repeat bit for bit. vocab <= 2^20. */
+ * gives token -1 and a NaN. Each e is held as an integer number of 2^-42, so one below 2^-43 counts as 0 and is never drawn;
+ * sums are exact in 64 bits and results repeat bit for bit. vocab <= 2^20. */
 int jx_sample(const void* logits16, int64_t rows, int vocab, int64_t ld, const float* uniforms,
               const float* temperatures, float temperature, const int32_t* top_ks, int top_k, const float* top_ps,
               float top_p, const float* min_ps, float min_p, int64_t* tokens, float* logprobs, jx_stream_t stream);

@@ -445,7 +445,8 @@ def sample(logits16: torch.Tensor, uniforms: torch.Tensor, temperature: float | 
     returns (tokens int64 [rows], logprobs f32 [rows]). Temperature, then top-k, then top-p over what top-k left,
     then min-p (relative to the largest probability); among equal logits the lower index ranks first. temperature
     0 is greedy; top_k 0, top_p 1 and min_p 0 are off. Each setting is a number, or a device tensor with one value
-    per row (f32; top_k int32). A row with a NaN or without a finite logit gives token -1 and a NaN."""
+    per row (f32; top_k int32). Probabilities are held to 2^-43 of the largest; a token below that is never drawn. A row with a
+    NaN, or with nothing but -inf, gives token -1 and a NaN."""
     rows, vocab, ld = _logit_rows(logits16, "logits16")
     here = [logits16, uniforms]
     _check(uniforms, F32, "uniforms")
