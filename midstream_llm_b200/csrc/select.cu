@@ -1273,9 +1273,9 @@ int launch_sample_as(const SampleParams& p, int64_t rows, cudaStream_t s) {
   return JX_OK;
 }
 
-// Short lists are worth the look where top-k or min-p may make them (one row of 32000 with all filters 15.7 -> 10.7 us, 20000
-// rows of 2000 483 -> 246). Where neither can, the code for them would only cost the long lists' loops registers (1024
-// rows of 50257 with top-p 199 -> 217 us).
+// Short lists are worth the look where top-k or min-p may make them (one row of 32000 with all filters 15.7 -> 10.6 us, 20000
+// rows of 2000 with top-k 680 -> 204). Where neither can, the code for them would only cost the long lists' loops registers
+// (1024 rows of 50257 with top-p 170 -> 171 us).
 template <int NT>
 int launch_sample(const SampleParams& p, int64_t rows, cudaStream_t s) {
   return p.top_k || p.top_k_s > 0 || p.min_p || p.min_p_s > 0.f ? launch_sample_as<NT, true>(p, rows, s)
@@ -1318,7 +1318,7 @@ extern "C" int jx_sample(const void* logits16, int64_t rows, int vocab, int64_t 
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   // Two blocks of 512 threads share an SM where there are rows for them, else a row gets 1024 (one row of 32000 with top-k
   // and top-p: 10.7 us, 1024 rows of 50257 with top-p 170 us). Five small blocks where rows are short and
-  // many waves of them come (20000 rows of 2000 with top-p 1026 -> 530 us; 400 rows of 4000 31 -> 43).
+  // many waves of them come (20000 rows of 2000 with top-p 1070 -> 527 us; 600 rows of 4000 with settings row by row 38 -> 46).
   if (rows > 8 * num_sms() && vocab <= sel::kShort) return sel::launch_sample<128>(p, rows, s);
   return rows > num_sms() ? sel::launch_sample<512>(p, rows, s) : sel::launch_sample<1024>(p, rows, s);
 }
