@@ -41,7 +41,8 @@
 //   warp 6    issues the second products, and puts the new value into such a tile and clears what is behind it, since
 //             0 * garbage may be NaN. It alone touches V's slots: it waits for every fill of theirs in turn, so no wait
 //             can take an earlier fill for its own (with one warp for both products, its twelve products a tile, their waits and
-//             commits follow each other: 36.4 against 35.4 us at 64 rows of 32749 keys, 29.4 against 27.6 at one).
+//             commits follow each other: 36.4 against 35.4 us at 64 rows of 32749 keys, 29.4 against 27.6 at one, with P in
+//             one fp16 number).
 // 64 sequences of 16 heads on a prefix of 32749, 1 to 1000 own tokens: 63 us, 4.2 TB/s. The prefix's tiles are bound by
 // the chain scores - exponents - exponentials - product of a tile, not by memory: with one own token each 43.8 us, of which
 // about 4 are the join, for 4096 tiles in 296 blocks: 2.9 us a tile in a block, 1.4 us a tile and SM, as two blocks share one.
@@ -1107,7 +1108,7 @@ extern "C" int jx_attn_decode_prefix(const void* qkv, int64_t ld_qkv, const void
   cfg.dynamicSmemBytes = 0;
   if (p.s.plain) {
     // Eight warps share the keys of a pair where four would leave SMs empty (256 pairs of up to 257 keys behind 1791:
-    // 12.1 -> 11.1 us; 1024 pairs of up to 1000 58.8 -> 59.8).
+    // 12.0 -> 11.2 us; 1024 pairs of up to 1000 62.6 either way).
     const int NT = max_len > 128 && B * Hkv < 2 * num_sms() ? 256 : 128;
     cfg.gridDim = dim3(B * Hkv);
     cfg.blockDim = dim3(NT);
